@@ -1,6 +1,7 @@
 """Torch-tensor front end of the C-ABI (include/dppm_hip.h).  torch is used only as the owner of device memory and
 of the current HIP stream; every function validates its operands on the host (shape, dtype, device, contiguity)
 before a raw pointer reaches a kernel, and raises RuntimeError on a non-zero status.  No CPU path exists."""
+import bisect
 import contextlib
 import ctypes as C
 
@@ -12,6 +13,18 @@ from ._lib import PRECISIONS, PpgnLayer, PpgnParams, check, lib
 
 def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _on(device):
+    """Context in which a launch goes to `device` and its current stream, whichever device is current."""
+    return _NO_CONTEXT if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+_NO_CONTEXT = contextlib.nullcontext()
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _chk(t, name, shape=None, dtype=torch.float32):
@@ -380,6 +393,135 @@ def adam_step(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, weight_de
         _chk(t, n, (param.numel(),))
     check(lib.dppm_adam_step(_ptr(param), _ptr(grad), _ptr(exp_avg), _ptr(exp_avg_sq), C.c_size_t(param.numel()), lr, beta1,
                              beta2, eps, weight_decay, int(step), grad_scale, _stream()), "dppm_adam_step")
+
+
+STATE_BLOCK = 256      # values of a tensor that share one scale of its 8-bit moments (include/dppm_hip.h, dppm_tensor_entry)
+
+
+class TensorSet:
+    """The tensors of one AdamW step, laid out once: a device table of their addresses, and their moments in flat buffers.
+
+    params: contiguous float32 tensors on one GPU, 16-byte aligned, none overlapping another; grads: one for each, all float32 or all
+    bfloat16, same number of values; copies: None, or for each parameter a bfloat16 tensor (or None) that every step writes the new
+    parameter to.  weight_decay: one number, or one for each tensor.  state_bits: 32 (float32 moments) or 8 (e4m3 of m and of sqrt(v)
+    with a float32 scale per 256 values).  state: buffers as in self.state to go on from; zeros if None.
+    The set keeps its tensors alive; set_grads() points it at other gradients.  Moments of tensor i lie at self.offsets[i] of the flat
+    buffers (offsets are multiples of 256 values)."""
+
+    def __init__(self, params, grads, copies=None, weight_decay=0.0, state_bits=32, state=None):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits {state_bits}: expected 8 or 32")
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("TensorSet: no tensors")
+        n = len(self.params)
+        for i, p in enumerate(self.params):
+            _chk(p, f"params[{i}]")
+            if p.device != self.params[0].device:
+                raise ValueError(f"params[{i}]: on {p.device}, params[0] on {self.params[0].device}")
+        self.copies = [None] * n if copies is None else list(copies)
+        self.weight_decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        for name, v in (("copies", self.copies), ("weight_decay", self.weight_decay)):
+            if len(v) != n:
+                raise ValueError(f"{name}: {len(v)} entries for {n} tensors")
+        for i, c in enumerate(self.copies):
+            if c is not None:
+                _chk(c, f"copies[{i}]", None, torch.bfloat16)
+        self.device = self.params[0].device
+        self.state_bits = state_bits
+        sizes = [p.numel() for p in self.params]
+        self.offsets = np.concatenate([[0], np.cumsum([(s + STATE_BLOCK - 1) // STATE_BLOCK * STATE_BLOCK for s in sizes])]).tolist()
+        self.state = self._state(state)
+        per = lib.dppm_adamw_chunk()
+        counts = np.asarray([(s + per - 1) // per for s in sizes], dtype=np.int64)
+        if counts.sum() > 2 ** 31 - 1:
+            raise ValueError("TensorSet: too many values")
+        which = np.repeat(np.arange(n, dtype=np.int64), counts)
+        chunk = np.arange(counts.sum(), dtype=np.int64) - np.repeat(np.cumsum(counts) - counts, counts)
+        self.chunks = torch.as_tensor(np.stack([which, chunk], 1).astype(np.int32), device=self.device)
+        self.n_chunks = self.chunks.shape[0]
+        self.table = torch.empty(n, 9, device=self.device, dtype=torch.int64)
+        self.workspace = torch.empty(lib.dppm_adamw_workspace_bytes() // 8, device=self.device, dtype=torch.float64)
+        self.set_grads(grads)
+
+    def _state(self, given):
+        total = self.offsets[-1]
+        if self.state_bits == 32:
+            want = {"exp_avg": (total, torch.float32), "exp_avg_sq": (total, torch.float32)}
+        else:
+            want = {"exp_avg": (total, torch.float8_e4m3fn), "exp_avg_scale": (total // STATE_BLOCK, torch.float32),
+                    "exp_avg_root": (total, torch.float8_e4m3fn), "exp_avg_root_scale": (total // STATE_BLOCK, torch.float32)}
+        if given is None:
+            return {k: torch.zeros(s, device=self.device, dtype=torch.float32).to(t) for k, (s, t) in want.items()}
+        if set(given) != set(want):
+            raise ValueError(f"state: buffers {sorted(given)}, expected {sorted(want)}")
+        for k, (s, t) in want.items():
+            if _chk(given[k], f"state[{k!r}]", (s,), t).device != self.device:
+                raise ValueError(f"state[{k!r}]: on {given[k].device}, the parameters on {self.device}")
+        return dict(given)
+
+    def _refuse_shared(self, grads):
+        """No byte that a step writes belongs to two tensors, or to a gradient: reads and writes of different workgroups would race."""
+        def span(t):
+            return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+        spans = sorted(span(t) for t in [*self.params, *(c for c in self.copies if c is not None), *self.state.values()] if t.numel())
+        ends = [e for _, e in spans]
+        if any(begin < end for end, (begin, _) in zip(ends, spans[1:])):
+            raise ValueError("TensorSet: two of the tensors share memory")
+        for i, g in enumerate(grads):
+            begin, end = span(g)
+            at = bisect.bisect_right(ends, begin)                 # the first written span that ends behind the gradient's begin
+            if begin < end and at < len(spans) and spans[at][0] < end:
+                raise ValueError(f"grads[{i}]: shares memory with a tensor that the step writes")
+
+    def set_grads(self, grads):
+        """Points the set at these gradients (and lays its table out again: one small upload)."""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError(f"grads: {len(grads)} tensors for {len(self.params)} parameters")
+        kind = grads[0].dtype if isinstance(grads[0], torch.Tensor) else None
+        if kind not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"grads[0]: dtype {kind}, expected float32 or bfloat16")
+        rows = []
+        eight = self.state_bits == 8
+        m, v = self.state["exp_avg"], self.state["exp_avg_root" if eight else "exp_avg_sq"]
+        for i, (p, g, c, off) in enumerate(zip(self.params, grads, self.copies, self.offsets)):
+            _chk(g, f"grads[{i}]", None, kind)
+            for t, name, align in ((p, "params", 16), (g, "grads", 4 * g.element_size()), (c, "copies", 8)):
+                if t is None:
+                    continue
+                if t.numel() != p.numel() or t.device != self.device:
+                    raise ValueError(f"{name}[{i}]: {t.numel()} values on {t.device}, the parameter {p.numel()} on {self.device}")
+                if t.data_ptr() % align:
+                    raise ValueError(f"{name}[{i}]: not aligned to {align} bytes")
+            scales = [self.state[k + "_scale"].data_ptr() + off // STATE_BLOCK * 4 for k in ("exp_avg", "exp_avg_root")] if eight else [0, 0]
+            decay = int(np.float64(self.weight_decay[i]).view(np.int64))
+            rows.append([p.data_ptr(), g.data_ptr(), 0 if c is None else c.data_ptr(), m.data_ptr() + off * m.element_size(),
+                         v.data_ptr() + off * v.element_size(), *scales, p.numel(), decay])
+        self._refuse_shared(grads)
+        self.grads = grads
+        self.grad_bf16 = kind == torch.bfloat16
+        self.table.copy_(torch.as_tensor(np.asarray(rows, dtype=np.int64)))
+
+
+def adamw_step(tensors, lr, beta1, beta2, eps, step, max_norm=None, grad_scale=1.0, seed=0):
+    """One AdamW step over a TensorSet: parameters, moments and copies are updated in place (include/dppm_hip.h, dppm_adamw_step).
+    max_norm: clip the norm of all gradients together to it; then the norm before clipping is returned (float32, 0-d, on the device),
+    and a step whose norm is infinite or NaN changes nothing.  Without it returns None, and such gradients reach the parameters.
+    seed: key of the random bits that round 8-bit moments.  A captured call replays the step number it was captured with."""
+    if not isinstance(tensors, TensorSet):
+        raise TypeError(f"tensors: expected a TensorSet, got {type(tensors)}")
+    if max_norm is not None and not max_norm > 0:
+        raise ValueError(f"max_norm {max_norm}: expected a positive number or None")
+    s = tensors
+    with _on(s.device):
+        norm = torch.empty((), device=s.device, dtype=torch.float32) if max_norm is not None else None
+        check(lib.dppm_adamw_step(s.table.data_ptr(), s.chunks.data_ptr(), s.n_chunks, s.grad_bf16, s.state_bits, lr, beta1, beta2, eps,
+                                  int(step), grad_scale, 0.0 if norm is None else float(max_norm), int(seed) & (2 ** 64 - 1),
+                                  None if norm is None else norm.data_ptr(), s.workspace.data_ptr(), s.workspace.numel() * 8,
+                                  _raw_stream(s.device)), "dppm_adamw_step")
+    return norm
 
 
 # ------------------------------------------------------------------------------------------------- graph statistics

@@ -264,6 +264,32 @@ int dppm_adam_step(float* param, const float* grad, float* exp_avg, float* exp_a
                    float lr, float beta1, float beta2, float eps, float weight_decay, int step, float grad_scale,
                    void* stream);
 
+/* One tensor of an AdamW step: an entry of the DEVICE table dppm_adamw_step reads.  param float32 (16-byte aligned); grad float32 or
+ * bfloat16 (16 / 8-byte aligned); copy (nullable): bfloat16 working weights, written from the new param (8-byte aligned).
+ * 32-bit moments: exp_avg / exp_avg_sq float32 [numel] (16-byte aligned), scales unused.
+ * 8-bit moments: exp_avg holds m, exp_avg_sq holds sqrt(v), both OCP e4m3 codes [numel rounded up to 256] (4-byte aligned), value =
+ * code * scale with one float32 scale per 256 values. */
+typedef struct dppm_tensor_entry {
+  float* param; const void* grad; uint16_t* copy;
+  void* exp_avg; void* exp_avg_sq; float* exp_avg_scale; float* exp_avg_sq_scale;
+  int64_t numel;
+  double weight_decay;
+} dppm_tensor_entry;
+
+/* One AdamW step (decoupled weight decay, bias correction with `step` starting at 1) over all tensors of `table`, in one launch, or in
+ * three with max_norm > 0: then the gradients' norm over all tensors (of grad * grad_scale) goes to *norm_out, the gradients are scaled
+ * by min(1, max_norm / (norm + 1e-6)), and a step whose norm is infinite or NaN changes nothing.
+ * chunks: DEVICE array [n_chunks][2] of (index in table, chunk in that tensor), one pair for each dppm_adamw_chunk() values begun of
+ * every tensor.  state_bits 8 or 32; 8-bit moments are rounded stochastically from Philox4x32-10 with key = seed and counter =
+ * (g, tensor, g >> 32, step), g = index / 4: the same call gives the same bits, and a captured call replays the step number and the
+ * random bits it was captured with.  Tensors must not overlap.  workspace: dppm_adamw_workspace_bytes(), read with max_norm > 0 only;
+ * calls that may run at the same time need their own.  No counterpart in the reference (its optimizer: ppgn_simple.py:259-262). */
+int dppm_adamw_chunk(void);
+size_t dppm_adamw_workspace_bytes(void);
+int dppm_adamw_step(const dppm_tensor_entry* table, const int32_t* chunks, int n_chunks, int grad_bf16, int state_bits, double lr,
+                    double beta1, double beta2, double eps, int step, double grad_scale, double max_norm, uint64_t seed,
+                    float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------------
  * Graph statistics for model selection (the step after sampling; the reference does it with networkx / pyemd on the CPU)
  * ---------------------------------------------------------------------------------------------- */

@@ -1,0 +1,49 @@
+"""CPU checks of the operators for categorical states: what their C entry points and Python front ends refuse before anything reaches a
+GPU, and the plain forms of oracle/classes.py against torch's autograd and optimizer in float64."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from discrete_dppm_graphs_amd import ops
+from discrete_dppm_graphs_amd._lib import lib
+from oracle import classes
+
+
+def test_adamw_oracle_is_torch_adamw():
+    rng = np.random.default_rng(0)
+    p = torch.as_tensor(rng.normal(size=50))
+    t = p.clone().requires_grad_(True)
+    opt = torch.optim.AdamW([t], lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+    q, m, v = p.numpy(), np.zeros(50), np.zeros(50)
+    for step in range(1, 5):
+        g = rng.normal(size=50)
+        t.grad = torch.as_tensor(g)
+        opt.step()
+        q, m, v = classes.adamw(q, g, m, v, 1e-2, 0.9, 0.999, 1e-8, step, 0.1)
+    np.testing.assert_allclose(q, t.detach().numpy(), rtol=1e-12)
+
+
+def test_e4m3_neighbours_hold_the_value():
+    x = np.random.default_rng(1).normal(size=1000) * np.repeat([1e-20, 1e-3, 1.0, 1e20], 250)
+    scale, low, high, part = classes.e4m3_neighbours(x)
+    assert (np.abs(low) <= np.abs(x) * (1 + 1e-12)).all() and (np.abs(x) <= np.abs(high)).all() and (part >= 0).all() and (part < 1).all()
+    s = torch.as_tensor(np.repeat(scale, 256)[:1000])
+    for y in (low, high):
+        q = (torch.as_tensor(np.abs(y)) / s).clamp(max=448.0)      # above a block's largest value there is no neighbour
+        assert torch.equal(q.float().to(torch.float8_e4m3fn).float(), q.float())
+
+
+def test_adamw_entry_refuses():
+    one = C.c_void_p(16)      # refused before any pointer is read
+    good = dict(table=one, chunks=one, n=1, bf=0, bits=32, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, step=1, gs=1.0, mn=0.0, seed=0, norm=None, ws=None, wb=0, st=None)
+    for bad in ({"table": None}, {"chunks": None}, {"n": -1}, {"bits": 4}, {"b1": 1.0}, {"b2": -0.1}, {"eps": -1.0}, {"step": 0}, {"b1": float("nan")},
+                {"mn": 1.0}, {"mn": 1.0, "norm": one, "ws": one, "wb": 64}):
+        assert lib.dppm_adamw_step(*{**good, **bad}.values()) == -1, bad
+    assert lib.dppm_adamw_chunk() % 256 == 0 and lib.dppm_adamw_workspace_bytes() > 0
+
+
+def test_front_ends_refuse_cpu_tensors():
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.TensorSet([torch.zeros(4)], [torch.zeros(4)])
