@@ -84,6 +84,10 @@ SIGNATURES = {
     "dppm_debug_get": (C.c_int, [C.c_char_p, C.POINTER(C.c_int)]),
     "dppm_adam_step": (C.c_int, [c_f32p, c_f32p, c_f32p, c_f32p, C.c_size_t, C.c_float, C.c_float, C.c_float, C.c_float,
                                  C.c_float, C.c_int, C.c_float, c_stream]),
+    "dppm_embedding_fwd": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_float, C.c_void_p] + [C.c_int64] * 3 + [c_stream]),
+    "dppm_embedding_wgrad_workspace_bytes": (C.c_size_t, [C.c_int64] * 3),
+    "dppm_embedding_wgrad": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_float, C.c_void_p, C.c_int, C.c_int] + [C.c_int64] * 3
+                             + [C.c_void_p, C.c_size_t, c_stream]),
     "dppm_adamw_chunk": (C.c_int, []),
     "dppm_adamw_workspace_bytes": (C.c_size_t, []),
     "dppm_adamw_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int] + [C.c_double] * 4 + [C.c_int, C.c_double, C.c_double,

@@ -1,0 +1,542 @@
+// A table of classes: out[t] = scale * W[id_t], and its gradient dW[v] = scale * sum over t with id_t = v of dout[t].
+// An id outside [0, V) stands for no class (a padded position): its row of `out` is zero and it adds nothing to any gradient.
+//
+// Both are HBM-bound.  The lookup reads and writes each row once, 16 bytes a lane.  The gradient sorts the positions by class (a stable
+// radix sort of (class, position) pairs), so that the rows of one class lie together and are summed in the order of their positions in
+// float32 registers: no atomics, the same bits from call to call, and one write per row of dW.  A class with many positions is split over
+// fixed chunks of the sorted order, whose partial rows a second launch joins, again in order.
+#include "dppm_common.h"
+
+namespace dppm {
+namespace {
+
+template <class T> using glb = __attribute__((address_space(1))) T*;
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {   // round to nearest even (v_cvt_pk_bf16_f32)
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
+}
+__device__ __forceinline__ uint16_t to_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// VEC values from / to memory, as float32.  VEC > 1: 16 bytes of the input's type, aligned.
+template <bool BF, int VEC>
+__device__ __forceinline__ void load_vec(const void* src, long at, float (&v)[VEC]) {
+  if constexpr (BF && VEC == 8) {
+    const u32x4 w = *(glb<const u32x4>)((glb<const uint16_t>)src + at);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { v[2 * k] = bf16_lo(w[k]); v[2 * k + 1] = bf16_hi(w[k]); }
+  } else if constexpr (BF) {
+    static_assert(VEC == 1, "");
+    v[0] = bf16_lo(((glb<const uint16_t>)src)[at]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) {
+      if constexpr (VEC >= 4) {
+        const f32x4 w = *(glb<const f32x4>)((glb<const float>)src + at + k);
+        v[k] = w.x; v[k + 1] = w.y; v[k + 2] = w.z; v[k + 3] = w.w;
+      } else v[0] = ((glb<const float>)src)[at];
+    }
+  }
+}
+template <bool BF, int VEC>
+__device__ __forceinline__ void store_vec(void* dst, long at, const float (&v)[VEC]) {
+  if constexpr (BF) {
+    const glb<uint16_t> q = (glb<uint16_t>)dst + at;
+    if constexpr (VEC == 8) *(glb<u32x4>)q = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+    else if constexpr (VEC == 4) *(glb<u32x2>)q = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    else *q = to_bf16(v[0]);
+  } else {
+    const glb<float> q = (glb<float>)dst + at;
+    if constexpr (VEC == 1) *q = v[0];
+    else {
+#pragma unroll
+      for (int k = 0; k < VEC; k += 4) *(glb<f32x4>)(q + k) = f32x4{v[k], v[k + 1], v[k + 2], v[k + 3]};
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ lookup
+// `tpr` threads (a power of two, at most 256) walk a row; a workgroup holds 256 / tpr rows at a time and four such groups, whose loads
+// are issued together.
+constexpr int FWD_ROWS = 4;
+template <bool BF, int VEC>
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__ w, const int64_t* __restrict__ ids, float scale, void* __restrict__ out,
+                                                        long T, long V, int D, int tpr_log2) {
+  const int tpr = 1 << tpr_log2, rpb = 256 >> tpr_log2, lane = threadIdx.x & (tpr - 1);
+  const long t0 = (long)blockIdx.x * rpb * FWD_ROWS + (threadIdx.x >> tpr_log2);
+  long id[FWD_ROWS];
+#pragma unroll
+  for (int r = 0; r < FWD_ROWS; ++r) {
+    const long t = t0 + r * rpb;
+    const long i = t < T ? ids[t] : -1;
+    id[r] = i < V ? i : -1;
+  }
+  for (int c = lane * VEC; c < D; c += tpr * VEC) {
+    float v[FWD_ROWS][VEC];
+#pragma unroll
+    for (int r = 0; r < FWD_ROWS; ++r) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[r][k] = 0.f;
+      if (id[r] >= 0) load_vec<BF, VEC>(w, id[r] * D + c, v[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < FWD_ROWS; ++r) {
+      const long t = t0 + r * rpb;
+      if (t < T) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[r][k] *= scale;
+        if (id[r] < 0) {   // 0 * scale would be NaN for an infinite scale
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) v[r][k] = 0.f;
+        }
+        store_vec<BF, VEC>(out, t * D + c, v[r]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sorting positions by class
+// Least significant digit first, 8 bits a pass: count the digits of every tile, then place every pair at
+//   (pairs with a smaller digit) + (pairs with the digit in earlier tiles) + (rank among the tile's pairs with the digit),
+// which keeps the order of equal digits.  Classes without a row sort behind all others as class V.
+constexpr int DIGITS = 256, PER_THREAD = 8;
+constexpr int MAX_TILES = 128;                 // every tile's placement reads the counts of all
+constexpr int ONE_TILE = 8192;                 // up to here one workgroup of 1024 threads sorts alone, in one launch
+
+struct SortBufs { uint32_t *key[2], *pos[2]; };
+
+__device__ __forceinline__ uint32_t class_key(const int64_t* ids, long t, long V) {
+  const long i = ids[t];
+  return (uint32_t)((i >= 0 && i < V) ? i : V);
+}
+
+template <int NT>
+struct RankShared { uint32_t cnt[NT / 64][DIGITS]; uint32_t base[DIGITS]; uint32_t scan[DIGITS]; };
+
+// Places NT * PER_THREAD consecutive pairs (those before `n`).  s.base[d]: where the next pair with digit d goes; moved on for the next call.
+// A wave takes 64 * PER_THREAD consecutive pairs, 64 at a time; lanes with the same digit are found with one ballot per bit.
+template <int NT, bool FIRST>
+__device__ __forceinline__ void place(RankShared<NT>& s, const int64_t* ids, long V, const uint32_t* key_in, const uint32_t* pos_in, uint32_t* key_out,
+                                      uint32_t* pos_out, long begin, long n, int shift) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int i = threadIdx.x; i < (NT / 64) * DIGITS; i += NT) (&s.cnt[0][0])[i] = 0;
+  __syncthreads();
+  uint32_t key[PER_THREAD], pos[PER_THREAD], rank[PER_THREAD];
+  const long at0 = begin + (long)wave * 64 * PER_THREAD + lane;
+#pragma unroll
+  for (int r = 0; r < PER_THREAD; ++r) {
+    const long at = at0 + r * 64;
+    key[r] = 0; pos[r] = 0;
+    if (at < n) {
+      if (FIRST) { key[r] = class_key(ids, at, V); pos[r] = (uint32_t)at; }
+      else { key[r] = key_in[at]; pos[r] = pos_in[at]; }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < PER_THREAD; ++r) {
+    const bool in = at0 + r * 64 < n;
+    const uint32_t d = (key[r] >> shift) & (DIGITS - 1);
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const uint64_t one = __ballot((d >> b) & 1u);
+      same &= ((d >> b) & 1u) ? one : ~one;
+    }
+    const uint64_t before = same & ((1ull << lane) - 1ull);
+    uint32_t seen = 0;
+    if (in) seen = s.cnt[wave][d];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    rank[r] = seen + __popcll(before);
+    if (in && before == 0) s.cnt[wave][d] = seen + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();
+  if (threadIdx.x < DIGITS) {   // per digit: where each wave's pairs begin
+    uint32_t b = s.base[threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+      const uint32_t c = s.cnt[w][threadIdx.x];
+      s.cnt[w][threadIdx.x] = b;
+      b += c;
+    }
+    s.base[threadIdx.x] = b;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < PER_THREAD; ++r)
+    if (at0 + r * 64 < n) {
+      const uint32_t to = s.cnt[wave][(key[r] >> shift) & (DIGITS - 1)] + rank[r];
+      key_out[to] = key[r];
+      pos_out[to] = pos[r];
+    }
+  __syncthreads();
+}
+
+// exclusive prefix sum of s.scan over the digits, into s.scan; called by every thread
+template <int NT>
+__device__ __forceinline__ void scan_digits(RankShared<NT>& s) {
+  __syncthreads();
+  uint32_t own = 0;
+  if (threadIdx.x < DIGITS) own = s.scan[threadIdx.x];
+  for (int o = 1; o < DIGITS; o <<= 1) {
+    uint32_t add = 0;
+    if (threadIdx.x < DIGITS && (int)threadIdx.x >= o) add = s.scan[threadIdx.x - o];
+    __syncthreads();
+    if (threadIdx.x < DIGITS) s.scan[threadIdx.x] += add;
+    __syncthreads();
+  }
+  if (threadIdx.x < DIGITS) s.scan[threadIdx.x] -= own;
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(1024) void sort_one_kernel(const int64_t* __restrict__ ids, long T, long V, int passes, SortBufs b) {
+  __shared__ RankShared<1024> s;
+  for (int p = 0; p < passes; ++p) {
+    const uint32_t *ki = b.key[(p + 1) & 1], *pi = b.pos[(p + 1) & 1];
+    uint32_t *ko = b.key[p & 1], *po = b.pos[p & 1];
+    if (threadIdx.x < DIGITS) s.scan[threadIdx.x] = 0;
+    __syncthreads();
+    for (long t = threadIdx.x; t < T; t += 1024) {
+      const uint32_t k = p == 0 ? class_key(ids, t, V) : ki[t];
+      atomicAdd(&s.scan[(k >> (8 * p)) & (DIGITS - 1)], 1u);
+    }
+    scan_digits(s);
+    if (threadIdx.x < DIGITS) s.base[threadIdx.x] = s.scan[threadIdx.x];
+    __syncthreads();
+    for (long t = 0; t < T; t += 1024 * PER_THREAD) {
+      if (p == 0) place<1024, true>(s, ids, V, ki, pi, ko, po, t, T, 8 * p);
+      else place<1024, false>(s, ids, V, ki, pi, ko, po, t, T, 8 * p);
+    }
+  }
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ key, long T, long V, int shift, long tile,
+                                                         uint32_t* __restrict__ hist) {
+  __shared__ uint32_t h[DIGITS];
+  h[threadIdx.x] = 0;
+  __syncthreads();
+  const long begin = blockIdx.x * tile, end = begin + tile < T ? begin + tile : T;
+  for (long t = begin + threadIdx.x; t < end; t += 256) atomicAdd(&h[((FIRST ? class_key(ids, t, V) : key[t]) >> shift) & (DIGITS - 1)], 1u);
+  __syncthreads();
+  hist[blockIdx.x * DIGITS + threadIdx.x] = h[threadIdx.x];
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(256) void sort_place_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ key_in, const uint32_t* __restrict__ pos_in,
+                                                         uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out, long T, long V, int shift, long tile,
+                                                         const uint32_t* __restrict__ hist) {
+  __shared__ RankShared<256> s;
+  uint32_t all = 0, earlier = 0;
+#pragma unroll 8
+  for (int t = 0; t < (int)gridDim.x; ++t) {
+    const uint32_t c = hist[t * DIGITS + threadIdx.x];
+    all += c;
+    if (t < (int)blockIdx.x) earlier += c;
+  }
+  s.scan[threadIdx.x] = all;
+  scan_digits(s);
+  s.base[threadIdx.x] = s.scan[threadIdx.x] + earlier;
+  __syncthreads();
+  const long begin = blockIdx.x * tile, end = begin + tile < T ? begin + tile : T;
+  for (long t = begin; t < end; t += 256 * PER_THREAD) place<256, FIRST>(s, ids, V, key_in, pos_in, key_out, pos_out, t, end, shift);
+}
+
+// ------------------------------------------------------------------------------------------------ sums of sorted rows
+struct SumArgs {
+  const void* dout;
+  const uint32_t *key, *pos;
+  void* dw;
+  float* part;           // [chunks][2][pitch]: sums of a chunk's run that began in an earlier chunk (0), of one that goes on in the next (1)
+  long T, V;
+  int D, pitch, cp, lanes_log2, slices, accumulate;
+  float scale;
+};
+
+template <bool OBF, int VEC>
+__device__ __forceinline__ void finish_row(const SumArgs& a, uint32_t k, int c, float (&acc)[VEC]) {
+  const long at = (long)k * a.D + c;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] *= a.scale;
+  if (a.accumulate) {
+    if constexpr (VEC == 4 && OBF) {   // 8 bytes of bfloat16
+      const u32x2 w = *(glb<const u32x2>)((glb<const uint16_t>)a.dw + at);
+      acc[0] += bf16_lo(w.x); acc[1] += bf16_hi(w.x); acc[2] += bf16_lo(w.y); acc[3] += bf16_hi(w.y);
+    } else {
+      float old[VEC];
+      load_vec<OBF, VEC>(a.dw, at, old);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += old[i];
+    }
+  }
+  store_vec<OBF, VEC>(a.dw, at, acc);
+}
+
+// One group of `lanes` lanes sums the rows of `cp` consecutive sorted positions over lanes * VEC columns.  Workgroups behind those
+// write zeros to the rows that have no position (found by bisection: the sorted classes are in L2).
+constexpr int FILL_ROWS = 64;
+template <bool IBF, bool OBF, int VEC>
+__global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a, int sum_blocks) {
+  if ((int)blockIdx.x >= sum_blocks) {
+    __shared__ int absent[FILL_ROWS];
+    const long r0 = (long)((int)blockIdx.x - sum_blocks) * FILL_ROWS;
+    if (threadIdx.x < FILL_ROWS) {
+      const long row = r0 + threadIdx.x;
+      long lo = 0, hi = a.T;
+      while (lo < hi) {
+        const long mid = (lo + hi) >> 1;
+        if ((long)a.key[mid] < row) lo = mid + 1;
+        else hi = mid;
+      }
+      absent[threadIdx.x] = row < a.V && !(lo < a.T && (long)a.key[lo] == row);
+    }
+    __syncthreads();
+    float zero[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) zero[i] = 0.f;
+    const int lane = threadIdx.x & 63;
+    for (int r = threadIdx.x >> 6; r < FILL_ROWS; r += 4)
+      if (absent[r])
+        for (int c = lane * VEC; c < a.D; c += 64 * VEC) store_vec<OBF, VEC>(a.dw, (r0 + r) * a.D + c, zero);
+    return;
+  }
+  const int lanes = 1 << a.lanes_log2;
+  const long group = (long)blockIdx.x * (256 >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
+  const long chunk = group / a.slices;
+  const int c = ((int)(group - chunk * a.slices) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
+  const long p0 = chunk * a.cp;
+  if (p0 >= a.T || c >= a.D) return;
+  const long p1 = p0 + a.cp < a.T ? p0 + a.cp : a.T;
+  const uint32_t none = (uint32_t)a.V;
+  const uint32_t before = p0 > 0 ? a.key[p0 - 1] : none, behind = p1 < a.T ? a.key[p1] : none;
+  float acc[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+  uint32_t cur = none;
+  bool first = true;    // whether the current run is the chunk's first
+  const auto flush = [&](bool last) {
+    if (cur == none) return;
+    if (first && cur == before) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) a.part[(chunk * 2) * a.pitch + c + i] = acc[i];
+    } else if (last && cur == behind) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) a.part[(chunk * 2 + 1) * a.pitch + c + i] = acc[i];
+    } else finish_row<OBF, VEC>(a, cur, c, acc);
+  };
+  constexpr int AHEAD = 8;
+  for (long p = p0; p < p1; p += AHEAD) {
+    uint32_t k[AHEAD];
+    float v[AHEAD][VEC];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const bool in = p + u < p1;
+      k[u] = in ? a.key[p + u] : none;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[u][i] = 0.f;
+      if (k[u] != none) load_vec<IBF, VEC>(a.dout, (long)a.pos[p + u] * a.D + c, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (p + u < p1 && k[u] != cur) {
+        if (p + u > p0) { flush(false); first = false; }
+        cur = k[u];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += v[u][i];
+    }
+  }
+  flush(true);
+}
+
+// A run that goes on behind the chunk it began in: its first partial row plus those of the chunks that follow, shared over the groups of
+// a workgroup and added up in a fixed order.
+template <bool OBF, int VEC>
+__global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, long chunks) {
+  const int lanes = 1 << a.lanes_log2, groups = 256 >> a.lanes_log2;
+  const long chunk = blockIdx.x;
+  const uint32_t none = (uint32_t)a.V;
+  const long p0 = chunk * a.cp, p1 = p0 + a.cp;
+  if (p1 >= a.T) return;
+  const uint32_t k = a.key[p1 - 1];
+  if (k == none || a.key[p1] != k) return;
+  if (a.key[p0] == k && p0 > 0 && a.key[p0 - 1] == k) return;       // began earlier: joined there
+  __shared__ float sums[256 * VEC];
+  const int g = threadIdx.x >> a.lanes_log2, l = threadIdx.x & (lanes - 1);
+  for (int slice = 0; slice < a.slices; ++slice) {
+    const int c = (slice * lanes + l) * VEC;
+    float acc[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+    if (c < a.D) {
+      bool on = true;
+      for (long q = chunk + 1 + g; on && q < chunks; q += 4 * groups) {   // four chunks of this group at a time
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const long x = q + u * groups;
+          float v[VEC];
+          const bool in = x < chunks && a.key[(x < chunks ? x : q) * a.cp] == k;
+          on = in;
+          if (in) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = a.part[(x * 2) * a.pitch + c + i];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] += v[i];
+          }
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sums[i * 256 + threadIdx.x] = acc[i];
+    __syncthreads();
+    if (g == 0 && c < a.D) {
+      float row[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        row[i] = a.part[(chunk * 2 + 1) * a.pitch + c + i];
+        for (int j = 0; j < groups; ++j) row[i] += sums[i * 256 + j * lanes + l];
+      }
+      finish_row<OBF, VEC>(a, k, c, row);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void embed_zero_kernel(uint16_t* __restrict__ p, long halves) {   // a gradient without positions
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < halves; i += (long)gridDim.x * 256) p[i] = 0;
+}
+
+int log2_ceil(long x) { int l = 0; while ((1L << l) < x) ++l; return l; }
+
+struct Layout { long tile, tiles, chunks; int cp, pitch, passes; size_t key[2], pos[2], hist, part, total; };
+Layout layout_of(long T, long V, long D) {
+  Layout L;
+  L.passes = 1;
+  while (L.passes < 4 && (V >> (8 * L.passes)) != 0) ++L.passes;
+  L.tile = 2048 * cdiv(T, 2048L * MAX_TILES);
+  L.tiles = (T + L.tile - 1) / L.tile;
+  // Positions of one chunk: 64 where that leaves the chip thousands of waves, fewer for small inputs, down to 8 (one round of loads).
+  L.cp = 64;
+  while (L.cp > 8 && T * D / L.cp < (1L << 21)) L.cp >>= 1;
+  L.chunks = (T + L.cp - 1) / L.cp;
+  L.pitch = (int)((D + 7) / 8 * 8);
+  size_t at = 0;
+  const auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+  for (int i = 0; i < 2; ++i) { L.key[i] = take(4 * (size_t)T); L.pos[i] = take(4 * (size_t)T); }
+  L.hist = take((size_t)L.tiles * DIGITS * 4);
+  L.part = take((size_t)L.chunks * 2 * L.pitch * 4);
+  L.total = at;
+  return L;
+}
+
+template <bool IBF, bool OBF, int VEC>
+void launch_sums(const SumArgs& s, long chunks, hipStream_t st) {
+  const int per_block = 256 >> s.lanes_log2;
+  const long sum_blocks = (chunks * s.slices + per_block - 1) / per_block;
+  const long fill = s.accumulate ? 0 : (s.V + FILL_ROWS - 1) / FILL_ROWS;
+  hipLaunchKernelGGL((embed_sum_kernel<IBF, OBF, VEC>), dim3((unsigned)(sum_blocks + fill)), dim3(256), 0, st, s, (int)sum_blocks);
+  if (chunks > 1) hipLaunchKernelGGL((embed_join_kernel<OBF, VEC>), dim3((unsigned)(chunks - 1)), dim3(256), 0, st, s, chunks);
+}
+
+}  // namespace
+}  // namespace dppm
+
+using namespace dppm;
+
+#define DPPM_REQUIRE_TABLE(what)                                                                                                       \
+  DPPM_REQUIRE(T >= 0 && V >= 1 && D >= 1, what ": T=%ld V=%ld D=%ld", (long)T, (long)V, (long)D);                                     \
+  DPPM_REQUIRE(T < (1L << 31) && V < (1L << 31) && D < (1L << 24), what ": T=%ld V=%ld D=%ld are too large", (long)T, (long)V, (long)D)
+
+extern "C" int dppm_embedding_fwd(const void* weight, int bf16, const int64_t* ids, float scale, void* out, int64_t T, int64_t V, int64_t D,
+                                  void* stream) {
+  DPPM_REQUIRE_TABLE("dppm_embedding_fwd");
+  if (T == 0) return DPPM_OK;
+  DPPM_REQUIRE(weight && ids && out, "dppm_embedding_fwd: null pointer");
+  const int vec = bf16 ? 8 : 4;
+  // 16 bytes a lane where rows allow it; else one value a lane
+  const bool wide = D % vec == 0 && ((uintptr_t)weight | (uintptr_t)out) % 16 == 0;
+  const long per_row = wide ? D / vec : D;
+  const int tl = log2_ceil(per_row) < 8 ? log2_ceil(per_row) : 8;
+  const long rows = (256 >> tl) * FWD_ROWS;
+  const dim3 grid((unsigned)((T + rows - 1) / rows)), block(256);
+  const hipStream_t st = as_stream(stream);
+  if (bf16) {
+    if (wide) hipLaunchKernelGGL((embed_fwd_kernel<true, 8>), grid, block, 0, st, weight, ids, scale, out, (long)T, (long)V, (int)D, tl);
+    else hipLaunchKernelGGL((embed_fwd_kernel<true, 1>), grid, block, 0, st, weight, ids, scale, out, (long)T, (long)V, (int)D, tl);
+  } else {
+    if (wide) hipLaunchKernelGGL((embed_fwd_kernel<false, 4>), grid, block, 0, st, weight, ids, scale, out, (long)T, (long)V, (int)D, tl);
+    else hipLaunchKernelGGL((embed_fwd_kernel<false, 1>), grid, block, 0, st, weight, ids, scale, out, (long)T, (long)V, (int)D, tl);
+  }
+  return check_launch("dppm_embedding_fwd");
+}
+
+extern "C" size_t dppm_embedding_wgrad_workspace_bytes(int64_t T, int64_t V, int64_t D) {
+  if (T < 1 || V < 1 || D < 1 || T >= (1L << 31) || V >= (1L << 31) || D >= (1L << 24)) return 0;
+  return layout_of(T, V, D).total;
+}
+
+extern "C" int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64_t* ids, float scale, void* dweight, int dweight_bf16, int accumulate,
+                                    int64_t T, int64_t V, int64_t D, void* workspace, size_t workspace_bytes, void* stream) {
+  DPPM_REQUIRE_TABLE("dppm_embedding_wgrad");
+  DPPM_REQUIRE(dweight, "dppm_embedding_wgrad: null pointer");
+  const hipStream_t st = as_stream(stream);
+  if (T == 0) {
+    if (!accumulate) {
+      const long halves = V * D * (dweight_bf16 ? 1 : 2);
+      const long blocks = (halves + 255) / 256;
+      hipLaunchKernelGGL(embed_zero_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, reinterpret_cast<uint16_t*>(dweight), halves);
+    }
+    return check_launch("dppm_embedding_wgrad");
+  }
+  DPPM_REQUIRE(dout && ids && workspace, "dppm_embedding_wgrad: null pointer");
+  const Layout L = layout_of(T, V, D);
+  DPPM_REQUIRE(workspace_bytes >= L.total, "dppm_embedding_wgrad: workspace of %zu bytes, %zu needed", workspace_bytes, L.total);
+  DPPM_REQUIRE((uintptr_t)workspace % 16 == 0, "dppm_embedding_wgrad: the workspace must be 16-byte aligned");
+  char* ws = reinterpret_cast<char*>(workspace);
+  SortBufs b;
+  for (int i = 0; i < 2; ++i) {
+    b.key[i] = reinterpret_cast<uint32_t*>(ws + L.key[i]);
+    b.pos[i] = reinterpret_cast<uint32_t*>(ws + L.pos[i]);
+  }
+  if (T <= ONE_TILE) {
+    hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(1024), 0, st, ids, (long)T, (long)V, L.passes, b);
+  } else {
+    uint32_t* hist = reinterpret_cast<uint32_t*>(ws + L.hist);
+    const dim3 grid((unsigned)L.tiles), block(256);
+    for (int p = 0; p < L.passes; ++p) {
+      const int in = (p + 1) & 1, out = p & 1;
+      if (p == 0) {
+        hipLaunchKernelGGL((sort_count_kernel<true>), grid, block, 0, st, ids, b.key[in], (long)T, (long)V, 0, L.tile, hist);
+        hipLaunchKernelGGL((sort_place_kernel<true>), grid, block, 0, st, ids, b.key[in], b.pos[in], b.key[out], b.pos[out], (long)T, (long)V, 0, L.tile, hist);
+      } else {
+        hipLaunchKernelGGL((sort_count_kernel<false>), grid, block, 0, st, ids, b.key[in], (long)T, (long)V, 8 * p, L.tile, hist);
+        hipLaunchKernelGGL((sort_place_kernel<false>), grid, block, 0, st, ids, b.key[in], b.pos[in], b.key[out], b.pos[out], (long)T, (long)V, 8 * p, L.tile, hist);
+      }
+    }
+  }
+  SumArgs s;
+  s.dout = dout; s.key = b.key[(L.passes - 1) & 1]; s.pos = b.pos[(L.passes - 1) & 1]; s.dw = dweight;
+  s.part = reinterpret_cast<float*>(ws + L.part);
+  s.T = T; s.V = V; s.D = (int)D; s.pitch = L.pitch; s.cp = L.cp; s.accumulate = accumulate != 0; s.scale = scale;
+  const int vec = dout_bf16 ? 8 : 4;
+  const bool wide = D % vec == 0 && (uintptr_t)dout % 16 == 0 && (uintptr_t)dweight % 16 == 0;
+  const long per_row = wide ? D / vec : D;
+  s.lanes_log2 = log2_ceil(per_row) < 6 ? log2_ceil(per_row) : 6;
+  s.slices = (int)((per_row + (1 << s.lanes_log2) - 1) >> s.lanes_log2);
+  if (dout_bf16) {
+    if (dweight_bf16) wide ? launch_sums<true, true, 8>(s, L.chunks, st) : launch_sums<true, true, 1>(s, L.chunks, st);
+    else wide ? launch_sums<true, false, 8>(s, L.chunks, st) : launch_sums<true, false, 1>(s, L.chunks, st);
+  } else {
+    if (dweight_bf16) wide ? launch_sums<false, true, 4>(s, L.chunks, st) : launch_sums<false, true, 1>(s, L.chunks, st);
+    else wide ? launch_sums<false, false, 4>(s, L.chunks, st) : launch_sums<false, false, 1>(s, L.chunks, st);
+  }
+  return check_launch("dppm_embedding_wgrad");
+}

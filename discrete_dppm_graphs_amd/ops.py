@@ -395,6 +395,65 @@ def adam_step(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, weight_de
                              beta2, eps, weight_decay, int(step), grad_scale, _stream()), "dppm_adam_step")
 
 
+# ------------------------------------------------------------------------------------------------- categorical states
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+def _chk_float(t, name, shape=None):
+    """A contiguous float32 or bfloat16 tensor on the GPU."""
+    if isinstance(t, torch.Tensor) and t.dtype not in _FLOATS:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected float32 or bfloat16")
+    return _chk(t, name, shape, t.dtype if isinstance(t, torch.Tensor) else None)
+
+
+def _chk_device(t, name, like, like_name):
+    if t.device != like.device:
+        raise ValueError(f"{name}: on {t.device}, {like_name} on {like.device}")
+    return t
+
+
+def embedding_fwd(weight, ids, scale=1.0, out=None):
+    """scale * weight[ids]: weight [V, D] float32 or bfloat16, ids int64 of any shape -> [*ids.shape, D] in weight's type.  An id
+    outside [0, V) (a padded position) gives a row of zeros."""
+    weight = _chk_float(weight, "weight")
+    if weight.dim() != 2:
+        raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [V, D]")
+    ids = _chk_device(_chk(ids, "ids", None, torch.int64), "ids", weight, "weight")
+    shape = (*ids.shape, weight.shape[1])
+    if out is None:
+        out = torch.empty(shape, device=weight.device, dtype=weight.dtype)
+    else:
+        _chk_device(_chk(out, "out", shape, weight.dtype), "out", weight, "weight")
+    with _on(weight.device):
+        check(lib.dppm_embedding_fwd(weight.data_ptr(), weight.dtype == torch.bfloat16, ids.data_ptr(), scale, out.data_ptr(), ids.numel(),
+                                     weight.shape[0], weight.shape[1], _raw_stream(weight.device)), "dppm_embedding_fwd")
+    return out
+
+
+def embedding_wgrad(dout, ids, num_rows, scale=1.0, out=None, accumulate=False):
+    """Gradient of embedding_fwd: dout [*ids.shape, D] -> [num_rows, D], scale times the sum of dout over the positions of each class,
+    the same bits from call to call.  out: where it goes (float32 or bfloat16; default: dout's type); accumulate=True adds to it and
+    leaves rows without a position as they are."""
+    dout = _chk_float(dout, "dout")
+    ids = _chk_device(_chk(ids, "ids", None, torch.int64), "ids", dout, "dout")
+    if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:
+        raise ValueError(f"dout: shape {tuple(dout.shape)}, expected [*{tuple(ids.shape)}, D]")
+    T, V, D = ids.numel(), int(num_rows), dout.shape[-1]
+    if out is None:
+        if accumulate:
+            raise ValueError("embedding_wgrad: accumulate needs an out")
+        out = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
+    else:
+        _chk_device(_chk_float(out, "out", (V, D)), "out", dout, "dout")
+    nbytes = lib.dppm_embedding_wgrad_workspace_bytes(T, V, D)
+    with _on(dout.device):
+        ws = torch.empty(nbytes, device=dout.device, dtype=torch.uint8)
+        check(lib.dppm_embedding_wgrad(dout.data_ptr(), dout.dtype == torch.bfloat16, ids.data_ptr(), scale, out.data_ptr(),
+                                       out.dtype == torch.bfloat16, accumulate, T, V, D, ws.data_ptr(), nbytes, _raw_stream(dout.device)),
+              "dppm_embedding_wgrad")
+    return out
+
+
 STATE_BLOCK = 256      # values of a tensor that share one scale of its 8-bit moments (include/dppm_hip.h, dppm_tensor_entry)
 
 

@@ -47,3 +47,30 @@ def test_adamw_entry_refuses():
 def test_front_ends_refuse_cpu_tensors():
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.TensorSet([torch.zeros(4)], [torch.zeros(4)])
+
+
+def test_embedding_oracle_is_torch_embedding():
+    torch.manual_seed(2)
+    w = torch.randn(7, 3, dtype=torch.float64, requires_grad=True)
+    ids = torch.randint(0, 7, (4, 5))
+    d = torch.randn(4, 5, 3, dtype=torch.float64)
+    y = torch.nn.functional.embedding(ids, w) * 1.5
+    y.backward(d)
+    assert torch.allclose(classes.embedding(w.detach(), ids, 1.5), y.detach()) and torch.allclose(classes.embedding_wgrad(d, ids, 7, 1.5), w.grad)
+    assert (classes.embedding(w.detach(), torch.tensor([-1, 7]), 1.5) == 0).all()
+
+
+def test_embedding_entries_refuse():
+    one = C.c_void_p(16)
+    for bad in ((-1, 5, 4), (3, 0, 4), (3, 5, 0), (1 << 31, 5, 4), (3, 1 << 31, 4), (3, 5, 1 << 24)):
+        assert lib.dppm_embedding_fwd(one, 0, one, 1.0, one, *bad, None) == -1
+        assert lib.dppm_embedding_wgrad(one, 0, one, 1.0, one, 0, 0, *bad, one, 1 << 40, None) == -1
+        assert lib.dppm_embedding_wgrad_workspace_bytes(*bad) == 0
+    for k in range(3):
+        ptrs = [one, one, one]
+        ptrs[k] = None
+        assert lib.dppm_embedding_fwd(ptrs[0], 0, ptrs[1], 1.0, ptrs[2], 3, 5, 4, None) == -1
+        assert lib.dppm_embedding_wgrad(ptrs[0], 0, ptrs[1], 1.0, ptrs[2], 0, 0, 3, 5, 4, one, 1 << 40, None) == -1
+    need = lib.dppm_embedding_wgrad_workspace_bytes(3, 5, 4)
+    assert lib.dppm_embedding_wgrad(one, 0, one, 1.0, one, 0, 0, 3, 5, 4, one, need - 1, None) == -1
+    assert lib.dppm_embedding_wgrad(one, 0, one, 1.0, one, 0, 0, 3, 5, 4, C.c_void_p(8), need, None) == -1
