@@ -24,7 +24,7 @@ namespace {
 
 constexpr int BLK = 256;           // values that share a scale = one quad of values on each lane of a wave
 constexpr int CHUNK = 4096;        // values of one workgroup: 256 threads x 4 quads
-constexpr int NORM_GRID = 1024;    // partial sums of the gradient's norm
+constexpr int NORM_GRID = 2048;    // partial sums of the gradient's norm: as many workgroups as the chip holds
 
 struct StepArgs {
   float one_minus_b1, b2, one_minus_b2, eps, step_size, bc2_rsqrt, gscale;
@@ -139,17 +139,29 @@ template <bool GBF>
 __global__ __launch_bounds__(256) void grad_sq_kernel(const dppm_tensor_entry* __restrict__ tab, const int2* __restrict__ chunks, int n_chunks,
                                                       double* __restrict__ part) {
   double s = 0.0;
-  for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
-    const int2 ch = chunks[c];
-    const void* g = tab[ch.x].grad;
-    const long n = tab[ch.x].numel, base = (long)ch.y * CHUNK;
-    float q[4][4];
+  // two chunks at a time: a chunk's loads wait for its table entry, which waits for its pair
+  for (int c = blockIdx.x; c < n_chunks; c += 2 * gridDim.x) {
+    float q[2][4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load4<GBF, false>(g, base + (i * 256 + threadIdx.x) * 4, n, q[i]);
+    for (int j = 0; j < 2; ++j) {
+      const bool in = c + j * (int)gridDim.x < n_chunks;
+      const int2 ch = chunks[in ? c + j * (int)gridDim.x : c];
+      const void* g = tab[ch.x].grad;
+      const long n = in ? tab[ch.x].numel : 0, base = (long)ch.y * CHUNK;
+      if (base + CHUNK <= n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) load4<GBF, true>(g, base + (i * 256 + threadIdx.x) * 4, n, q[j][i]);
+      } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s += (double)q[i][k] * (double)q[i][k];
+        for (int i = 0; i < 4; ++i) load4<GBF, false>(g, base + (i * 256 + threadIdx.x) * 4, n, q[j][i]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s += (double)q[j][i][k] * (double)q[j][i][k];
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);

@@ -102,12 +102,15 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------ sorting positions by class
-// Least significant digit first, 8 bits a pass: count the digits of every tile, then place every pair at
+// Least significant digit first: count the digits of every tile, then place every pair at
 //   (pairs with a smaller digit) + (pairs with the digit in earlier tiles) + (rank among the tile's pairs with the digit),
-// which keeps the order of equal digits.  Classes without a row sort behind all others as class V.
-constexpr int DIGITS = 256, PER_THREAD = 8;
+// which keeps the order of equal digits.  Classes without a row sort behind all others as class V.  The bits of V are shared evenly over
+// as few passes as the digit's width allows.  Up to ONE_TILE positions one workgroup sorts alone in one launch, 10 bits a pass; more are
+// cut into tiles of 1024 positions and up, 9 bits a pass and two launches each.
+constexpr int ONE_BITS = 10, TILE_BITS = 9;
 constexpr int MAX_TILES = 128;                 // every tile's placement reads the counts of all
-constexpr int ONE_TILE = 8192;                 // up to here one workgroup of 1024 threads sorts alone, in one launch
+constexpr int ONE_TILE = 8192;                 // 1024 threads x 8
+constexpr int TILE = 1024;                     // 256 threads x 4
 
 struct SortBufs { uint32_t *key[2], *pos[2]; };
 
@@ -116,21 +119,47 @@ __device__ __forceinline__ uint32_t class_key(const int64_t* ids, long t, long V
   return (uint32_t)((i >= 0 && i < V) ? i : V);
 }
 
-template <int NT>
-struct RankShared { uint32_t cnt[NT / 64][DIGITS]; uint32_t base[DIGITS]; uint32_t scan[DIGITS]; };
+template <int NT, int BITS>
+struct RankShared { uint32_t cnt[NT / 64][1 << BITS]; uint32_t base[1 << BITS]; uint32_t wave[NT / 64]; };
 
-// Places NT * PER_THREAD consecutive pairs (those before `n`).  s.base[d]: where the next pair with digit d goes; moved on for the next call.
-// A wave takes 64 * PER_THREAD consecutive pairs, 64 at a time; lanes with the same digit are found with one ballot per bit.
-template <int NT, bool FIRST>
-__device__ __forceinline__ void place(RankShared<NT>& s, const int64_t* ids, long V, const uint32_t* key_in, const uint32_t* pos_in, uint32_t* key_out,
-                                      uint32_t* pos_out, long begin, long n, int shift) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int i = threadIdx.x; i < (NT / 64) * DIGITS; i += NT) (&s.cnt[0][0])[i] = 0;
+// s.base: counts -> their exclusive prefix sum.  Called by every thread, between barriers of its own.
+template <int NT, int BITS>
+__device__ __forceinline__ void scan_digits(RankShared<NT, BITS>& s) {
+  constexpr int E = ((1 << BITS) + NT - 1) / NT;     // digits of a thread
+  static_assert(E * NT == (1 << BITS), "");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __syncthreads();
-  uint32_t key[PER_THREAD], pos[PER_THREAD], rank[PER_THREAD];
-  const long at0 = begin + (long)wave * 64 * PER_THREAD + lane;
+  uint32_t own[E], sum = 0;
 #pragma unroll
-  for (int r = 0; r < PER_THREAD; ++r) {
+  for (int e = 0; e < E; ++e) { own[e] = s.base[threadIdx.x * E + e]; sum += own[e]; }
+  uint32_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t up = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 63) s.wave[wave] = incl;
+  __syncthreads();
+  uint32_t at = incl - sum;
+  for (int w = 0; w < wave; ++w) at += s.wave[w];
+#pragma unroll
+  for (int e = 0; e < E; ++e) { s.base[threadIdx.x * E + e] = at; at += own[e]; }
+  __syncthreads();
+}
+
+// Places NT * PER consecutive pairs from `begin` on (those before `n`).  s.base[d]: where the next pair with digit d goes, moved on for the
+// next call; ALONE: these are all pairs, and s.base comes from their counts.  A wave takes 64 * PER consecutive pairs, 64 at a time; lanes
+// with the same digit are found with one ballot per bit.
+template <int NT, int BITS, int PER, bool FIRST, bool ALONE>
+__device__ __forceinline__ void place(RankShared<NT, BITS>& s, const int64_t* ids, long V, const uint32_t* key_in, const uint32_t* pos_in, uint32_t* key_out,
+                                      uint32_t* pos_out, long begin, long n, int shift, int bits) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t low = (1u << bits) - 1u;
+  for (int i = threadIdx.x; i < (NT / 64) << BITS; i += NT) (&s.cnt[0][0])[i] = 0;
+  uint32_t key[PER], pos[PER], rank[PER];
+  const long at0 = begin + (long)wave * 64 * PER + lane;
+#pragma unroll
+  for (int r = 0; r < PER; ++r) {
     const long at = at0 + r * 64;
     key[r] = 0; pos[r] = 0;
     if (at < n) {
@@ -138,13 +167,13 @@ __device__ __forceinline__ void place(RankShared<NT>& s, const int64_t* ids, lon
       else { key[r] = key_in[at]; pos[r] = pos_in[at]; }
     }
   }
+  __syncthreads();
 #pragma unroll
-  for (int r = 0; r < PER_THREAD; ++r) {
+  for (int r = 0; r < PER; ++r) {
     const bool in = at0 + r * 64 < n;
-    const uint32_t d = (key[r] >> shift) & (DIGITS - 1);
+    const uint32_t d = (key[r] >> shift) & low;
     uint64_t same = __ballot(in);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
+    for (int b = 0; b < bits; ++b) {
       const uint64_t one = __ballot((d >> b) & 1u);
       same &= ((d >> b) & 1u) ? one : ~one;
     }
@@ -157,95 +186,79 @@ __device__ __forceinline__ void place(RankShared<NT>& s, const int64_t* ids, lon
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   __syncthreads();
-  if (threadIdx.x < DIGITS) {   // per digit: where each wave's pairs begin
-    uint32_t b = s.base[threadIdx.x];
+  if (ALONE) {
+    for (int d = threadIdx.x; d < (1 << BITS); d += NT) {
+      uint32_t c = 0;
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) c += s.cnt[w][d];
+      s.base[d] = c;
+    }
+    scan_digits(s);
+  }
+  for (int d = threadIdx.x; d < (1 << BITS); d += NT) {   // where each wave's pairs with the digit begin
+    uint32_t b = s.base[d];
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) {
-      const uint32_t c = s.cnt[w][threadIdx.x];
-      s.cnt[w][threadIdx.x] = b;
+      const uint32_t c = s.cnt[w][d];
+      s.cnt[w][d] = b;
       b += c;
     }
-    s.base[threadIdx.x] = b;
+    s.base[d] = b;
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < PER_THREAD; ++r)
+  for (int r = 0; r < PER; ++r)
     if (at0 + r * 64 < n) {
-      const uint32_t to = s.cnt[wave][(key[r] >> shift) & (DIGITS - 1)] + rank[r];
+      const uint32_t to = s.cnt[wave][(key[r] >> shift) & low] + rank[r];
       key_out[to] = key[r];
       pos_out[to] = pos[r];
     }
   __syncthreads();
 }
 
-// exclusive prefix sum of s.scan over the digits, into s.scan; called by every thread
-template <int NT>
-__device__ __forceinline__ void scan_digits(RankShared<NT>& s) {
-  __syncthreads();
-  uint32_t own = 0;
-  if (threadIdx.x < DIGITS) own = s.scan[threadIdx.x];
-  for (int o = 1; o < DIGITS; o <<= 1) {
-    uint32_t add = 0;
-    if (threadIdx.x < DIGITS && (int)threadIdx.x >= o) add = s.scan[threadIdx.x - o];
-    __syncthreads();
-    if (threadIdx.x < DIGITS) s.scan[threadIdx.x] += add;
-    __syncthreads();
-  }
-  if (threadIdx.x < DIGITS) s.scan[threadIdx.x] -= own;
-  __syncthreads();
-}
-
-__global__ __launch_bounds__(1024) void sort_one_kernel(const int64_t* __restrict__ ids, long T, long V, int passes, SortBufs b) {
-  __shared__ RankShared<1024> s;
-  for (int p = 0; p < passes; ++p) {
-    const uint32_t *ki = b.key[(p + 1) & 1], *pi = b.pos[(p + 1) & 1];
-    uint32_t *ko = b.key[p & 1], *po = b.pos[p & 1];
-    if (threadIdx.x < DIGITS) s.scan[threadIdx.x] = 0;
-    __syncthreads();
-    for (long t = threadIdx.x; t < T; t += 1024) {
-      const uint32_t k = p == 0 ? class_key(ids, t, V) : ki[t];
-      atomicAdd(&s.scan[(k >> (8 * p)) & (DIGITS - 1)], 1u);
-    }
-    scan_digits(s);
-    if (threadIdx.x < DIGITS) s.base[threadIdx.x] = s.scan[threadIdx.x];
-    __syncthreads();
-    for (long t = 0; t < T; t += 1024 * PER_THREAD) {
-      if (p == 0) place<1024, true>(s, ids, V, ki, pi, ko, po, t, T, 8 * p);
-      else place<1024, false>(s, ids, V, ki, pi, ko, po, t, T, 8 * p);
-    }
+__global__ __launch_bounds__(1024) void sort_one_kernel(const int64_t* __restrict__ ids, long T, long V, int passes, int bits, SortBufs b) {
+  __shared__ RankShared<1024, ONE_BITS> s;
+  place<1024, ONE_BITS, ONE_TILE / 1024, true, true>(s, ids, V, nullptr, nullptr, b.key[0], b.pos[0], 0, T, 0, bits);
+  for (int p = 1; p < passes; ++p) {
+    const int out = p & 1;
+    place<1024, ONE_BITS, ONE_TILE / 1024, false, true>(s, ids, V, b.key[out ^ 1], b.pos[out ^ 1], b.key[out], b.pos[out], 0, T, bits * p, bits);
   }
 }
 
 template <bool FIRST>
-__global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ key, long T, long V, int shift, long tile,
-                                                         uint32_t* __restrict__ hist) {
-  __shared__ uint32_t h[DIGITS];
-  h[threadIdx.x] = 0;
+__global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ key, long T, long V, int shift, int bits,
+                                                         long tile, uint32_t* __restrict__ hist) {
+  __shared__ uint32_t h[1 << TILE_BITS];
+  for (int d = threadIdx.x; d < (1 << TILE_BITS); d += 256) h[d] = 0;
   __syncthreads();
+  const uint32_t low = (1u << bits) - 1u;
   const long begin = blockIdx.x * tile, end = begin + tile < T ? begin + tile : T;
-  for (long t = begin + threadIdx.x; t < end; t += 256) atomicAdd(&h[((FIRST ? class_key(ids, t, V) : key[t]) >> shift) & (DIGITS - 1)], 1u);
+  for (long t = begin + threadIdx.x; t < end; t += 256) atomicAdd(&h[((FIRST ? class_key(ids, t, V) : key[t]) >> shift) & low], 1u);
   __syncthreads();
-  hist[blockIdx.x * DIGITS + threadIdx.x] = h[threadIdx.x];
+  for (int d = threadIdx.x; d < (1 << TILE_BITS); d += 256) hist[((long)blockIdx.x << TILE_BITS) + d] = h[d];
 }
 
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_place_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ key_in, const uint32_t* __restrict__ pos_in,
-                                                         uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out, long T, long V, int shift, long tile,
-                                                         const uint32_t* __restrict__ hist) {
-  __shared__ RankShared<256> s;
-  uint32_t all = 0, earlier = 0;
-#pragma unroll 8
+                                                         uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out, long T, long V, int shift, int bits,
+                                                         long tile, const uint32_t* __restrict__ hist) {
+  __shared__ RankShared<256, TILE_BITS> s;
+  static_assert(1 << TILE_BITS == 512, "two digits a thread");
+  uint32_t all0 = 0, all1 = 0, earlier0 = 0, earlier1 = 0;
+#pragma unroll 16
   for (int t = 0; t < (int)gridDim.x; ++t) {
-    const uint32_t c = hist[t * DIGITS + threadIdx.x];
-    all += c;
-    if (t < (int)blockIdx.x) earlier += c;
+    const uint2 c = reinterpret_cast<const uint2*>(hist + ((long)t << TILE_BITS))[threadIdx.x];
+    all0 += c.x; all1 += c.y;
+    if (t < (int)blockIdx.x) { earlier0 += c.x; earlier1 += c.y; }
   }
-  s.scan[threadIdx.x] = all;
+  s.base[2 * threadIdx.x] = all0;
+  s.base[2 * threadIdx.x + 1] = all1;
   scan_digits(s);
-  s.base[threadIdx.x] = s.scan[threadIdx.x] + earlier;
+  s.base[2 * threadIdx.x] += earlier0;
+  s.base[2 * threadIdx.x + 1] += earlier1;
   __syncthreads();
   const long begin = blockIdx.x * tile, end = begin + tile < T ? begin + tile : T;
-  for (long t = begin; t < end; t += 256 * PER_THREAD) place<256, FIRST>(s, ids, V, key_in, pos_in, key_out, pos_out, t, end, shift);
+  for (long t = begin; t < end; t += TILE) place<256, TILE_BITS, TILE / 256, FIRST, false>(s, ids, V, key_in, pos_in, key_out, pos_out, t, end, shift, bits);
 }
 
 // ------------------------------------------------------------------------------------------------ sums of sorted rows
@@ -371,42 +384,43 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, long chunks)
   if (a.key[p0] == k && p0 > 0 && a.key[p0 - 1] == k) return;       // began earlier: joined there
   __shared__ float sums[256 * VEC];
   const int g = threadIdx.x >> a.lanes_log2, l = threadIdx.x & (lanes - 1);
-  for (int slice = 0; slice < a.slices; ++slice) {
-    const int c = (slice * lanes + l) * VEC;
-    float acc[VEC];
+  const int c = ((int)blockIdx.y * lanes + l) * VEC;
+  float acc[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-    if (c < a.D) {
-      bool on = true;
-      for (long q = chunk + 1 + g; on && q < chunks; q += 4 * groups) {   // four chunks of this group at a time
+  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+  if (c < a.D) {
+    // eight chunks of this group at a time: their rows are read while it is not known yet whether they belong to the run
+    constexpr int AHEAD = 8;
+    bool on = true;
+    for (long q = chunk + 1 + g; on && q < chunks; q += AHEAD * groups) {
+      uint32_t key[AHEAD];
+      float v[AHEAD][VEC];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const long x = q + u * groups;
-          float v[VEC];
-          const bool in = x < chunks && a.key[(x < chunks ? x : q) * a.cp] == k;
-          on = in;
-          if (in) {
+      for (int u = 0; u < AHEAD; ++u) {
+        const long x = q + u * groups;
+        const long y = x < chunks ? x : q;
+        key[u] = a.key[y * a.cp];
+        load_vec<false, VEC>(a.part, (y * 2) * a.pitch + c, v[u]);
+        if (x >= chunks) key[u] = none;
+      }
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = a.part[(x * 2) * a.pitch + c + i];
+      for (int u = 0; u < AHEAD; ++u) {
+        on = key[u] == k;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] += v[i];
-          }
-        }
+        for (int i = 0; i < VEC; ++i) acc[i] += on ? v[u][i] : 0.f;
       }
     }
-    __syncthreads();
+  }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sums[i * 256 + threadIdx.x] = acc[i];
-    __syncthreads();
-    if (g == 0 && c < a.D) {
-      float row[VEC];
+  for (int i = 0; i < VEC; ++i) sums[i * 256 + threadIdx.x] = acc[i];
+  __syncthreads();
+  if (g == 0 && c < a.D) {
+    float row[VEC];
+    load_vec<false, VEC>(a.part, (chunk * 2 + 1) * a.pitch + c, row);
+    for (int j = 0; j < groups; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        row[i] = a.part[(chunk * 2 + 1) * a.pitch + c + i];
-        for (int j = 0; j < groups; ++j) row[i] += sums[i * 256 + j * lanes + l];
-      }
-      finish_row<OBF, VEC>(a, k, c, row);
-    }
+      for (int i = 0; i < VEC; ++i) row[i] += sums[i * 256 + j * lanes + l];
+    finish_row<OBF, VEC>(a, k, c, row);
   }
 }
 
@@ -416,12 +430,13 @@ __global__ __launch_bounds__(256) void embed_zero_kernel(uint16_t* __restrict__ 
 
 int log2_ceil(long x) { int l = 0; while ((1L << l) < x) ++l; return l; }
 
-struct Layout { long tile, tiles, chunks; int cp, pitch, passes; size_t key[2], pos[2], hist, part, total; };
+struct Layout { long tile, tiles, chunks; int cp, pitch, passes, bits; size_t key[2], pos[2], hist, part, total; };
 Layout layout_of(long T, long V, long D) {
   Layout L;
-  L.passes = 1;
-  while (L.passes < 4 && (V >> (8 * L.passes)) != 0) ++L.passes;
-  L.tile = 2048 * cdiv(T, 2048L * MAX_TILES);
+  const int all = log2_ceil(V + 1);                           // keys are 0 .. V
+  L.passes = cdiv(all, T <= ONE_TILE ? ONE_BITS : TILE_BITS);
+  L.bits = cdiv(all, L.passes);
+  L.tile = TILE * cdiv(T, (long)TILE * MAX_TILES);
   L.tiles = (T + L.tile - 1) / L.tile;
   // Positions of one chunk: 64 where that leaves the chip thousands of waves, fewer for small inputs, down to 8 (one round of loads).
   L.cp = 64;
@@ -431,7 +446,7 @@ Layout layout_of(long T, long V, long D) {
   size_t at = 0;
   const auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   for (int i = 0; i < 2; ++i) { L.key[i] = take(4 * (size_t)T); L.pos[i] = take(4 * (size_t)T); }
-  L.hist = take((size_t)L.tiles * DIGITS * 4);
+  L.hist = take((size_t)L.tiles << (TILE_BITS + 2));
   L.part = take((size_t)L.chunks * 2 * L.pitch * 4);
   L.total = at;
   return L;
@@ -443,7 +458,7 @@ void launch_sums(const SumArgs& s, long chunks, hipStream_t st) {
   const long sum_blocks = (chunks * s.slices + per_block - 1) / per_block;
   const long fill = s.accumulate ? 0 : (s.V + FILL_ROWS - 1) / FILL_ROWS;
   hipLaunchKernelGGL((embed_sum_kernel<IBF, OBF, VEC>), dim3((unsigned)(sum_blocks + fill)), dim3(256), 0, st, s, (int)sum_blocks);
-  if (chunks > 1) hipLaunchKernelGGL((embed_join_kernel<OBF, VEC>), dim3((unsigned)(chunks - 1)), dim3(256), 0, st, s, chunks);
+  if (chunks > 1) hipLaunchKernelGGL((embed_join_kernel<OBF, VEC>), dim3((unsigned)(chunks - 1), (unsigned)s.slices), dim3(256), 0, st, s, chunks);
 }
 
 }  // namespace
@@ -507,18 +522,18 @@ extern "C" int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64
     b.pos[i] = reinterpret_cast<uint32_t*>(ws + L.pos[i]);
   }
   if (T <= ONE_TILE) {
-    hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(1024), 0, st, ids, (long)T, (long)V, L.passes, b);
+    hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(1024), 0, st, ids, (long)T, (long)V, L.passes, L.bits, b);
   } else {
     uint32_t* hist = reinterpret_cast<uint32_t*>(ws + L.hist);
     const dim3 grid((unsigned)L.tiles), block(256);
     for (int p = 0; p < L.passes; ++p) {
       const int in = (p + 1) & 1, out = p & 1;
       if (p == 0) {
-        hipLaunchKernelGGL((sort_count_kernel<true>), grid, block, 0, st, ids, b.key[in], (long)T, (long)V, 0, L.tile, hist);
-        hipLaunchKernelGGL((sort_place_kernel<true>), grid, block, 0, st, ids, b.key[in], b.pos[in], b.key[out], b.pos[out], (long)T, (long)V, 0, L.tile, hist);
+        hipLaunchKernelGGL((sort_count_kernel<true>), grid, block, 0, st, ids, b.key[in], (long)T, (long)V, 0, L.bits, L.tile, hist);
+        hipLaunchKernelGGL((sort_place_kernel<true>), grid, block, 0, st, ids, b.key[in], b.pos[in], b.key[out], b.pos[out], (long)T, (long)V, 0, L.bits, L.tile, hist);
       } else {
-        hipLaunchKernelGGL((sort_count_kernel<false>), grid, block, 0, st, ids, b.key[in], (long)T, (long)V, 8 * p, L.tile, hist);
-        hipLaunchKernelGGL((sort_place_kernel<false>), grid, block, 0, st, ids, b.key[in], b.pos[in], b.key[out], b.pos[out], (long)T, (long)V, 8 * p, L.tile, hist);
+        hipLaunchKernelGGL((sort_count_kernel<false>), grid, block, 0, st, ids, b.key[in], (long)T, (long)V, L.bits * p, L.bits, L.tile, hist);
+        hipLaunchKernelGGL((sort_place_kernel<false>), grid, block, 0, st, ids, b.key[in], b.pos[in], b.key[out], b.pos[out], (long)T, (long)V, L.bits * p, L.bits, L.tile, hist);
       }
     }
   }
