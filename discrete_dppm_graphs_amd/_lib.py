@@ -88,6 +88,9 @@ SIGNATURES = {
     "dppm_embedding_wgrad_workspace_bytes": (C.c_size_t, [C.c_int64] * 3),
     "dppm_embedding_wgrad": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_float, C.c_void_p, C.c_int, C.c_int] + [C.c_int64] * 3
                              + [C.c_void_p, C.c_size_t, c_stream]),
+    "dppm_loss_ce_workspace_bytes": (C.c_size_t, [C.c_int64] * 3 + [C.c_int] * 2),
+    "dppm_loss_ce_fwd_bwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_double] + [C.c_int64] * 3
+                             + [C.c_void_p] * 5 + [C.c_size_t, c_stream]),
     "dppm_adamw_chunk": (C.c_int, []),
     "dppm_adamw_workspace_bytes": (C.c_size_t, []),
     "dppm_adamw_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int] + [C.c_double] * 4 + [C.c_int, C.c_double, C.c_double,

@@ -1,0 +1,599 @@
+// Softmax cross entropy over many classes, from the last hidden layer and the classes' rows, with both gradients; the scores never reach
+// memory.  For row t of x with class y_t, weight w_t and n = denom (default: the number of rows that have a class):
+//
+//   s_tv = x_t . W_v      lse_t = log sum_v exp s_tv      loss = sum_t w_t / n (lse_t - s_{t,y_t})
+//   d_tv = (exp(s_tv - lse_t) - [v = y_t]) w_t / n        dx_t = sum_v d_tv W_v        dW_v = sum_t d_tv x_t
+//
+// A row whose class lies outside [0, V) has none: its loss and its gradient row are zero, and it adds nothing to dW.
+//
+// Three matrix products, each 2 T V D operations, and the exponentials between them:
+//  * scores: tiles of s on the matrix cores; from the accumulators each strip of classes gives its maximum and its sum of exponentials per
+//    row, and (with gradients) the exponentials relative to the strip's maximum, bfloat16 for bfloat16 inputs and float32 for float32;
+//  * rows: lse, the rows' losses;
+//  * turn: exponentials to d, rounded once to the operands' type, as it stands and transposed;
+//  * dx = d W and dW = d^T x, both with the contracted dimension contiguous in both operands: W and x are transposed once.
+// The exponentials held at a time are those of one block of rows, at most 2^29 (bfloat16) or 2^27 (float32) of them: memory does not grow
+// with T.  Several blocks add up dW in float32.
+#include "dppm_common.h"
+#include "dppm_tngemm.h"
+
+namespace dppm {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {   // round to nearest even (v_cvt_pk_bf16_f32)
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
+}
+__device__ __forceinline__ uint16_t to_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+__device__ __forceinline__ float from_bf16(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+
+// exp x: for float32 inputs to the last bits; else by one multiplication and v_exp_f32, off by |x| 2^-24 and the instruction's own last bit,
+// far under the rounding of bfloat16 results
+template <bool F32>
+__device__ __forceinline__ float exp_of(float x) { return F32 ? expf(x) : __expf(x); }
+
+// plane `p` (0 hi, 1 mid, 2 lo) of a float32 value: each the nearest bfloat16 to what the planes before it leave
+__device__ __forceinline__ void split3(float v, uint16_t (&out)[3]) {
+  out[0] = to_bf16(v);
+  float r = v - from_bf16(out[0]);
+  out[1] = to_bf16(r);
+  r = r - from_bf16(out[1]);
+  out[2] = to_bf16(r);
+  if (!(fabsf(v) <= 3.3e38f)) { out[1] = 0; out[2] = 0; }     // infinity and NaN (and what rounds to infinity) stand in the first plane alone
+}
+
+// ------------------------------------------------------------------------------------------------ counting rows, losses
+__global__ __launch_bounds__(1024) void count_kernel(const int64_t* __restrict__ target, long T, long V, float denom, float* __restrict__ inv) {
+  __shared__ uint32_t w[16];
+  uint32_t n = 0;
+  for (long t = threadIdx.x; t < T; t += 1024) n += target[t] >= 0 && target[t] < V;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t all = 0;
+    for (int i = 0; i < 16; ++i) all += w[i];
+    *inv = 1.f / (denom > 0.f ? denom : (float)(all ? all : 1u));
+  }
+}
+
+__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ row_loss, const float* __restrict__ row_weight, const float* __restrict__ inv, long T,
+                                                    float* __restrict__ loss) {
+  __shared__ double w[16];
+  double s = 0.0;
+  for (long t = threadIdx.x; t < T; t += 1024) {
+    const float l = row_loss[t];
+    if (l != 0.f) s += (double)l * (row_weight ? row_weight[t] : 1.f);      // rows without a class have 0, whatever their weight
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    for (int i = 0; i < 16; ++i) all += w[i];
+    *loss = (float)(all * *inv);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ scores
+struct ScoreOut {
+  float2* stats;            // [strips][rows of the block]: (maximum, sum of exponentials relative to it)
+  float* target_score;      // [rows]
+  const int64_t* target;    // [rows]
+  void* e;                  // exponentials [rows][pitch], or null
+  long pitch;
+  int V;
+};
+
+// m = class, n = row: a lane holds 16 classes of one row per 32 x 32 tile, so that maxima and sums run inside lanes and cross one pair.
+template <class T, bool F32>
+__global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  int tm, tn;
+  tn_tile_of(blockIdx.x, gridDim.x, g.tiles_m, g.tiles_n, tm, tn);
+  const int m0 = tm * T::BM, n0 = tn * T::BN;
+  tn_acc acc[T::MI][T::NI];
+  tn_product<T>(g, lds, m0, n0, 0, g.ksteps * g.pairs, acc);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;     // this wave's strip of classes, its rows
+  const int strip = ms / T::WM, half = (lane >> 5) * 4;
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int n = ns + j * 32 + (lane & 31);
+    if (ms + T::WM > o.V) {      // classes behind the last
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (ms + i * 32 + (k >> 2) * 8 + half + (k & 3) >= o.V) acc[i][j][k] = -INFINITY;
+    }
+    const int64_t y = n < g.N ? o.target[n] : -1;
+    const bool here = y >= ms && y < ms + T::WM && y < o.V;
+    if (__any(here)) {
+      const int at = (int)(y - ms);
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (here && at == i * 32 + (k >> 2) * 8 + half + (k & 3)) o.target_score[n] = acc[i][j][k];
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) top = fmaxf(top, acc[i][j][k]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float ref = top == -INFINITY ? 0.f : top;      // a strip of nothing but -inf: exponentials of 0
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float e = exp_of<F32>(acc[i][j][k] - ref);
+        acc[i][j][k] = e;
+        sum += e;
+      }
+    sum += __shfl_xor(sum, 32, 64);
+    if (lane < 32 && n < g.N && ms < o.V) o.stats[(long)strip * g.N + n] = make_float2(top, sum);
+  }
+  if (o.e) {
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j)
+      tn_rows<T>(lds, acc, j, [&](int row, int m, const float (&v)[8]) {
+        const int n = ns + j * 32 + row, c = ms + m;
+        if (n < g.N && c < o.pitch) {
+          const long at = (long)n * o.pitch + c;
+          if (F32) {
+            f32x4* p = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(o.e) + at);
+            p[0] = f32x4{v[0], v[1], v[2], v[3]};
+            p[1] = f32x4{v[4], v[5], v[6], v[7]};
+          } else
+            *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(o.e) + at) =
+                u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+        }
+      });
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ rows
+// 32 rows a workgroup, 8 threads each over the strips.
+__global__ __launch_bounds__(256) void rows_kernel(const float2* __restrict__ stats, int strips, int rows, const int64_t* __restrict__ target, long V,
+                                                   const float* __restrict__ target_score, float* __restrict__ lse, float* __restrict__ row_loss) {
+  __shared__ float2 part[8][32];
+  const int r = threadIdx.x & 31, q = threadIdx.x >> 5, n = blockIdx.x * 32 + r;
+  float top = -INFINITY, sum = 0.f;
+  if (n < rows) {
+#pragma unroll 4
+    for (int s = q; s < strips; s += 8) {
+      const float2 x = stats[(long)s * rows + n];
+      const float t = fmaxf(top, x.x);
+      if (t != -INFINITY) sum = sum * expf(top - t) + x.y * expf(x.x - t);
+      if (x.y != x.y) sum = x.y;                      // NaN scores leave no maximum behind
+      top = t;
+    }
+  }
+  part[q][r] = make_float2(top, sum);
+  __syncthreads();
+  if (q == 0 && n < rows) {
+    float t = -INFINITY, s = 0.f;
+    for (int i = 0; i < 8; ++i) t = fmaxf(t, part[i][r].x);
+    for (int i = 0; i < 8; ++i)
+      if (part[i][r].y != 0.f) s += part[i][r].y * expf(part[i][r].x - t);
+    const float l = t + logf(s);
+    lse[n] = l;
+    const int64_t y = target[n];
+    row_loss[n] = (y >= 0 && y < V) ? l - target_score[n] : 0.f;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ turn
+struct TurnArgs {
+  const void* e; long pitch_e;           // exponentials [rows][pitch_e]
+  const float2* stats; const float* lse; const float* target_score; const int64_t* target; const float* row_weight; const float* inv;
+  uint16_t* d; long plane_d;             // [planes][rows][pitch_e]; may be e itself (bfloat16)
+  uint16_t* dt; long pitch_t, plane_t;   // [planes][pitch_e][pitch_t]
+  int rows, V, strip;                    // strip: classes that share a maximum
+};
+
+// 64 rows x 64 classes a workgroup: d_tv = e_tv * exp(max_strip - lse_t) * w_t / n, the row's own class from its float32 score, written as it
+// stands and transposed.  Rows from `rows` to pitch_t and classes from V to pitch_e are zeros.
+template <bool F32>
+__global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
+  constexpr int P = F32 ? 3 : 1;
+  __shared__ uint16_t tile[P][64][66];
+  __shared__ float factor[2][64];     // of the tile's first and second 32 classes: strips of 32 are the shortest
+  __shared__ float own[64];
+  __shared__ int at[64];
+  const int v0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
+  if (threadIdx.x < 64) {
+    const int t = t0 + threadIdx.x;
+    float f[2] = {0.f, 0.f}, mine = 0.f;
+    int where = -1;
+    if (t < a.rows) {
+      const int64_t y = a.target[t];
+      if (y >= 0 && y < a.V) {
+        const float g = (a.row_weight ? a.row_weight[t] : 1.f) * *a.inv;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (v0 + 32 * k < a.V) f[k] = expf(a.stats[(long)((v0 + 32 * k) / a.strip) * a.rows + t].x - a.lse[t]) * g;
+        if (y >= v0 && y < v0 + 64) {
+          where = (int)(y - v0);
+          mine = (expf(a.target_score[t] - a.lse[t]) - 1.f) * g;
+        }
+      }
+    }
+    factor[0][threadIdx.x] = f[0];
+    factor[1][threadIdx.x] = f[1];
+    own[threadIdx.x] = mine;
+    at[threadIdx.x] = where;
+  }
+  __syncthreads();
+  const int c = (threadIdx.x & 15) * 4;
+#pragma unroll
+  for (int r = threadIdx.x >> 4; r < 64; r += 16) {
+    const int t = t0 + r, v = v0 + c;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (t < a.rows) {
+      const float f = factor[c >> 5][r];
+      if (f != 0.f) {
+        if (F32) {
+          const f32x4 w = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(a.e) + (long)t * a.pitch_e + v);
+          x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint16_t*>(a.e) + (long)t * a.pitch_e + v);
+          x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u);
+          x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] *= f;
+      }
+      const int y = at[r] - c;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (y == k && at[r] >= 0) x[k] = own[r];
+    }
+    uint16_t s[4][3];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (F32) split3(x[k], s[k]);
+      else s[k][0] = to_bf16(x[k]);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (t < a.rows)
+        *reinterpret_cast<u32x2*>(a.d + p * a.plane_d + (long)t * a.pitch_e + v) =
+            u32x2{(uint32_t)s[0][p] | ((uint32_t)s[1][p] << 16), (uint32_t)s[2][p] | ((uint32_t)s[3][p] << 16)};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tile[p][r][c + k] = s[k][p];
+    }
+  }
+  __syncthreads();
+  const int t = (threadIdx.x & 7) * 8;
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int v = threadIdx.x >> 3; v < 64; v += 32) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = (uint32_t)tile[p][t + 2 * k][v] | ((uint32_t)tile[p][t + 2 * k + 1][v] << 16);
+      *reinterpret_cast<u32x4*>(a.dt + p * a.plane_t + (long)(v0 + v) * a.pitch_t + t0 + t) = u32x4{w[0], w[1], w[2], w[3]};
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ operands
+// [rows][cols] of the caller, contiguous -> bfloat16 planes, as they stand [rows][pitch] (cols .. pitch zero) and/or transposed [cols][pitch_t]
+// (rows .. pitch_t zero).  64 x 64 a workgroup.
+template <bool F32>
+__global__ __launch_bounds__(256) void lay_out_kernel(const void* __restrict__ src, int rows, int cols, uint16_t* __restrict__ as_is, long pitch, long plane,
+                                                      uint16_t* __restrict__ turned, long pitch_t, long plane_t) {
+  constexpr int P = F32 ? 3 : 1;
+  __shared__ uint16_t tile[P][64][66];
+  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
+  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+    const int r = i >> 6, c = i & 63;
+    uint16_t s[3] = {0, 0, 0};
+    if (r0 + r < rows && c0 + c < cols) {
+      const long at = (long)(r0 + r) * cols + c0 + c;
+      if (F32) split3(reinterpret_cast<const float*>(src)[at], s);
+      else s[0] = reinterpret_cast<const uint16_t*>(src)[at];
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (as_is && r0 + r < rows && c0 + c < pitch) as_is[p * plane + (long)(r0 + r) * pitch + c0 + c] = s[p];
+      tile[p][r][c] = s[p];
+    }
+  }
+  if (!turned) return;
+  __syncthreads();
+  const int r = (threadIdx.x & 7) * 8;
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    for (int c = threadIdx.x >> 3; c < 64; c += 32) {
+      if (c0 + c >= cols || r0 + r >= pitch_t) continue;
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = (uint32_t)tile[p][r + 2 * k][c] | ((uint32_t)tile[p][r + 2 * k + 1][c] << 16);
+      *reinterpret_cast<u32x4*>(turned + p * plane_t + (long)(c0 + c) * pitch_t + r0 + r) = u32x4{w[0], w[1], w[2], w[3]};
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ gradients
+struct GradOut {
+  void* c; long ldc;          // [N][ldc], M values a row
+  const float* add;           // float32 [N][ldc] that is added first, or null
+  float* part; long part_stride;   // with splits: float32 [splits][N][ldc] instead
+  int c_bf16, wide;           // wide: rows of c start on 16 bytes and M is a multiple of 8
+};
+
+__device__ __forceinline__ void put8(const GradOut& o, long at, int left, const float (&v)[8]) {
+  if (o.c_bf16) {
+    uint16_t* p = reinterpret_cast<uint16_t*>(o.c) + at;
+    if (o.wide) *reinterpret_cast<u32x4*>(p) = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+    else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < left) p[k] = to_bf16(v[k]);
+    }
+  } else {
+    float* p = reinterpret_cast<float*>(o.c) + at;
+    if (o.wide) {
+      reinterpret_cast<f32x4*>(p)[0] = f32x4{v[0], v[1], v[2], v[3]};
+      reinterpret_cast<f32x4*>(p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < left) p[k] = v[k];
+    }
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(T::NT) void grad_kernel(TnArgs g, GradOut o) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tiles = g.tiles_m * g.tiles_n, split = blockIdx.x / tiles;
+  int tm, tn;
+  tn_tile_of(blockIdx.x - split * tiles, tiles, g.tiles_m, g.tiles_n, tm, tn);
+  const int m0 = tm * T::BM, n0 = tn * T::BN;
+  const long steps = (long)g.ksteps * g.pairs;
+  tn_acc acc[T::MI][T::NI];
+  tn_product<T>(g, lds, m0, n0, (int)(steps * split / g.splits), (int)(steps * (split + 1) / g.splits), acc);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j)
+    tn_rows<T>(lds, acc, j, [&](int row, int m, const float (&v)[8]) {
+      const int n = ns + j * 32 + row, left = g.M - (ms + m);
+      if (n >= g.N || left <= 0) return;
+      const long at = (long)n * o.ldc + ms + m;
+      GradOut q = o;
+      if (o.part) {
+        q.c = o.part + split * o.part_stride;
+        q.c_bf16 = 0;
+        q.wide = o.ldc % 4 == 0 && left >= 8;
+        put8(q, at, left, v);
+      } else if (o.add) {
+        float w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = v[k] + (k < left ? o.add[at + k] : 0.f);
+        put8(q, at, left, w);
+      } else put8(q, at, left, v);
+    });
+}
+
+// the parts of a split product, in order, and what was there before
+__global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ part, long stride, int splits, const float* __restrict__ add, long n, void* __restrict__ c,
+                                                    int c_bf16) {
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+    float s = add ? add[i] : 0.f;
+    for (int k = 0; k < splits; ++k) s += part[k * stride + i];
+    if (c_bf16) reinterpret_cast<uint16_t*>(c)[i] = to_bf16(s);
+    else reinterpret_cast<float*>(c)[i] = s;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+using Wide = TnTile<256, 256, 2, 4>;
+using Mid = TnTile<128, 128, 2, 2>;
+using Narrow = TnTile<128, 32, 4, 1>;     // few rows: as many workgroups as strips of 128 classes
+
+constexpr long CUS = 256;
+long up(long a, long b) { return (a + b - 1) / b * b; }
+
+struct Plan {
+  bool f32, grad, direct;        // direct: x and W are used where they are
+  long T, V, D, Kp, Vp, R, Rp;   // padded D and V; rows of a block, padded
+  int blocks, planes, pairs, tile_scores, strips, strip;
+  size_t inv, stats, lse, tscore, xp, wp, wt, xt, e, d, dt, dw, part, total, part_bytes;
+};
+
+// 256 x 256 tiles where they fill the chip, 128 x 128 ones where only those do, 128 x 32 for few rows
+int tile_for_scores(long rows, long V) {
+  if (rows <= 32) return 2;
+  return cdiv(V, 256) * (long)cdiv(rows, 256) >= CUS ? 0 : 1;
+}
+long grad_tile(long M, long N) { return cdiv(M, 256) * (long)cdiv(N, 256) >= CUS ? 256 : 128; }
+// parts of k: enough for every CU (two 128-tiles fit one), while a part keeps at least 16 steps and all parts together 2^28 values
+int grad_splits(long M, long N, long steps) {
+  const long t = grad_tile(M, N), tiles = cdiv(M, t) * (long)cdiv(N, t), want = t == 256 ? CUS : 2 * CUS;
+  long s = tiles >= want * 3 / 4 ? 1 : cdiv(want, tiles);
+  if (s > steps / 16) s = steps / 16;
+  while (s > 1 && s * M * N > (1L << 28)) --s;
+  return s < 1 ? 1 : (int)s;
+}
+
+Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
+  Plan p{};
+  p.f32 = f32; p.grad = grad; p.T = T; p.V = V; p.D = D;
+  p.planes = f32 ? 3 : 1;
+  p.pairs = f32 ? 6 : 1;
+  p.Kp = up(D, 64);
+  p.Vp = up(V, 64);
+  p.direct = direct && !f32 && D % 64 == 0;
+  const long most = grad ? (1L << (f32 ? 27 : 29)) : (1L << 31);     // (row, class) pairs of a block; without gradients only statistics are held
+  p.R = T;
+  if (T * p.Vp > most) {
+    p.R = most / p.Vp / 256 * 256;
+    if (p.R < 256) p.R = 256;
+    if (p.R > T) p.R = T;
+  }
+  p.blocks = cdiv(T, p.R);
+  p.Rp = up(p.R, 64);
+  p.tile_scores = tile_for_scores(p.R, V);
+  p.strip = p.tile_scores == 0 ? Wide::WM : p.tile_scores == 1 ? Mid::WM : Narrow::WM;
+  p.strips = cdiv(V, p.strip);
+  size_t at = 0;
+  const auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+  p.inv = take(4);
+  p.stats = take((size_t)p.strips * p.R * 8);
+  p.lse = take((size_t)p.R * 4);
+  p.tscore = take((size_t)p.R * 4);
+  if (!p.direct) {
+    p.xp = take((size_t)p.planes * T * p.Kp * 2);
+    p.wp = take((size_t)p.planes * V * p.Kp * 2);
+  }
+  if (grad) {
+    p.wt = take((size_t)p.planes * D * p.Vp * 2);
+    p.xt = take((size_t)p.planes * D * p.Rp * 2);
+    p.e = take((size_t)p.R * p.Vp * (f32 ? 4 : 2));
+    p.d = f32 ? take((size_t)3 * p.R * p.Vp * 2) : p.e;
+    p.dt = take((size_t)p.planes * p.Vp * p.Rp * 2);
+    if (p.blocks > 1 && !f32) p.dw = take((size_t)V * D * 4);
+    const int s1 = grad_splits(D, p.R, p.Vp / 64 * p.pairs), s2 = grad_splits(D, V, p.Rp / 64 * p.pairs);
+    const size_t b1 = s1 > 1 ? (size_t)s1 * D * p.R * 4 : 0, b2 = s2 > 1 ? (size_t)s2 * D * V * 4 : 0;
+    p.part_bytes = b1 > b2 ? b1 : b2;
+    p.part = take(p.part_bytes);
+  }
+  p.total = at;
+  return p;
+}
+
+template <class T, bool F32>
+int launch_scores(TnArgs g, const ScoreOut& o, hipStream_t st) {
+  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(scores_kernel<T, F32>), T::LDS, "dppm_loss_ce"));
+  g.tiles_m = cdiv(g.M, T::BM);
+  g.tiles_n = cdiv(g.N, T::BN);
+  hipLaunchKernelGGL((scores_kernel<T, F32>), dim3(g.tiles_m * g.tiles_n), dim3(T::NT), T::LDS, st, g, o);
+  return DPPM_OK;
+}
+
+template <class T>
+int launch_grad(TnArgs g, const GradOut& o, hipStream_t st) {
+  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(grad_kernel<T>), T::LDS, "dppm_loss_ce"));
+  g.tiles_m = cdiv(g.M, T::BM);
+  g.tiles_n = cdiv(g.N, T::BN);
+  hipLaunchKernelGGL((grad_kernel<T>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(T::NT), T::LDS, st, g, o);
+  return DPPM_OK;
+}
+
+// c[n][m] (+= add) = sum_k A[m][k] B[n][k]
+int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, size_t part_bytes, hipStream_t st) {
+  GradOut o{};
+  o.c = c; o.ldc = g.M; o.add = add; o.c_bf16 = c_bf16;
+  o.wide = g.M % 8 == 0 && (uintptr_t)c % 16 == 0;
+  g.splits = grad_splits(g.M, g.N, (long)g.ksteps * g.pairs);
+  if (g.splits > 1 && (size_t)g.splits * g.M * g.N * 4 > part_bytes) g.splits = 1;
+  if (g.splits > 1) { o.part = part; o.part_stride = (long)g.M * g.N; o.add = nullptr; }
+  if (grad_tile(g.M, g.N) == 256) DPPM_TRY(launch_grad<Wide>(g, o, st));
+  else DPPM_TRY(launch_grad<Mid>(g, o, st));
+  if (g.splits > 1) {
+    const long n = (long)g.M * g.N, blocks = (n + 255) / 256;
+    hipLaunchKernelGGL(parts_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, part, n, g.splits, add, n, c, (int)c_bf16);
+  }
+  return DPPM_OK;
+}
+
+void lay_out(bool f32, const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, hipStream_t st) {
+  const long r = turned ? (pitch_t > rows ? pitch_t : rows) : rows, c = as_is ? pitch : cols;
+  const dim3 grid((unsigned)cdiv(c, 64), (unsigned)cdiv(r, 64));
+  if (f32) hipLaunchKernelGGL((lay_out_kernel<true>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t);
+  else hipLaunchKernelGGL((lay_out_kernel<false>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t);
+}
+
+bool sizes_ok(int64_t T, int64_t V, int64_t D) { return T >= 0 && V >= 1 && D >= 1 && T < (1L << 30) && V <= (1L << 23) && D <= (1L << 16); }   // 255 rows of any operand lie within 2^32 bytes
+// the layout is the same whether or not the operands can be used where they are, so that the size does not depend on addresses
+Plan plan_for(int64_t T, int64_t V, int64_t D, bool bf16, bool grad, bool aligned) {
+  Plan p = plan_of(T, V, D, !bf16, grad, true);
+  if (p.direct && !aligned) p = plan_of(T, V, D, !bf16, grad, false);
+  return p;
+}
+
+}  // namespace
+}  // namespace dppm
+
+using namespace dppm;
+
+extern "C" size_t dppm_loss_ce_workspace_bytes(int64_t T, int64_t V, int64_t D, int bf16, int want_grad) {
+  if (!sizes_ok(T, V, D) || T == 0) return 0;
+  const size_t a = plan_for(T, V, D, bf16, want_grad, true).total, b = plan_for(T, V, D, bf16, want_grad, false).total;
+  return a > b ? a : b;
+}
+
+extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16, const int64_t* target, const float* row_weight, double denom, int64_t T,
+                                    int64_t V, int64_t D, float* loss_out, float* row_loss, void* dx, void* dweight, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  DPPM_REQUIRE(sizes_ok(T, V, D), "dppm_loss_ce_fwd_bwd: T=%ld V=%ld D=%ld", (long)T, (long)V, (long)D);
+  DPPM_REQUIRE(denom >= 0, "dppm_loss_ce_fwd_bwd: denom=%g", denom);
+  DPPM_REQUIRE(T >= 1, "dppm_loss_ce_fwd_bwd: no rows");
+  DPPM_REQUIRE(x && weight && target && loss_out && row_loss && workspace, "dppm_loss_ce_fwd_bwd: null pointer");
+  DPPM_REQUIRE((dx == nullptr) == (dweight == nullptr), "dppm_loss_ce_fwd_bwd: dx and dweight come together");
+  DPPM_REQUIRE((uintptr_t)workspace % 16 == 0, "dppm_loss_ce_fwd_bwd: the workspace must be 16-byte aligned");
+  const bool grad = dx != nullptr, aligned = ((uintptr_t)x | (uintptr_t)weight) % 16 == 0;
+  const Plan p = plan_for(T, V, D, bf16, grad, aligned);
+  DPPM_REQUIRE(workspace_bytes >= p.total, "dppm_loss_ce_fwd_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
+  const hipStream_t st = as_stream(stream);
+  char* ws = reinterpret_cast<char*>(workspace);
+  const auto h = [&](size_t at) { return reinterpret_cast<uint16_t*>(ws + at); };
+  const auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
+  float2* stats = reinterpret_cast<float2*>(ws + p.stats);
+  hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, target, (long)T, (long)V, (float)denom, f(p.inv));
+  const uint16_t *xp = reinterpret_cast<const uint16_t*>(x), *wp = reinterpret_cast<const uint16_t*>(weight);
+  if (!p.direct || grad) lay_out(p.f32, weight, V, D, p.direct ? nullptr : h(p.wp), p.Kp, grad ? h(p.wt) : nullptr, p.Vp, st);
+  if (!p.direct) {
+    lay_out(p.f32, x, T, D, h(p.xp), p.Kp, nullptr, 0, st);
+    xp = h(p.xp); wp = h(p.wp);
+  }
+  for (int b = 0; b < p.blocks; ++b) {
+    const long t0 = b * p.R, rows = T - t0 < p.R ? T - t0 : p.R, Rp = up(rows, 64);
+    TnArgs g{};
+    g.A = wp; g.lda = p.Kp; g.plane_a = V * p.Kp; g.M = (int)V;
+    g.B = xp + t0 * p.Kp; g.ldb = p.Kp; g.plane_b = T * p.Kp; g.N = (int)rows;
+    g.ksteps = (int)(p.Kp / 64); g.pairs = p.pairs; g.splits = 1;
+    ScoreOut o{};
+    o.stats = stats; o.target_score = f(p.tscore); o.target = target + t0; o.e = grad ? ws + p.e : nullptr; o.pitch = p.Vp; o.V = (int)V;
+    if (p.tile_scores == 0) DPPM_TRY(p.f32 ? (launch_scores<Wide, true>(g, o, st)) : (launch_scores<Wide, false>(g, o, st)));
+    else if (p.tile_scores == 1) DPPM_TRY(p.f32 ? (launch_scores<Mid, true>(g, o, st)) : (launch_scores<Mid, false>(g, o, st)));
+    else DPPM_TRY(p.f32 ? (launch_scores<Narrow, true>(g, o, st)) : (launch_scores<Narrow, false>(g, o, st)));
+    hipLaunchKernelGGL(rows_kernel, dim3(cdiv(rows, 32)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
+    if (!grad) continue;
+    TurnArgs a{};
+    a.e = ws + p.e; a.pitch_e = p.Vp; a.stats = stats; a.lse = f(p.lse); a.target_score = f(p.tscore); a.target = target + t0;
+    a.row_weight = row_weight ? row_weight + t0 : nullptr; a.inv = f(p.inv);
+    a.d = h(p.d); a.plane_d = rows * p.Vp; a.dt = h(p.dt); a.pitch_t = Rp; a.plane_t = p.Vp * Rp;
+    a.rows = (int)rows; a.V = (int)V; a.strip = p.strip;
+    const dim3 grid((unsigned)(p.Vp / 64), (unsigned)(Rp / 64));
+    if (p.f32) hipLaunchKernelGGL((turn_kernel<true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((turn_kernel<false>), grid, dim3(256), 0, st, a);
+    const size_t es = bf16 ? 2 : 4;
+    lay_out(p.f32, reinterpret_cast<const char*>(x) + t0 * D * es, rows, D, nullptr, 0, h(p.xt), Rp, st);
+    TnArgs gx{};       // dx[t][d] = sum_v d[t][v] W^T[d][v]
+    gx.A = h(p.wt); gx.lda = p.Vp; gx.plane_a = D * p.Vp; gx.M = (int)D;
+    gx.B = a.d; gx.ldb = p.Vp; gx.plane_b = a.plane_d; gx.N = (int)rows;
+    gx.ksteps = (int)(p.Vp / 64); gx.pairs = p.pairs;
+    DPPM_TRY(grad_product(gx, reinterpret_cast<char*>(dx) + t0 * D * es, bf16, nullptr, f(p.part), p.part_bytes, st));
+    TnArgs gw{};       // dW[v][d] = sum_t d^T[v][t] x^T[d][t]
+    gw.A = h(p.xt); gw.lda = Rp; gw.plane_a = D * Rp; gw.M = (int)D;
+    gw.B = a.dt; gw.ldb = Rp; gw.plane_b = a.plane_t; gw.N = (int)V;
+    gw.ksteps = (int)(Rp / 64); gw.pairs = p.pairs;
+    const bool last = b == p.blocks - 1;
+    float* sum = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
+    DPPM_TRY(grad_product(gw, last || p.f32 ? dweight : (void*)sum, bf16 && last, b == 0 ? nullptr : sum, f(p.part), p.part_bytes, st));
+  }
+  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, f(p.inv), (long)T, loss_out);
+  return check_launch("dppm_loss_ce_fwd_bwd");
+}

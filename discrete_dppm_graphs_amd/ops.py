@@ -454,6 +454,40 @@ def embedding_wgrad(dout, ids, num_rows, scale=1.0, out=None, accumulate=False):
     return out
 
 
+def loss_ce(x, weight, target, row_weight=None, denom=None, want_grad=True):
+    """Softmax cross entropy over classes: x [T, D], weight [V, D] (both float32 or both bfloat16), target [T] int64 (a class outside
+    [0, V) means none: the row counts for nothing), row_weight None or [T] float32, denom a positive number (default: the number of rows
+    that have a class).  Returns (loss float32 0-d, row_loss [T] float32, dx or None, dweight or None), gradients in x's type, of
+    loss = sum(row_weight * row_loss) / denom (include/dppm_hip.h, dppm_loss_ce_fwd_bwd)."""
+    x = _chk_float(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x: shape {tuple(x.shape)}, expected [T, D]")
+    T, D = x.shape
+    if isinstance(weight, torch.Tensor) and (weight.dim() != 2 or weight.shape[1] != D):
+        raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [V, {D}]")
+    _chk_device(_chk(weight, "weight", None, x.dtype), "weight", x, "x")
+    _chk_device(_chk(target, "target", (T,), torch.int64), "target", x, "x")
+    if row_weight is not None:
+        _chk_device(_chk(row_weight, "row_weight", (T,)), "row_weight", x, "x")
+    if denom is not None and not 0 < float(denom) < float("inf"):
+        raise ValueError(f"denom {denom}: expected a positive number or None")
+    V, bf16 = weight.shape[0], x.dtype == torch.bfloat16
+    if T == 0:
+        zero = torch.zeros((), device=x.device, dtype=torch.float32)
+        return (zero, zero.new_zeros(0), torch.empty_like(x), torch.zeros_like(weight)) if want_grad else (zero, zero.new_zeros(0), None, None)
+    nbytes = lib.dppm_loss_ce_workspace_bytes(T, V, D, bf16, want_grad)
+    with _on(x.device):
+        out = torch.empty(T + 1, device=x.device, dtype=torch.float32)
+        loss, row_loss = out[T], out[:T]
+        dx, dweight = (torch.empty_like(x), torch.empty_like(weight)) if want_grad else (None, None)
+        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+        check(lib.dppm_loss_ce_fwd_bwd(x.data_ptr(), weight.data_ptr(), bf16, target.data_ptr(), None if row_weight is None else row_weight.data_ptr(),
+                                       0.0 if denom is None else float(denom), T, V, D, loss.data_ptr(), row_loss.data_ptr(),
+                                       None if dx is None else dx.data_ptr(), None if dx is None else dweight.data_ptr(), ws.data_ptr(), nbytes,
+                                       _raw_stream(x.device)), "dppm_loss_ce_fwd_bwd")
+    return loss, row_loss, dx, dweight
+
+
 STATE_BLOCK = 256      # values of a tensor that share one scale of its 8-bit moments (include/dppm_hip.h, dppm_tensor_entry)
 
 

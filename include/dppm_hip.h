@@ -282,6 +282,21 @@ size_t dppm_embedding_wgrad_workspace_bytes(int64_t T, int64_t V, int64_t D);
 int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64_t* ids, float scale, void* dweight, int dweight_bf16, int accumulate,
                          int64_t T, int64_t V, int64_t D, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Softmax cross entropy over V classes from the last hidden layer x [T][D] and the classes' rows weight [V][D] (both float32, or bfloat16
+ * with bf16 != 0), forward and gradients, without the scores in memory:
+ *   s = x weight^T;  row_loss[t] = log sum_v exp s[t][v] - s[t][target[t]];  *loss_out = sum_t row_weight[t] row_loss[t] / denom;
+ *   dx = d weight, dweight = d^T x with d[t][v] = (softmax(s[t])[v] - [v = target[t]]) row_weight[t] / denom.
+ * A row whose target lies outside [0, V) has no class: its row_loss and its row of dx are zero and it adds nothing else.  row_weight
+ * (nullable) [T]; denom: 0 stands for the number of rows that have a class (1 if none has).  loss_out: one float; row_loss [T] float32.
+ * dx [T][D] and dweight [V][D], in the inputs' type and overwritten, are both given or both NULL.  bfloat16: products of bfloat16 operands
+ * (d is rounded to bfloat16 once), sums in float32.  float32: operands split into three bfloat16 pieces, float32-grade products
+ * (DPPM_PREC_F32X6).  The same bits from call to call.  T < 2^30, V <= 2^23, D <= 2^16.
+ * workspace: dppm_loss_ce_workspace_bytes(), 16-byte aligned; it holds up to 2^29 exponentials (2^27 for float32) at a time whatever T. */
+size_t dppm_loss_ce_workspace_bytes(int64_t T, int64_t V, int64_t D, int bf16, int want_grad);
+int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16, const int64_t* target, const float* row_weight, double denom,
+                         int64_t T, int64_t V, int64_t D, float* loss_out, float* row_loss, void* dx, void* dweight, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 /* One tensor of an AdamW step: an entry of the DEVICE table dppm_adamw_step reads.  param float32 (16-byte aligned); grad float32 or
  * bfloat16 (16 / 8-byte aligned); copy (nullable): bfloat16 working weights, written from the new param (8-byte aligned).
  * 32-bit moments: exp_avg / exp_avg_sq float32 [numel] (16-byte aligned), scales unused.

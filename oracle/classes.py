@@ -27,21 +27,23 @@ def embedding_wgrad(dout, ids, rows, scale=1.0):
 
 
 def cross_entropy(x, weight, target, row_weight=None, denom=None):
-    """-> (loss, row_loss, dx, dweight) in float64."""
+    """-> (loss, row_loss, dx, dweight, and the rows' softmax and d, the gradient of the scores) in float64."""
     x, w = x.double(), weight.double()
     T, V = x.shape[0], w.shape[0]
     ok = (target >= 0) & (target < V)
     n = float(ok.sum().clamp(min=1)) if denom is None else float(denom)
-    share = (torch.ones(T, dtype=torch.float64) if row_weight is None else row_weight.double()) / n
-    row_loss, dl = torch.zeros(T, dtype=torch.float64), torch.zeros(T, V, dtype=torch.float64)
-    for t in range(T):
-        if ok[t]:
-            s = w @ x[t]
-            logp = s - torch.logsumexp(s, 0)
-            row_loss[t] = -logp[target[t]]
-            dl[t] = logp.exp() * share[t]
-            dl[t, target[t]] -= share[t]
-    return (row_loss * torch.where(ok, share, torch.zeros(()).double())).sum(), row_loss, dl @ w, dl.t() @ x
+    share = torch.where(ok, torch.ones(T, dtype=torch.float64) if row_weight is None else row_weight.double(), torch.zeros(T, dtype=torch.float64)) / n
+    s = x @ w.t()
+    s = torch.where(ok.unsqueeze(1), s, torch.zeros((), dtype=torch.float64))      # a row without a class does not count, whatever it holds
+    x = torch.where(ok.unsqueeze(1), x, torch.zeros((), dtype=torch.float64))
+    lse = torch.logsumexp(s, 1, keepdim=True)
+    at = target.clamp(0, V - 1).unsqueeze(1)
+    row_loss = torch.where(ok, (lse - s.gather(1, at)).squeeze(1), torch.zeros((), dtype=torch.float64))
+    p = (s - lse).exp()
+    d = p.clone()
+    d.scatter_add_(1, at, torch.full((T, 1), -1.0, dtype=torch.float64))
+    d = torch.where(ok.unsqueeze(1), d * share.unsqueeze(1), torch.zeros((), dtype=torch.float64))
+    return (row_loss * share).sum(), row_loss, d @ w, d.t() @ x, p, d
 
 
 def round_bits(n, tensor, step, seed):

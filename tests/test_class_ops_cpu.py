@@ -74,3 +74,31 @@ def test_embedding_entries_refuse():
     need = lib.dppm_embedding_wgrad_workspace_bytes(3, 5, 4)
     assert lib.dppm_embedding_wgrad(one, 0, one, 1.0, one, 0, 0, 3, 5, 4, one, need - 1, None) == -1
     assert lib.dppm_embedding_wgrad(one, 0, one, 1.0, one, 0, 0, 3, 5, 4, C.c_void_p(8), need, None) == -1
+
+
+def test_cross_entropy_oracle_is_torch_cross_entropy():
+    torch.manual_seed(3)
+    x, w = torch.randn(9, 4, dtype=torch.float64, requires_grad=True), torch.randn(6, 4, dtype=torch.float64, requires_grad=True)
+    target = torch.tensor([0, 5, 3, -100, 2, 2, -100, 1, 4])
+    loss = torch.nn.functional.cross_entropy(x @ w.t(), target, ignore_index=-100)
+    loss.backward()
+    got = classes.cross_entropy(x.detach(), w.detach(), target)
+    assert torch.allclose(got[0], loss.detach()) and torch.allclose(got[2], x.grad) and torch.allclose(got[3], w.grad)
+    weighted = classes.cross_entropy(x.detach(), w.detach(), target, torch.arange(9.0), 5.0)
+    per_row = torch.nn.functional.cross_entropy(x @ w.t(), target, ignore_index=-100, reduction="none")
+    g = torch.autograd.grad((per_row * torch.arange(9.0)).sum() / 5.0, (x, w))
+    assert torch.allclose(weighted[2], g[0]) and torch.allclose(weighted[3], g[1])
+
+
+def test_loss_ce_entry_refuses():
+    one = C.c_void_p(16)
+    good = dict(x=one, w=one, bf=1, target=one, rw=None, denom=0.0, T=4, V=5, D=8, loss=one, row=one, dx=one, dw=one, ws=one, n=1 << 40, st=None)
+    for bad in ({"x": None}, {"w": None}, {"target": None}, {"loss": None}, {"row": None}, {"ws": None}, {"dx": None}, {"dw": None}, {"T": 0}, {"T": -1},
+                {"T": 1 << 30}, {"V": 0}, {"V": (1 << 23) + 1}, {"D": 0}, {"D": (1 << 16) + 1}, {"denom": -1.0}, {"denom": float("nan")}, {"ws": C.c_void_p(8)}):
+        assert lib.dppm_loss_ce_fwd_bwd(*{**good, **bad}.values()) == -1, bad
+    need = lib.dppm_loss_ce_workspace_bytes(4, 5, 8, 1, 1)
+    assert need > lib.dppm_loss_ce_workspace_bytes(4, 5, 8, 1, 0) > 0
+    assert lib.dppm_loss_ce_fwd_bwd(*{**good, "n": 64}.values()) == -1
+    # beside a copy of x, memory is that of one block of rows, whatever their number
+    many, more = lib.dppm_loss_ce_workspace_bytes(1 << 16, 1 << 17, 1024, 1, 1), lib.dppm_loss_ce_workspace_bytes(1 << 17, 1 << 17, 1024, 1, 1)
+    assert more - many <= (1 << 16) * 1024 * 2 + 4096 and more < 8 << 30
