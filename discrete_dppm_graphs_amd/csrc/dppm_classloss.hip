@@ -12,7 +12,7 @@
 //  * rows: lse, the rows' losses;
 //  * turn: exponentials to d, rounded once to the operands' type, as it stands and transposed;
 //  * dx = d W and dW = d^T x, both with the contracted dimension contiguous in both operands: W and x are transposed once.
-// The exponentials held at a time are those of one block of rows, at most 2^29 (bfloat16) or 2^27 (float32) of them: memory does not grow
+// The exponentials held at a time are those of one block of rows, at most 2^30 (bfloat16) or 2^27 (float32) of them: memory does not grow
 // with T.  Several blocks add up dW in float32.
 #include "dppm_common.h"
 #include "dppm_tngemm.h"
@@ -47,25 +47,34 @@ __device__ __forceinline__ void split3(float v, uint16_t (&out)[3]) {
 }
 
 // ------------------------------------------------------------------------------------------------ counting rows, losses
-__global__ __launch_bounds__(1024) void count_kernel(const int64_t* __restrict__ target, long T, long V, float denom, float* __restrict__ inv) {
+// 1 / denom, or 1 / (rows with a class) where none is given; every thread of the 1024 gets it
+__device__ __forceinline__ float inverse_of_rows(const int64_t* target, long T, long V, float denom) {
   __shared__ uint32_t w[16];
   uint32_t n = 0;
-  for (long t = threadIdx.x; t < T; t += 1024) n += target[t] >= 0 && target[t] < V;
+  if (!(denom > 0.f)) {
+#pragma unroll 4
+    for (long t = threadIdx.x; t < T; t += 1024) n += target[t] >= 0 && target[t] < V;
+  }
 #pragma unroll
   for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = n;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    uint32_t all = 0;
-    for (int i = 0; i < 16; ++i) all += w[i];
-    *inv = 1.f / (denom > 0.f ? denom : (float)(all ? all : 1u));
-  }
+  uint32_t all = 0;
+  for (int i = 0; i < 16; ++i) all += w[i];
+  return 1.f / (denom > 0.f ? denom : (float)(all ? all : 1u));
 }
 
-__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ row_loss, const float* __restrict__ row_weight, const float* __restrict__ inv, long T,
-                                                    float* __restrict__ loss) {
+__global__ __launch_bounds__(1024) void count_kernel(const int64_t* __restrict__ target, long T, long V, float denom, float* __restrict__ inv) {
+  const float x = inverse_of_rows(target, T, V, denom);
+  if (threadIdx.x == 0) *inv = x;
+}
+
+// `inv`: what count_kernel left, or null (no gradients: nothing needed it before)
+__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ row_loss, const float* __restrict__ row_weight, const int64_t* __restrict__ target, long V,
+                                                    float denom, const float* __restrict__ inv, long T, float* __restrict__ loss) {
   __shared__ double w[16];
   double s = 0.0;
+#pragma unroll 4
   for (long t = threadIdx.x; t < T; t += 1024) {
     const float l = row_loss[t];
     if (l != 0.f) s += (double)l * (row_weight ? row_weight[t] : 1.f);      // rows without a class have 0, whatever their weight
@@ -73,11 +82,12 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ ro
 #pragma unroll
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
+  const float scale = inv ? *inv : inverse_of_rows(target, T, V, denom);
   __syncthreads();
   if (threadIdx.x == 0) {
     double all = 0.0;
     for (int i = 0; i < 16; ++i) all += w[i];
-    *loss = (float)(all * *inv);
+    *loss = (float)(all * scale);
   }
 }
 
@@ -91,7 +101,7 @@ struct ScoreOut {
   int V;
 };
 
-// m = class, n = row: a lane holds 16 classes of one row per 32 x 32 tile, so that maxima and sums run inside lanes and cross one pair.
+// m = class, n = row: a lane holds classes of one row per fragment, so that maxima and sums run inside lanes and then over four of them.
 template <class T, bool F32>
 __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -102,49 +112,51 @@ __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
   tn_product<T>(g, lds, m0, n0, 0, g.ksteps * g.pairs, acc);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;     // this wave's strip of classes, its rows
-  const int strip = ms / T::WM, half = (lane >> 5) * 4;
+  const int strip = ms / T::WM, first = ms + (lane >> 4) * 4;                         // class of acc[0][.][0]
 #pragma unroll
   for (int j = 0; j < T::NI; ++j) {
-    const int n = ns + j * 32 + (lane & 31);
+    const int n = ns + j * 16 + (lane & 15);
     if (ms + T::WM > o.V) {      // classes behind the last
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (ms + i * 32 + (k >> 2) * 8 + half + (k & 3) >= o.V) acc[i][j][k] = -INFINITY;
+        for (int k = 0; k < 4; ++k)
+          if (first + i * 16 + k >= o.V) acc[i][j][k] = -INFINITY;
     }
     const int64_t y = n < g.N ? o.target[n] : -1;
     const bool here = y >= ms && y < ms + T::WM && y < o.V;
     if (__any(here)) {
-      const int at = (int)(y - ms);
+      const int at = (int)(y - first);
 #pragma unroll
       for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (here && at == i * 32 + (k >> 2) * 8 + half + (k & 3)) o.target_score[n] = acc[i][j][k];
+        for (int k = 0; k < 4; ++k)
+          if (here && at == i * 16 + k) o.target_score[n] = acc[i][j][k];
     }
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-      for (int k = 0; k < 16; ++k) top = fmaxf(top, acc[i][j][k]);
+      for (int k = 0; k < 4; ++k) top = fmaxf(top, acc[i][j][k]);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float ref = top == -INFINITY ? 0.f : top;      // a strip of nothing but -inf: exponentials of 0
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
+      for (int k = 0; k < 4; ++k) {
         const float e = exp_of<F32>(acc[i][j][k] - ref);
         acc[i][j][k] = e;
         sum += e;
       }
+    sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
-    if (lane < 32 && n < g.N && ms < o.V) o.stats[(long)strip * g.N + n] = make_float2(top, sum);
+    if (lane < 16 && n < g.N && ms < o.V) o.stats[(long)strip * g.N + n] = make_float2(top, sum);
   }
   if (o.e) {
 #pragma unroll
-    for (int j = 0; j < T::NI; ++j)
+    for (int j = 0; j < T::WN / 32; ++j)
       tn_rows<T>(lds, acc, j, [&](int row, int m, const float (&v)[8]) {
         const int n = ns + j * 32 + row, c = ms + m;
         if (n < g.N && c < o.pitch) {
@@ -162,29 +174,44 @@ __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-// 32 rows a workgroup, 8 threads each over the strips.
+// ROWS rows a workgroup, 256 / ROWS threads each over the strips: 32, so that a strip's line is read whole, or 2 for few rows
+template <int ROWS>
 __global__ __launch_bounds__(256) void rows_kernel(const float2* __restrict__ stats, int strips, int rows, const int64_t* __restrict__ target, long V,
                                                    const float* __restrict__ target_score, float* __restrict__ lse, float* __restrict__ row_loss) {
-  __shared__ float2 part[8][32];
-  const int r = threadIdx.x & 31, q = threadIdx.x >> 5, n = blockIdx.x * 32 + r;
+  constexpr int LANES = 256 / ROWS, AHEAD = 8;
+  __shared__ float2 part[LANES][ROWS];
+  const int r = threadIdx.x % ROWS, q = threadIdx.x / ROWS, n = blockIdx.x * ROWS + r;
   float top = -INFINITY, sum = 0.f;
   if (n < rows) {
-#pragma unroll 4
-    for (int s = q; s < strips; s += 8) {
-      const float2 x = stats[(long)s * rows + n];
-      const float t = fmaxf(top, x.x);
-      if (t != -INFINITY) sum = sum * expf(top - t) + x.y * expf(x.x - t);
-      if (x.y != x.y) sum = x.y;                      // NaN scores leave no maximum behind
+    for (int s0 = q; s0 < strips; s0 += AHEAD * LANES) {
+      float2 x[AHEAD];
+      float t = top;
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int s = s0 + u * LANES;
+        x[u] = s < strips ? stats[(long)s * rows + n] : make_float2(-INFINITY, 0.f);
+        t = fmaxf(t, x[u].x);
+      }
+      sum = top == -INFINITY ? sum : sum * expf(top - t);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (x[u].y != 0.f) sum += x[u].x == -INFINITY ? x[u].y : x[u].y * expf(x[u].x - t);      // NaN scores leave no maximum behind, only a sum
       top = t;
     }
   }
   part[q][r] = make_float2(top, sum);
-  __syncthreads();
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) {
+    __syncthreads();
+    if (q < o) {
+      const float2 x = part[q][r], y = part[q + o][r];
+      const float t = fmaxf(x.x, y.x);
+      const float sx = x.y == 0.f || x.x == -INFINITY ? x.y : x.y * expf(x.x - t), sy = y.y == 0.f || y.x == -INFINITY ? y.y : y.y * expf(y.x - t);
+      part[q][r] = make_float2(t, sx + sy);
+    }
+  }
   if (q == 0 && n < rows) {
-    float t = -INFINITY, s = 0.f;
-    for (int i = 0; i < 8; ++i) t = fmaxf(t, part[i][r].x);
-    for (int i = 0; i < 8; ++i)
-      if (part[i][r].y != 0.f) s += part[i][r].y * expf(part[i][r].x - t);
+    const float t = part[0][r].x, s = part[0][r].y;
     const float l = t + logf(s);
     lse[n] = l;
     const int64_t y = target[n];
@@ -202,7 +229,7 @@ struct TurnArgs {
 };
 
 // 64 rows x 64 classes a workgroup: d_tv = e_tv * exp(max_strip - lse_t) * w_t / n, the row's own class from its float32 score, written as it
-// stands and transposed.  Rows from `rows` to pitch_t and classes from V to pitch_e are zeros.
+// stands and transposed.  Rows behind the last and classes behind the last are zeros, up to whole tiles.
 template <bool F32>
 __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
   constexpr int P = F32 ? 3 : 1;
@@ -289,24 +316,46 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
 // ------------------------------------------------------------------------------------------------ operands
 // [rows][cols] of the caller, contiguous -> bfloat16 planes, as they stand [rows][pitch] (cols .. pitch zero) and/or transposed [cols][pitch_t]
 // (rows .. pitch_t zero).  64 x 64 a workgroup.
-template <bool F32>
+// WIDE: cols and the source's address allow 16-byte reads (4 or 8 values).
+template <bool F32, bool WIDE>
 __global__ __launch_bounds__(256) void lay_out_kernel(const void* __restrict__ src, int rows, int cols, uint16_t* __restrict__ as_is, long pitch, long plane,
                                                       uint16_t* __restrict__ turned, long pitch_t, long plane_t) {
-  constexpr int P = F32 ? 3 : 1;
+  constexpr int P = F32 ? 3 : 1, VEC = WIDE ? (F32 ? 4 : 8) : 1, PER_ROW = 64 / VEC;
   __shared__ uint16_t tile[P][64][66];
   const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int r = i >> 6, c = i & 63;
-    uint16_t s[3] = {0, 0, 0};
+#pragma unroll 4
+  for (int i = threadIdx.x; i < 64 * PER_ROW; i += 256) {
+    const int r = i / PER_ROW, c = i % PER_ROW * VEC;
+    uint16_t s[VEC][3];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s[k][0] = s[k][1] = s[k][2] = 0;
     if (r0 + r < rows && c0 + c < cols) {
       const long at = (long)(r0 + r) * cols + c0 + c;
-      if (F32) split3(reinterpret_cast<const float*>(src)[at], s);
-      else s[0] = reinterpret_cast<const uint16_t*>(src)[at];
+      if constexpr (F32) {
+        float v[VEC];
+        if constexpr (WIDE) {
+          const f32x4 w = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(src) + at);
+          v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+        } else v[0] = reinterpret_cast<const float*>(src)[at];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) split3(v[k], s[k]);
+      } else if constexpr (WIDE) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(src) + at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { s[2 * k][0] = (uint16_t)w[k]; s[2 * k + 1][0] = (uint16_t)(w[k] >> 16); }
+      } else s[0][0] = reinterpret_cast<const uint16_t*>(src)[at];
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      if (as_is && r0 + r < rows && c0 + c < pitch) as_is[p * plane + (long)(r0 + r) * pitch + c0 + c] = s[p];
-      tile[p][r][c] = s[p];
+      if (as_is && r0 + r < rows && c0 + c < pitch) {
+        uint16_t* to = as_is + p * plane + (long)(r0 + r) * pitch + c0 + c;
+        if constexpr (VEC == 8) *reinterpret_cast<u32x4*>(to) = u32x4{s[0][p] | (uint32_t)s[1][p] << 16, s[2][p] | (uint32_t)s[3][p] << 16,
+                                                                     s[4][p] | (uint32_t)s[5][p] << 16, s[6][p] | (uint32_t)s[7][p] << 16};
+        else if constexpr (VEC == 4) *reinterpret_cast<u32x2*>(to) = u32x2{s[0][p] | (uint32_t)s[1][p] << 16, s[2][p] | (uint32_t)s[3][p] << 16};
+        else *to = s[0][p];
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) tile[p][r][c + k] = s[k][p];
     }
   }
   if (!turned) return;
@@ -366,7 +415,7 @@ __global__ __launch_bounds__(T::NT) void grad_kernel(TnArgs g, GradOut o) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;
 #pragma unroll
-  for (int j = 0; j < T::NI; ++j)
+  for (int j = 0; j < T::WN / 32; ++j)
     tn_rows<T>(lds, acc, j, [&](int row, int m, const float (&v)[8]) {
       const int n = ns + j * 32 + row, left = g.M - (ms + m);
       if (n >= g.N || left <= 0) return;
@@ -398,33 +447,41 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
 }
 
 // ------------------------------------------------------------------------------------------------ host
-using Wide = TnTile<256, 256, 2, 4>;
-using Mid = TnTile<128, 128, 2, 2>;
-using Narrow = TnTile<128, 32, 4, 1>;     // few rows: as many workgroups as strips of 128 classes
+using Wide = TnTile<256, 256, 2, 4, 2>;
+using Mid = TnTile<128, 128, 2, 2, 2>;
+using Narrow = TnTile<64, 32, 2, 1, 4>;     // few rows: many small workgroups that stream W
 
 constexpr long CUS = 256;
-long up(long a, long b) { return (a + b - 1) / b * b; }
+// Elements between rows of a buffer of this file's own: whole lines of 64, an odd number of them, so that the rows of a tile do not all start in
+// the same few L2 channels (a 4096-wide product took 3 % longer than a 4160-wide one).
+long pitch_of(long n) { const long lines = (n + 63) / 64; return (lines | 1) * 64; }
 
 struct Plan {
   bool f32, grad, direct;        // direct: x and W are used where they are
-  long T, V, D, Kp, Vp, R, Rp;   // padded D and V; rows of a block, padded
+  long T, V, D, Kp, Vp, R, Rp;   // pitches for D and V values; rows of a block, pitch for them
   int blocks, planes, pairs, tile_scores, strips, strip;
   size_t inv, stats, lse, tscore, xp, wp, wt, xt, e, d, dt, dw, part, total, part_bytes;
 };
 
-// 256 x 256 tiles where they fill the chip, 128 x 128 ones where only those do, 128 x 32 for few rows
-int tile_for_scores(long rows, long V) {
-  if (rows <= 32) return 2;
-  return cdiv(V, 256) * (long)cdiv(rows, 256) >= CUS ? 0 : 1;
+// Which tile, and how many parts of k: the choice with the shortest time by what one step of 64 in k takes a full chip of workgroups --
+// 1.15 us for 256 x 256 tiles (one a CU), 0.95 us for 128 x 128 ones (two a CU) -- times rounds of workgroups, plus the parts' way through
+// memory (written and read once more, at 4 TB/s, and a launch).
+struct Shape { int wide; int splits; };
+Shape shape_of(long M, long N, long steps, bool may_split) {
+  Shape best{1, 1};
+  double least = 1e300;
+  for (int wide = 0; wide < 2; ++wide) {
+    const long t = wide ? 256 : 128, tiles = cdiv(M, t) * (long)cdiv(N, t), slots = wide ? CUS : 2 * CUS;
+    for (long s = 1; s <= 64 && (s == 1 || (may_split && s * 8 <= steps && s * M * N <= (1L << 28))); ++s) {
+      const double us = (double)((tiles * s + slots - 1) / slots) * (double)((steps + s - 1) / s) * (wide ? 1.15 : 0.95) + (s > 1 ? 4.0 + (double)s * M * N * 8e-6 / 4.0 : 0.0);
+      if (us < least) { least = us; best = Shape{wide, (int)s}; }
+    }
+  }
+  return best;
 }
-long grad_tile(long M, long N) { return cdiv(M, 256) * (long)cdiv(N, 256) >= CUS ? 256 : 128; }
-// parts of k: enough for every CU (two 128-tiles fit one), while a part keeps at least 16 steps and all parts together 2^28 values
-int grad_splits(long M, long N, long steps) {
-  const long t = grad_tile(M, N), tiles = cdiv(M, t) * (long)cdiv(N, t), want = t == 256 ? CUS : 2 * CUS;
-  long s = tiles >= want * 3 / 4 ? 1 : cdiv(want, tiles);
-  if (s > steps / 16) s = steps / 16;
-  while (s > 1 && s * M * N > (1L << 28)) --s;
-  return s < 1 ? 1 : (int)s;
+int tile_for_scores(long rows, long V, long steps) {
+  if (rows <= 32) return 2;      // W streams through once either way: 64 x 32 tiles have it on every CU
+  return shape_of(V, rows, steps, false).wide ? 0 : 1;
 }
 
 Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
@@ -432,19 +489,19 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
   p.f32 = f32; p.grad = grad; p.T = T; p.V = V; p.D = D;
   p.planes = f32 ? 3 : 1;
   p.pairs = f32 ? 6 : 1;
-  p.Kp = up(D, 64);
-  p.Vp = up(V, 64);
   p.direct = direct && !f32 && D % 64 == 0;
-  const long most = grad ? (1L << (f32 ? 27 : 29)) : (1L << 31);     // (row, class) pairs of a block; without gradients only statistics are held
+  p.Kp = p.direct ? D : pitch_of(D);
+  p.Vp = pitch_of(V);
+  const long most = grad ? (1L << (f32 ? 27 : 30)) : (1L << 31);     // (row, class) pairs of a block; without gradients only statistics are held
   p.R = T;
-  if (T * p.Vp > most) {
-    p.R = most / p.Vp / 256 * 256;
-    if (p.R < 256) p.R = 256;
+  if (T * V > most) {       // blocks of one size, whole tiles
+    const long n = (T * V + most - 1) / most;
+    p.R = ((T + n - 1) / n + 255) / 256 * 256;
     if (p.R > T) p.R = T;
   }
   p.blocks = cdiv(T, p.R);
-  p.Rp = up(p.R, 64);
-  p.tile_scores = tile_for_scores(p.R, V);
+  p.Rp = pitch_of(p.R);
+  p.tile_scores = tile_for_scores(p.R, V, (long)cdiv(D, 64) * p.pairs);
   p.strip = p.tile_scores == 0 ? Wide::WM : p.tile_scores == 1 ? Mid::WM : Narrow::WM;
   p.strips = cdiv(V, p.strip);
   size_t at = 0;
@@ -464,7 +521,7 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
     p.d = f32 ? take((size_t)3 * p.R * p.Vp * 2) : p.e;
     p.dt = take((size_t)p.planes * p.Vp * p.Rp * 2);
     if (p.blocks > 1 && !f32) p.dw = take((size_t)V * D * 4);
-    const int s1 = grad_splits(D, p.R, p.Vp / 64 * p.pairs), s2 = grad_splits(D, V, p.Rp / 64 * p.pairs);
+    const int s1 = shape_of(D, p.R, (long)cdiv(V, 64) * p.pairs, true).splits, s2 = shape_of(D, V, (long)cdiv(p.R, 64) * p.pairs, true).splits;
     const size_t b1 = s1 > 1 ? (size_t)s1 * D * p.R * 4 : 0, b2 = s2 > 1 ? (size_t)s2 * D * V * 4 : 0;
     p.part_bytes = b1 > b2 ? b1 : b2;
     p.part = take(p.part_bytes);
@@ -496,10 +553,11 @@ int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, 
   GradOut o{};
   o.c = c; o.ldc = g.M; o.add = add; o.c_bf16 = c_bf16;
   o.wide = g.M % 8 == 0 && (uintptr_t)c % 16 == 0;
-  g.splits = grad_splits(g.M, g.N, (long)g.ksteps * g.pairs);
+  const Shape shape = shape_of(g.M, g.N, (long)g.ksteps * g.pairs, true);
+  g.splits = shape.splits;
   if (g.splits > 1 && (size_t)g.splits * g.M * g.N * 4 > part_bytes) g.splits = 1;
   if (g.splits > 1) { o.part = part; o.part_stride = (long)g.M * g.N; o.add = nullptr; }
-  if (grad_tile(g.M, g.N) == 256) DPPM_TRY(launch_grad<Wide>(g, o, st));
+  if (shape.wide) DPPM_TRY(launch_grad<Wide>(g, o, st));
   else DPPM_TRY(launch_grad<Mid>(g, o, st));
   if (g.splits > 1) {
     const long n = (long)g.M * g.N, blocks = (n + 255) / 256;
@@ -508,11 +566,17 @@ int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, 
   return DPPM_OK;
 }
 
-void lay_out(bool f32, const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, hipStream_t st) {
+template <bool F32>
+void lay_out(const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, hipStream_t st) {
   const long r = turned ? (pitch_t > rows ? pitch_t : rows) : rows, c = as_is ? pitch : cols;
   const dim3 grid((unsigned)cdiv(c, 64), (unsigned)cdiv(r, 64));
-  if (f32) hipLaunchKernelGGL((lay_out_kernel<true>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t);
-  else hipLaunchKernelGGL((lay_out_kernel<false>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t);
+  const bool wide = (uintptr_t)src % 16 == 0 && cols % (F32 ? 4 : 8) == 0;
+  if (wide) hipLaunchKernelGGL((lay_out_kernel<F32, true>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t);
+  else hipLaunchKernelGGL((lay_out_kernel<F32, false>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t);
+}
+void lay_out(bool f32, const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, hipStream_t st) {
+  if (f32) lay_out<true>(src, rows, cols, as_is, pitch, turned, pitch_t, st);
+  else lay_out<false>(src, rows, cols, as_is, pitch, turned, pitch_t, st);
 }
 
 bool sizes_ok(int64_t T, int64_t V, int64_t D) { return T >= 0 && V >= 1 && D >= 1 && T < (1L << 30) && V <= (1L << 23) && D <= (1L << 16); }   // 255 rows of any operand lie within 2^32 bytes
@@ -551,7 +615,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
   const auto h = [&](size_t at) { return reinterpret_cast<uint16_t*>(ws + at); };
   const auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
   float2* stats = reinterpret_cast<float2*>(ws + p.stats);
-  hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, target, (long)T, (long)V, (float)denom, f(p.inv));
+  if (grad) hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, target, (long)T, (long)V, (float)denom, f(p.inv));
   const uint16_t *xp = reinterpret_cast<const uint16_t*>(x), *wp = reinterpret_cast<const uint16_t*>(weight);
   if (!p.direct || grad) lay_out(p.f32, weight, V, D, p.direct ? nullptr : h(p.wp), p.Kp, grad ? h(p.wt) : nullptr, p.Vp, st);
   if (!p.direct) {
@@ -559,24 +623,26 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     xp = h(p.xp); wp = h(p.wp);
   }
   for (int b = 0; b < p.blocks; ++b) {
-    const long t0 = b * p.R, rows = T - t0 < p.R ? T - t0 : p.R, Rp = up(rows, 64);
+    const long t0 = b * p.R, rows = T - t0 < p.R ? T - t0 : p.R, Rp = pitch_of(rows);
     TnArgs g{};
     g.A = wp; g.lda = p.Kp; g.plane_a = V * p.Kp; g.M = (int)V;
     g.B = xp + t0 * p.Kp; g.ldb = p.Kp; g.plane_b = T * p.Kp; g.N = (int)rows;
-    g.ksteps = (int)(p.Kp / 64); g.pairs = p.pairs; g.splits = 1;
+    g.ksteps = cdiv(D, 64); g.pairs = p.pairs; g.splits = 1;
     ScoreOut o{};
     o.stats = stats; o.target_score = f(p.tscore); o.target = target + t0; o.e = grad ? ws + p.e : nullptr; o.pitch = p.Vp; o.V = (int)V;
     if (p.tile_scores == 0) DPPM_TRY(p.f32 ? (launch_scores<Wide, true>(g, o, st)) : (launch_scores<Wide, false>(g, o, st)));
     else if (p.tile_scores == 1) DPPM_TRY(p.f32 ? (launch_scores<Mid, true>(g, o, st)) : (launch_scores<Mid, false>(g, o, st)));
     else DPPM_TRY(p.f32 ? (launch_scores<Narrow, true>(g, o, st)) : (launch_scores<Narrow, false>(g, o, st)));
-    hipLaunchKernelGGL(rows_kernel, dim3(cdiv(rows, 32)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
+    // a thread's share of the strips is what takes the time: with few rows, more threads a row
+    if (rows <= 64) hipLaunchKernelGGL((rows_kernel<2>), dim3(cdiv(rows, 2)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
+    else hipLaunchKernelGGL((rows_kernel<32>), dim3(cdiv(rows, 32)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
     if (!grad) continue;
     TurnArgs a{};
     a.e = ws + p.e; a.pitch_e = p.Vp; a.stats = stats; a.lse = f(p.lse); a.target_score = f(p.tscore); a.target = target + t0;
     a.row_weight = row_weight ? row_weight + t0 : nullptr; a.inv = f(p.inv);
     a.d = h(p.d); a.plane_d = rows * p.Vp; a.dt = h(p.dt); a.pitch_t = Rp; a.plane_t = p.Vp * Rp;
     a.rows = (int)rows; a.V = (int)V; a.strip = p.strip;
-    const dim3 grid((unsigned)(p.Vp / 64), (unsigned)(Rp / 64));
+    const dim3 grid((unsigned)cdiv(V, 64), (unsigned)cdiv(rows, 64));
     if (p.f32) hipLaunchKernelGGL((turn_kernel<true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((turn_kernel<false>), grid, dim3(256), 0, st, a);
     const size_t es = bf16 ? 2 : 4;
@@ -584,16 +650,16 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     TnArgs gx{};       // dx[t][d] = sum_v d[t][v] W^T[d][v]
     gx.A = h(p.wt); gx.lda = p.Vp; gx.plane_a = D * p.Vp; gx.M = (int)D;
     gx.B = a.d; gx.ldb = p.Vp; gx.plane_b = a.plane_d; gx.N = (int)rows;
-    gx.ksteps = (int)(p.Vp / 64); gx.pairs = p.pairs;
+    gx.ksteps = cdiv(V, 64); gx.pairs = p.pairs;
     DPPM_TRY(grad_product(gx, reinterpret_cast<char*>(dx) + t0 * D * es, bf16, nullptr, f(p.part), p.part_bytes, st));
     TnArgs gw{};       // dW[v][d] = sum_t d^T[v][t] x^T[d][t]
     gw.A = h(p.xt); gw.lda = Rp; gw.plane_a = D * Rp; gw.M = (int)D;
     gw.B = a.dt; gw.ldb = Rp; gw.plane_b = a.plane_t; gw.N = (int)V;
-    gw.ksteps = (int)(Rp / 64); gw.pairs = p.pairs;
+    gw.ksteps = cdiv(rows, 64); gw.pairs = p.pairs;
     const bool last = b == p.blocks - 1;
     float* sum = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
     DPPM_TRY(grad_product(gw, last || p.f32 ? dweight : (void*)sum, bf16 && last, b == 0 ? nullptr : sum, f(p.part), p.part_bytes, st));
   }
-  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, f(p.inv), (long)T, loss_out);
+  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, target, (long)V, (float)denom, grad ? f(p.inv) : nullptr, (long)T, loss_out);
   return check_launch("dppm_loss_ce_fwd_bwd");
 }

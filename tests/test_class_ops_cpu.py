@@ -101,4 +101,4 @@ def test_loss_ce_entry_refuses():
     assert lib.dppm_loss_ce_fwd_bwd(*{**good, "n": 64}.values()) == -1
     # beside a copy of x, memory is that of one block of rows, whatever their number
     many, more = lib.dppm_loss_ce_workspace_bytes(1 << 16, 1 << 17, 1024, 1, 1), lib.dppm_loss_ce_workspace_bytes(1 << 17, 1 << 17, 1024, 1, 1)
-    assert more - many <= (1 << 16) * 1024 * 2 + 4096 and more < 8 << 30
+    assert more - many <= (1 << 16) * 1088 * 2 + 4096 and more < 8 << 30
