@@ -10,8 +10,9 @@
 //  * scores: tiles of s on the matrix cores; from the accumulators each strip of classes gives its maximum and its sum of exponentials per
 //    row, and (with gradients) the exponentials relative to the strip's maximum, bfloat16 for bfloat16 inputs and float32 for float32;
 //  * rows: lse, the rows' losses;
-//  * turn: exponentials to d, rounded once to the operands' type, as it stands and transposed;
-//  * dx = d W and dW = d^T x, both with the contracted dimension contiguous in both operands: W and x are transposed once.
+//  * turn: exponentials to d, rounded once to the operands' type;
+//  * dx = d W and dW = d^T x: W and d are read transposed from LDS where the contracted dimension is not the contiguous one; x, the smallest,
+//    is transposed in memory, with zeros for rows that have no class.
 // The exponentials held at a time are those of one block of rows, at most 2^30 (bfloat16) or 2^27 (float32) of them: memory does not grow
 // with T.  Several blocks add up dW in float32.
 #include "dppm_common.h"
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
   tn_tile_of(blockIdx.x, gridDim.x, g.tiles_m, g.tiles_n, tm, tn);
   const int m0 = tm * T::BM, n0 = tn * T::BN;
   tn_acc acc[T::MI][T::NI];
-  tn_product<T>(g, lds, m0, n0, 0, g.ksteps * g.pairs, acc);
+  tn_product<T, false, false>(g, lds, m0, n0, 0, g.ksteps * g.pairs, acc);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;     // this wave's strip of classes, its rows
   const int strip = ms / T::WM, first = ms + (lane >> 4) * 4;                         // class of acc[0][.][0]
@@ -221,105 +222,85 @@ __global__ __launch_bounds__(256) void rows_kernel(const float2* __restrict__ st
 
 // ------------------------------------------------------------------------------------------------ turn
 struct TurnArgs {
-  const void* e; long pitch_e;           // exponentials [rows][pitch_e]
+  const void* e; long pitch;             // exponentials [rows][pitch]
   const float2* stats; const float* lse; const float* target_score; const int64_t* target; const float* row_weight; const float* inv;
-  uint16_t* d; long plane_d;             // [planes][rows][pitch_e]; may be e itself (bfloat16)
-  uint16_t* dt; long pitch_t, plane_t;   // [planes][pitch_e][pitch_t]
+  uint16_t* d; long plane;               // [planes][rows, whole tiles of 64][pitch]; e itself for bfloat16
   int rows, V, strip;                    // strip: classes that share a maximum
 };
 
-// 64 rows x 64 classes a workgroup: d_tv = e_tv * exp(max_strip - lse_t) * w_t / n, the row's own class from its float32 score, written as it
-// stands and transposed.  Rows behind the last and classes behind the last are zeros, up to whole tiles.
+// 16 rows x 512 classes a workgroup, 8 classes a thread and row: d_tv = e_tv * exp(max_strip - lse_t) * w_t / n, the row's own class from its float32
+// score.  Rows behind the last (to whole tiles of 64) and without a class are zeros; so are classes behind the last, to the pitch.
 template <bool F32>
 __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
-  constexpr int P = F32 ? 3 : 1;
-  __shared__ uint16_t tile[P][64][66];
-  __shared__ float factor[2][64];     // of the tile's first and second 32 classes: strips of 32 are the shortest
-  __shared__ float own[64];
-  __shared__ int at[64];
-  const int v0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
-  if (threadIdx.x < 64) {
-    const int t = t0 + threadIdx.x;
-    float f[2] = {0.f, 0.f}, mine = 0.f;
+  constexpr int P = F32 ? 3 : 1, ROWS = 16;
+  __shared__ float factor[16][ROWS];     // of each 32 classes: strips of 32 are the shortest
+  __shared__ float own[ROWS];
+  __shared__ int at[ROWS];
+  const int v0 = blockIdx.x * 512, t0 = blockIdx.y * ROWS;
+  {
+    const int r = threadIdx.x & 15, k = threadIdx.x >> 4, t = t0 + r, v = v0 + 32 * k;
+    float f = 0.f, mine = 0.f;
     int where = -1;
     if (t < a.rows) {
       const int64_t y = a.target[t];
       if (y >= 0 && y < a.V) {
         const float g = (a.row_weight ? a.row_weight[t] : 1.f) * *a.inv;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (v0 + 32 * k < a.V) f[k] = expf(a.stats[(long)((v0 + 32 * k) / a.strip) * a.rows + t].x - a.lse[t]) * g;
-        if (y >= v0 && y < v0 + 64) {
-          where = (int)(y - v0);
-          mine = (expf(a.target_score[t] - a.lse[t]) - 1.f) * g;
-        }
+        if (v < a.V) f = expf(a.stats[(long)(v / a.strip) * a.rows + t].x - a.lse[t]) * g;
+        where = (int)y;
+        if (k == 0) mine = (expf(a.target_score[t] - a.lse[t]) - 1.f) * g;
       }
     }
-    factor[0][threadIdx.x] = f[0];
-    factor[1][threadIdx.x] = f[1];
-    own[threadIdx.x] = mine;
-    at[threadIdx.x] = where;
+    factor[k][r] = f;
+    if (k == 0) { own[r] = mine; at[r] = where; }
   }
   __syncthreads();
-  const int c = (threadIdx.x & 15) * 4;
+  const int c = (threadIdx.x & 63) * 8, v = v0 + c;
+  if (v >= a.pitch) return;
 #pragma unroll
-  for (int r = threadIdx.x >> 4; r < 64; r += 16) {
-    const int t = t0 + r, v = v0 + c;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (t < a.rows) {
-      const float f = factor[c >> 5][r];
-      if (f != 0.f) {
-        if (F32) {
-          const f32x4 w = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(a.e) + (long)t * a.pitch_e + v);
-          x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
-        } else {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint16_t*>(a.e) + (long)t * a.pitch_e + v);
-          x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u);
-          x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
-        }
+  for (int r = threadIdx.x >> 6; r < ROWS; r += 4) {
+    const int t = t0 + r;
+    const long to = (long)t * a.pitch + v;
+    const float f = factor[c >> 5][r];
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (t < a.rows && f != 0.f) {
+      if (F32) {
+        const f32x4* e = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(a.e) + to);
+        const f32x4 w0 = e[0], w1 = e[1];
+        x[0] = w0.x; x[1] = w0.y; x[2] = w0.z; x[3] = w0.w; x[4] = w1.x; x[5] = w1.y; x[6] = w1.z; x[7] = w1.w;
+      } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.e) + to);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] *= f;
+        for (int k = 0; k < 4; ++k) { x[2 * k] = __uint_as_float(w[k] << 16); x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u); }
       }
-      const int y = at[r] - c;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (y == k && at[r] >= 0) x[k] = own[r];
+      for (int k = 0; k < 8; ++k) x[k] *= f;
     }
-    uint16_t s[4][3];
+    const int y = at[r] - v;
+    if (y >= 0 && y < 8) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (F32) split3(x[k], s[k]);
-      else s[k][0] = to_bf16(x[k]);
+      for (int k = 0; k < 8; ++k)
+        if (y == k) x[k] = own[r];
     }
+    if (F32) {
+      uint16_t s[8][3];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      if (t < a.rows)
-        *reinterpret_cast<u32x2*>(a.d + p * a.plane_d + (long)t * a.pitch_e + v) =
-            u32x2{(uint32_t)s[0][p] | ((uint32_t)s[1][p] << 16), (uint32_t)s[2][p] | ((uint32_t)s[3][p] << 16)};
+      for (int k = 0; k < 8; ++k) split3(x[k], s[k]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) tile[p][r][c + k] = s[k][p];
-    }
+      for (int p = 0; p < P; ++p)
+        *reinterpret_cast<u32x4*>(a.d + p * a.plane + to) = u32x4{s[0][p] | (uint32_t)s[1][p] << 16, s[2][p] | (uint32_t)s[3][p] << 16,
+                                                                s[4][p] | (uint32_t)s[5][p] << 16, s[6][p] | (uint32_t)s[7][p] << 16};
+    } else
+      *reinterpret_cast<u32x4*>(a.d + to) = u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
   }
-  __syncthreads();
-  const int t = (threadIdx.x & 7) * 8;
-#pragma unroll
-  for (int p = 0; p < P; ++p)
-#pragma unroll
-    for (int v = threadIdx.x >> 3; v < 64; v += 32) {
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = (uint32_t)tile[p][t + 2 * k][v] | ((uint32_t)tile[p][t + 2 * k + 1][v] << 16);
-      *reinterpret_cast<u32x4*>(a.dt + p * a.plane_t + (long)(v0 + v) * a.pitch_t + t0 + t) = u32x4{w[0], w[1], w[2], w[3]};
-    }
 }
 
 // ------------------------------------------------------------------------------------------------ operands
 // [rows][cols] of the caller, contiguous -> bfloat16 planes, as they stand [rows][pitch] (cols .. pitch zero) and/or transposed [cols][pitch_t]
-// (rows .. pitch_t zero).  64 x 64 a workgroup.
+// (rows .. pitch_t zero).  target, V (or null): rows without a class are zeros.  64 x 64 a workgroup.
 // WIDE: cols and the source's address allow 16-byte reads (4 or 8 values).
 template <bool F32, bool WIDE>
 __global__ __launch_bounds__(256) void lay_out_kernel(const void* __restrict__ src, int rows, int cols, uint16_t* __restrict__ as_is, long pitch, long plane,
-                                                      uint16_t* __restrict__ turned, long pitch_t, long plane_t) {
+                                                      uint16_t* __restrict__ turned, long pitch_t, long plane_t, const int64_t* __restrict__ target, long V) {
   constexpr int P = F32 ? 3 : 1, VEC = WIDE ? (F32 ? 4 : 8) : 1, PER_ROW = 64 / VEC;
   __shared__ uint16_t tile[P][64][66];
   const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
@@ -329,7 +310,7 @@ __global__ __launch_bounds__(256) void lay_out_kernel(const void* __restrict__ s
     uint16_t s[VEC][3];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) s[k][0] = s[k][1] = s[k][2] = 0;
-    if (r0 + r < rows && c0 + c < cols) {
+    if (r0 + r < rows && c0 + c < cols && (!target || (target[r0 + r] >= 0 && target[r0 + r] < V))) {
       const long at = (long)(r0 + r) * cols + c0 + c;
       if constexpr (F32) {
         float v[VEC];
@@ -402,7 +383,7 @@ __device__ __forceinline__ void put8(const GradOut& o, long at, int left, const 
   }
 }
 
-template <class T>
+template <class T, bool TRA, bool TRB>
 __global__ __launch_bounds__(T::NT) void grad_kernel(TnArgs g, GradOut o) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tiles = g.tiles_m * g.tiles_n, split = blockIdx.x / tiles;
@@ -411,7 +392,7 @@ __global__ __launch_bounds__(T::NT) void grad_kernel(TnArgs g, GradOut o) {
   const int m0 = tm * T::BM, n0 = tn * T::BN;
   const long steps = (long)g.ksteps * g.pairs;
   tn_acc acc[T::MI][T::NI];
-  tn_product<T>(g, lds, m0, n0, (int)(steps * split / g.splits), (int)(steps * (split + 1) / g.splits), acc);
+  tn_product<T, TRA, TRB>(g, lds, m0, n0, (int)(steps * split / g.splits), (int)(steps * (split + 1) / g.splits), acc);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;
 #pragma unroll
@@ -460,7 +441,7 @@ struct Plan {
   bool f32, grad, direct;        // direct: x and W are used where they are
   long T, V, D, Kp, Vp, R, Rp;   // pitches for D and V values; rows of a block, pitch for them
   int blocks, planes, pairs, tile_scores, strips, strip;
-  size_t inv, stats, lse, tscore, xp, wp, wt, xt, e, d, dt, dw, part, total, part_bytes;
+  size_t inv, stats, lse, tscore, xp, wp, xt, e, d, dw, part, total, part_bytes;
 };
 
 // Which tile, and how many parts of k: the choice with the shortest time by what one step of 64 in k takes a full chip of workgroups --
@@ -494,8 +475,9 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
   p.Vp = pitch_of(V);
   const long most = grad ? (1L << (f32 ? 27 : 30)) : (1L << 31);     // (row, class) pairs of a block; without gradients only statistics are held
   p.R = T;
-  if (T * V > most) {       // blocks of one size, whole tiles
-    const long n = (T * V + most - 1) / most;
+  const long by_pairs = (T * V + most - 1) / most, by_rows = (T + (1L << 22) - 1) >> 22;     // 255 rows of x^T stay within 2^32 bytes
+  const long n = by_pairs > by_rows ? by_pairs : by_rows;
+  if (n > 1) {              // blocks of one size, whole tiles
     p.R = ((T + n - 1) / n + 255) / 256 * 256;
     if (p.R > T) p.R = T;
   }
@@ -515,11 +497,10 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
     p.wp = take((size_t)p.planes * V * p.Kp * 2);
   }
   if (grad) {
-    p.wt = take((size_t)p.planes * D * p.Vp * 2);
     p.xt = take((size_t)p.planes * D * p.Rp * 2);
-    p.e = take((size_t)p.R * p.Vp * (f32 ? 4 : 2));
-    p.d = f32 ? take((size_t)3 * p.R * p.Vp * 2) : p.e;
-    p.dt = take((size_t)p.planes * p.Vp * p.Rp * 2);
+    const size_t held = (size_t)((p.R + 63) / 64 * 64) * p.Vp;
+    p.e = take(held * (f32 ? 4 : 2));
+    p.d = f32 ? take(3 * held * 2) : p.e;
     if (p.blocks > 1 && !f32) p.dw = take((size_t)V * D * 4);
     const int s1 = shape_of(D, p.R, (long)cdiv(V, 64) * p.pairs, true).splits, s2 = shape_of(D, V, (long)cdiv(p.R, 64) * p.pairs, true).splits;
     const size_t b1 = s1 > 1 ? (size_t)s1 * D * p.R * 4 : 0, b2 = s2 > 1 ? (size_t)s2 * D * V * 4 : 0;
@@ -539,16 +520,17 @@ int launch_scores(TnArgs g, const ScoreOut& o, hipStream_t st) {
   return DPPM_OK;
 }
 
-template <class T>
+template <class T, bool TRA, bool TRB>
 int launch_grad(TnArgs g, const GradOut& o, hipStream_t st) {
-  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(grad_kernel<T>), T::LDS, "dppm_loss_ce"));
+  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(grad_kernel<T, TRA, TRB>), T::LDS, "dppm_loss_ce"));
   g.tiles_m = cdiv(g.M, T::BM);
   g.tiles_n = cdiv(g.N, T::BN);
-  hipLaunchKernelGGL((grad_kernel<T>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(T::NT), T::LDS, st, g, o);
+  hipLaunchKernelGGL((grad_kernel<T, TRA, TRB>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(T::NT), T::LDS, st, g, o);
   return DPPM_OK;
 }
 
 // c[n][m] (+= add) = sum_k A[m][k] B[n][k]
+template <bool TRA, bool TRB>
 int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, size_t part_bytes, hipStream_t st) {
   GradOut o{};
   o.c = c; o.ldc = g.M; o.add = add; o.c_bf16 = c_bf16;
@@ -557,8 +539,8 @@ int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, 
   g.splits = shape.splits;
   if (g.splits > 1 && (size_t)g.splits * g.M * g.N * 4 > part_bytes) g.splits = 1;
   if (g.splits > 1) { o.part = part; o.part_stride = (long)g.M * g.N; o.add = nullptr; }
-  if (shape.wide) DPPM_TRY(launch_grad<Wide>(g, o, st));
-  else DPPM_TRY(launch_grad<Mid>(g, o, st));
+  if (shape.wide) DPPM_TRY((launch_grad<Wide, TRA, TRB>(g, o, st)));
+  else DPPM_TRY((launch_grad<Mid, TRA, TRB>(g, o, st)));
   if (g.splits > 1) {
     const long n = (long)g.M * g.N, blocks = (n + 255) / 256;
     hipLaunchKernelGGL(parts_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, part, n, g.splits, add, n, c, (int)c_bf16);
@@ -567,16 +549,16 @@ int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, 
 }
 
 template <bool F32>
-void lay_out(const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, hipStream_t st) {
+void lay_out(const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, const int64_t* target, long V, hipStream_t st) {
   const long r = turned ? (pitch_t > rows ? pitch_t : rows) : rows, c = as_is ? pitch : cols;
   const dim3 grid((unsigned)cdiv(c, 64), (unsigned)cdiv(r, 64));
   const bool wide = (uintptr_t)src % 16 == 0 && cols % (F32 ? 4 : 8) == 0;
-  if (wide) hipLaunchKernelGGL((lay_out_kernel<F32, true>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t);
-  else hipLaunchKernelGGL((lay_out_kernel<F32, false>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t);
+  if (wide) hipLaunchKernelGGL((lay_out_kernel<F32, true>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t, target, V);
+  else hipLaunchKernelGGL((lay_out_kernel<F32, false>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t, target, V);
 }
-void lay_out(bool f32, const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, hipStream_t st) {
-  if (f32) lay_out<true>(src, rows, cols, as_is, pitch, turned, pitch_t, st);
-  else lay_out<false>(src, rows, cols, as_is, pitch, turned, pitch_t, st);
+void lay_out(bool f32, const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, const int64_t* target, long V, hipStream_t st) {
+  if (f32) lay_out<true>(src, rows, cols, as_is, pitch, turned, pitch_t, target, V, st);
+  else lay_out<false>(src, rows, cols, as_is, pitch, turned, pitch_t, target, V, st);
 }
 
 bool sizes_ok(int64_t T, int64_t V, int64_t D) { return T >= 0 && V >= 1 && D >= 1 && T < (1L << 30) && V <= (1L << 23) && D <= (1L << 16); }   // 255 rows of any operand lie within 2^32 bytes
@@ -617,9 +599,9 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
   float2* stats = reinterpret_cast<float2*>(ws + p.stats);
   if (grad) hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, target, (long)T, (long)V, (float)denom, f(p.inv));
   const uint16_t *xp = reinterpret_cast<const uint16_t*>(x), *wp = reinterpret_cast<const uint16_t*>(weight);
-  if (!p.direct || grad) lay_out(p.f32, weight, V, D, p.direct ? nullptr : h(p.wp), p.Kp, grad ? h(p.wt) : nullptr, p.Vp, st);
   if (!p.direct) {
-    lay_out(p.f32, x, T, D, h(p.xp), p.Kp, nullptr, 0, st);
+    lay_out(p.f32, weight, V, D, h(p.wp), p.Kp, nullptr, 0, nullptr, 0, st);
+    lay_out(p.f32, x, T, D, h(p.xp), p.Kp, nullptr, 0, nullptr, 0, st);
     xp = h(p.xp); wp = h(p.wp);
   }
   for (int b = 0; b < p.blocks; ++b) {
@@ -627,7 +609,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     TnArgs g{};
     g.A = wp; g.lda = p.Kp; g.plane_a = V * p.Kp; g.M = (int)V;
     g.B = xp + t0 * p.Kp; g.ldb = p.Kp; g.plane_b = T * p.Kp; g.N = (int)rows;
-    g.ksteps = cdiv(D, 64); g.pairs = p.pairs; g.splits = 1;
+    g.K = (int)D; g.ksteps = cdiv(D, 64); g.pairs = p.pairs; g.splits = 1;
     ScoreOut o{};
     o.stats = stats; o.target_score = f(p.tscore); o.target = target + t0; o.e = grad ? ws + p.e : nullptr; o.pitch = p.Vp; o.V = (int)V;
     if (p.tile_scores == 0) DPPM_TRY(p.f32 ? (launch_scores<Wide, true>(g, o, st)) : (launch_scores<Wide, false>(g, o, st)));
@@ -637,28 +619,28 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     if (rows <= 64) hipLaunchKernelGGL((rows_kernel<2>), dim3(cdiv(rows, 2)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
     else hipLaunchKernelGGL((rows_kernel<32>), dim3(cdiv(rows, 32)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
     if (!grad) continue;
+    const int whole = cdiv(rows, 64) * 64;
     TurnArgs a{};
-    a.e = ws + p.e; a.pitch_e = p.Vp; a.stats = stats; a.lse = f(p.lse); a.target_score = f(p.tscore); a.target = target + t0;
+    a.e = ws + p.e; a.pitch = p.Vp; a.stats = stats; a.lse = f(p.lse); a.target_score = f(p.tscore); a.target = target + t0;
     a.row_weight = row_weight ? row_weight + t0 : nullptr; a.inv = f(p.inv);
-    a.d = h(p.d); a.plane_d = rows * p.Vp; a.dt = h(p.dt); a.pitch_t = Rp; a.plane_t = p.Vp * Rp;
-    a.rows = (int)rows; a.V = (int)V; a.strip = p.strip;
-    const dim3 grid((unsigned)cdiv(V, 64), (unsigned)cdiv(rows, 64));
+    a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip;
+    const dim3 grid((unsigned)cdiv(p.Vp, 512), (unsigned)(whole / 16));
     if (p.f32) hipLaunchKernelGGL((turn_kernel<true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((turn_kernel<false>), grid, dim3(256), 0, st, a);
     const size_t es = bf16 ? 2 : 4;
-    lay_out(p.f32, reinterpret_cast<const char*>(x) + t0 * D * es, rows, D, nullptr, 0, h(p.xt), Rp, st);
-    TnArgs gx{};       // dx[t][d] = sum_v d[t][v] W^T[d][v]
-    gx.A = h(p.wt); gx.lda = p.Vp; gx.plane_a = D * p.Vp; gx.M = (int)D;
-    gx.B = a.d; gx.ldb = p.Vp; gx.plane_b = a.plane_d; gx.N = (int)rows;
-    gx.ksteps = cdiv(V, 64); gx.pairs = p.pairs;
-    DPPM_TRY(grad_product(gx, reinterpret_cast<char*>(dx) + t0 * D * es, bf16, nullptr, f(p.part), p.part_bytes, st));
-    TnArgs gw{};       // dW[v][d] = sum_t d^T[v][t] x^T[d][t]
+    lay_out(p.f32, reinterpret_cast<const char*>(x) + t0 * D * es, rows, D, nullptr, 0, h(p.xt), Rp, target + t0, V, st);
+    TnArgs gx{};       // dx[t][d] = sum_v d[t][v] W[v][d]
+    gx.A = wp; gx.lda = p.Kp; gx.plane_a = V * p.Kp; gx.M = (int)D;
+    gx.B = a.d; gx.ldb = p.Vp; gx.plane_b = a.plane; gx.N = (int)rows;
+    gx.K = (int)V; gx.ksteps = cdiv(V, 64); gx.pairs = p.pairs;
+    DPPM_TRY((grad_product<true, false>(gx, reinterpret_cast<char*>(dx) + t0 * D * es, bf16, nullptr, f(p.part), p.part_bytes, st)));
+    TnArgs gw{};       // dW[v][d] = sum_t d[t][v] x^T[d][t]
     gw.A = h(p.xt); gw.lda = Rp; gw.plane_a = D * Rp; gw.M = (int)D;
-    gw.B = a.dt; gw.ldb = Rp; gw.plane_b = a.plane_t; gw.N = (int)V;
-    gw.ksteps = cdiv(rows, 64); gw.pairs = p.pairs;
+    gw.B = a.d; gw.ldb = p.Vp; gw.plane_b = a.plane; gw.N = (int)V;
+    gw.K = whole; gw.ksteps = cdiv(rows, 64); gw.pairs = p.pairs;      // d has zeros to whole steps
     const bool last = b == p.blocks - 1;
     float* sum = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
-    DPPM_TRY(grad_product(gw, last || p.f32 ? dweight : (void*)sum, bf16 && last, b == 0 ? nullptr : sum, f(p.part), p.part_bytes, st));
+    DPPM_TRY((grad_product<false, true>)(gw, last || p.f32 ? dweight : (void*)sum, bf16 && last, b == 0 ? nullptr : sum, f(p.part), p.part_bytes, st));
   }
   hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, target, (long)V, (float)denom, grad ? f(p.inv) : nullptr, (long)T, loss_out);
   return check_launch("dppm_loss_ce_fwd_bwd");

@@ -1,5 +1,5 @@
-// C[n][m] = sum over k of A[m][k] * B[n][k] for bfloat16 operands that are both contiguous in k, accumulated in float32 on
-// v_mfma_f32_16x16x32_bf16, for the products of the class loss (dppm_classloss.hip).
+// C[n][m] = sum over k of A[m][k] * B[n][k] for bfloat16 operands, accumulated in float32 on v_mfma_f32_16x16x32_bf16, for the products of the
+// class loss (dppm_classloss.hip).  Either operand may be contiguous in k, or in m (n): then it is given as [k][m].
 //
 // A float32 operand comes as three bfloat16 planes (hi + mid + lo hold its 24 significant bits); the same loop then walks six pairs of
 // planes per step of k (all products down to 2^-16 of the largest), which makes a float32-grade product at a sixth of the bfloat16 rate --
@@ -11,6 +11,11 @@
 // a time, lanes 0-3, 12-15 and 20-27 together (then the others), that is rows 0-3 and 12-15 of one chunk with rows 4-11 of the next, and this
 // way they fall on all banks (SQ_LDS_BANK_CONFLICT 0; with g = r & 7 half of the LDS time was conflicts).  The DMA writes lanes side by side, so
 // the swizzle is made on the global side: a lane fetches the chunk whose slot it fills.
+//
+// An operand that is contiguous in m lies in a stage as it comes, 64 rows of k with BM values, and its fragments are read by
+// ds_read_b64_tr_b16: 16 lanes give the addresses of a block of 4 k by 16 m, 8 bytes each, and lane i gets column i's four values.  Two of them
+// make the eight k of a lane.  32 lanes read 8 rows (k = 0-3 and 8-11, or 4 more) at once, 32 bytes each: the 32-byte blocks of a row are turned
+// by (k & 3) + 4 (k >> 3 & 1), which puts them on all banks.
 #pragma once
 #include "dppm_common.h"
 
@@ -21,9 +26,9 @@ typedef float tn_acc __attribute__((ext_vector_type(4)));
 
 struct TnArgs {
   const uint16_t* A; const uint16_t* B;
-  long lda, ldb;          // elements between rows; multiples of 8, as the planes' distance
+  long lda, ldb;          // elements between rows (of m or n, or of k); multiples of 8, as the planes' distance
   long plane_a, plane_b;  // elements between planes
-  int M, N, ksteps;       // ksteps = k / 64: operands are padded with zeros to whole steps
+  int M, N, K, ksteps;       // ksteps = k / 64: operands contiguous in k are padded with zeros to whole steps
   int pairs;              // 1, or 6 for float32 operands in three planes
   int splits;             // parts that the steps of k are dealt to
   int tiles_m, tiles_n;
@@ -56,38 +61,56 @@ __device__ __forceinline__ void tn_tile_of(int id, int count, int tiles_m, int t
   tn = in / rows;
 }
 
+template <int N> struct Int { static constexpr int value = N; };
+
 // what chunk numbers of a row are turned by
 __device__ __forceinline__ int tn_turn(int row) {
   const int q = (row >> 1) & 7;
   return q ^ (((q >> 1) ^ (q >> 2)) & 1);
 }
 
-template <class T>
+// Offsets in bytes of the 16-byte chunks a thread brings in, one a round, from an operand whose tile begins at row (or column) `first` of `count`.
+// Contiguous in k: WIDTH rows of 8 chunks; rows behind the last repeat it, their results are not kept.  Else: 64 rows of k with WIDTH / 8
+// chunks; chunks behind the pitch repeat its last, and in the last step rows of k behind `ks` repeat the last, where the other operand
+// holds zeros.
+template <int WIDTH, int NT, bool TR>
+__device__ __forceinline__ void tn_offsets(uint32_t (&off)[WIDTH * 8 / NT], long ld, int first, int count, int ks) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int r = 0; r < WIDTH * 8 / NT; ++r) {
+    if constexpr (TR) {
+      constexpr int PER = WIDTH / 8;
+      const int k = (r * NT + tid) / PER, turn = ((k & 3) | ((k >> 1) & 4)) << 1;
+      const int c = ((tid % PER) ^ turn), last = (int)(ld / 8) - 1 - first / 8;
+      off[r] = (uint32_t)(((long)(k < ks ? k : ks - 1) * ld + (c < last ? c : last) * 8) * 2);
+    } else {
+      const int row = tid >> 3, chunk = (tid & 7) ^ tn_turn(row), x = row + r * (NT / 8), last = count - 1 - first;
+      off[r] = (uint32_t)(((long)(x < last ? x : last) * ld + chunk * 8) * 2);
+    }
+  }
+}
+
+// TRA, TRB: the operand is contiguous in m (n)
+template <class T, bool TRA, bool TRB>
 __device__ __forceinline__ void tn_product(const TnArgs& g, char* lds, int m0, int n0, int it0, int it1, tn_acc (&acc)[T::MI][T::NI]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % T::WGM, wn = wave / T::WGM;
-  constexpr int RA = T::BM * 8 / T::NT, RB = T::BN * 8 / T::NT, ROWS = T::NT / 8;   // rounds of loads, rows of a round
+  constexpr int RA = T::BM * 8 / T::NT, RB = T::BN * 8 / T::NT;   // rounds of loads
   uint32_t off_a[RA], off_b[RB];
-  {
-    const int row = tid >> 3, chunk = (tid & 7) ^ tn_turn(row);
-#pragma unroll
-    for (int r = 0; r < RA; ++r) {
-      const int x = row + r * ROWS, last = g.M - 1 - m0;
-      off_a[r] = (uint32_t)(((long)(x < last ? x : last) * g.lda + chunk * 8) * 2);      // rows behind the last repeat it: their results are not kept
-    }
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      const int x = row + r * ROWS, last = g.N - 1 - n0;
-      off_b[r] = (uint32_t)(((long)(x < last ? x : last) * g.ldb + chunk * 8) * 2);
-    }
-  }
+  tn_offsets<T::BM, T::NT, TRA>(off_a, g.lda, m0, g.M, 64);
+  tn_offsets<T::BN, T::NT, TRB>(off_b, g.ldb, n0, g.N, 64);
   int pair = it0 % g.pairs;
   long step = it0 / g.pairs;
-  const uint16_t *base_a = g.A + (long)m0 * g.lda, *base_b = g.B + (long)n0 * g.ldb;
+  const uint16_t *base_a = g.A + (TRA ? (long)m0 : (long)m0 * g.lda), *base_b = g.B + (TRB ? (long)n0 : (long)n0 * g.ldb);
   const char *src_a, *src_b;
   const auto seek = [&] {      // where the next stage comes from
-    src_a = reinterpret_cast<const char*>(base_a + (long)((kPairA >> (4 * pair)) & 15u) * g.plane_a + step * 64);
-    src_b = reinterpret_cast<const char*>(base_b + (long)((kPairB >> (4 * pair)) & 15u) * g.plane_b + step * 64);
+    src_a = reinterpret_cast<const char*>(base_a + (long)((kPairA >> (4 * pair)) & 15u) * g.plane_a + (TRA ? step * 64 * g.lda : step * 64));
+    src_b = reinterpret_cast<const char*>(base_b + (long)((kPairB >> (4 * pair)) & 15u) * g.plane_b + (TRB ? step * 64 * g.ldb : step * 64));
+    if (step == g.ksteps - 1) {      // (and that is where these offsets stay)
+      const int left = g.K - (int)step * 64;
+      if (TRA && left < 64) tn_offsets<T::BM, T::NT, TRA>(off_a, g.lda, m0, g.M, left);
+      if (TRB && left < 64) tn_offsets<T::BN, T::NT, TRB>(off_b, g.ldb, n0, g.N, left);
+    }
     if (++pair == g.pairs) { pair = 0; ++step; }
   };
   const auto load = [&](int stage, int r0, int r1) {    // rounds r0 .. r1 - 1 of A's followed by B's
@@ -105,23 +128,77 @@ __device__ __forceinline__ void tn_product(const TnArgs& g, char* lds, int m0, i
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[i][j][k] = 0.f;
   if (it0 >= it1) return;
-  // fragments: this lane's row is lane & 15 of 16, its chunk 4 ks + (lane >> 4) for the two halves ks of a stage
+  // Contiguous in k: this lane's row is lane & 15 of 16, its chunk 4 ks + (lane >> 4) for the two halves ks of a stage.
   uint32_t slot[2];
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) slot[ks] = (uint32_t)((lane & 15) * 128 + (((4 * ks + (lane >> 4)) ^ tn_turn(lane & 15)) * 16));
+  // Else: the address this lane gives for row 8 (lane >> 4) + (lane >> 2 & 3) of k, in the block of 16 m that its turn makes of block i
+  const uint32_t block = ((lane >> 2) & 3) | ((lane >> 2) & 4), row = (uint32_t)(8 * (lane >> 4) + ((lane >> 2) & 3)), within = (lane & 3) * 8;
+  uint32_t tr_a[TRA ? T::MI : 1], tr_b[TRB ? T::NI : 1];
+#pragma unroll
+  for (int i = 0; i < (TRA ? T::MI : 1); ++i) tr_a[i] = row * (T::BM * 2) + (((wm * T::MI + i) ^ block) * 32) + within;
+#pragma unroll
+  for (int j = 0; j < (TRB ? T::NI : 1); ++j) tr_b[j] = T::BM * 128 + row * (T::BN * 2) + (((wn * T::NI + j) ^ block) * 32) + within;
   const uint32_t frag_a = wm * T::WM * 128, frag_b = T::BM * 128 + wn * T::WN * 128;
   constexpr int HALF = T::MI / 2;
+  static_assert(!TRA || HALF == 4 || HALF == 2, "");
+  static_assert(!TRB || T::NI % 4 == 0, "");
   tn_frag a[T::MI], b[2][T::NI];
+  // The builtin for these reads makes the compiler wait for every global_load_lds in flight first, so they are written out, with their wait:
+  // nothing is in flight when the block ends.  The other wave of the SIMD multiplies meanwhile.
+  typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+  const auto turned4 = [&](tn_frag* out, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, auto pitch) {
+    u32x2v r0, r1, r2, r3, r4, r5, r6, r7;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3), "=&v"(r4), "=&v"(r5), "=&v"(r6), "=&v"(r7)
+        : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(4 * decltype(pitch)::value));
+    out[0] = __builtin_bit_cast(tn_frag, __builtin_shufflevector(r0, r1, 0, 1, 2, 3));
+    out[1] = __builtin_bit_cast(tn_frag, __builtin_shufflevector(r2, r3, 0, 1, 2, 3));
+    out[2] = __builtin_bit_cast(tn_frag, __builtin_shufflevector(r4, r5, 0, 1, 2, 3));
+    out[3] = __builtin_bit_cast(tn_frag, __builtin_shufflevector(r6, r7, 0, 1, 2, 3));
+  };
+  const auto turned2 = [&](tn_frag* out, uint32_t a0, uint32_t a1, auto pitch) {
+    u32x2v r0, r1, r2, r3;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+        : "v"(a0), "v"(a1), "n"(4 * decltype(pitch)::value));
+    out[0] = __builtin_bit_cast(tn_frag, __builtin_shufflevector(r0, r1, 0, 1, 2, 3));
+    out[1] = __builtin_bit_cast(tn_frag, __builtin_shufflevector(r2, r3, 0, 1, 2, 3));
+  };
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   const auto read_a = [&](int i0, int i1, int stage, int ks) {
-    const char* s = lds + stage * T::STAGE + frag_a + slot[ks];
+    if constexpr (TRA) {
+      const uint32_t s = lds_at + stage * T::STAGE + ks * 32 * (T::BM * 2);
 #pragma unroll
-    for (int i = 0; i < T::MI; ++i)
-      if (i >= i0 && i < i1) a[i] = *reinterpret_cast<const tn_frag*>(s + i * 2048);
+      for (int i = 0; i < T::MI; i += HALF)      // a half is 4 or 2 fragments
+        if (i == i0) {
+          if constexpr (HALF == 4) turned4(a + i, s + tr_a[i], s + tr_a[i + 1], s + tr_a[i + 2], s + tr_a[i + 3], Int<T::BM * 2>{});
+          else turned2(a + i, s + tr_a[i], s + tr_a[i + 1], Int<T::BM * 2>{});
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+        if (i >= i0 && i < i1) a[i] = *reinterpret_cast<const tn_frag*>(lds + stage * T::STAGE + frag_a + slot[ks] + i * 2048);
+    }
   };
   const auto read_b = [&](int stage, int ks) {
-    const char* s = lds + stage * T::STAGE + frag_b + slot[ks];
+    if constexpr (TRB) {
+      const uint32_t s = lds_at + stage * T::STAGE + ks * 32 * (T::BN * 2);
 #pragma unroll
-    for (int j = 0; j < T::NI; ++j) b[ks][j] = *reinterpret_cast<const tn_frag*>(s + j * 2048);
+      for (int j = 0; j < T::NI; j += 4) turned4(b[ks] + j, s + tr_b[j], s + tr_b[j + 1], s + tr_b[j + 2], s + tr_b[j + 3], Int<T::BN * 2>{});
+    } else {
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) b[ks][j] = *reinterpret_cast<const tn_frag*>(lds + stage * T::STAGE + frag_b + slot[ks] + j * 2048);
+    }
   };
   const auto multiply = [&](int i0, int i1, int ks) {
     __builtin_amdgcn_sched_barrier(0);
