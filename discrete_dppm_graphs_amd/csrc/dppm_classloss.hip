@@ -47,6 +47,16 @@ __device__ __forceinline__ void split3(float v, uint16_t (&out)[3]) {
   if (!(fabsf(v) <= 3.3e38f)) { out[1] = 0; out[2] = 0; }     // infinity and NaN (and what rounds to infinity) stand in the first plane alone
 }
 
+// Stores of what the kernel does not read again.  Buffers larger than the 256 MB that the last cache holds go past the L2, where they would only
+// push operands out (bfloat16, 8192 x 131072 exponentials: scores 7.3 -> 6.8 ms); smaller ones are left for the next kernel to find
+// (float32, 2047 x 20011: 0.87 ms with stores past the L2, 0.83 without).
+template <class V>
+__device__ __forceinline__ void store_out(V v, V* p, bool past) {
+  if (past) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+constexpr size_t CACHED = 256u << 20;
+
 // ------------------------------------------------------------------------------------------------ counting rows, losses
 // 1 / denom, or 1 / (rows with a class) where none is given; every thread of the 1024 gets it
 __device__ __forceinline__ float inverse_of_rows(const int64_t* target, long T, long V, float denom) {
@@ -100,6 +110,7 @@ struct ScoreOut {
   void* e;                  // exponentials [rows][pitch], or null
   long pitch;
   int V;
+  bool past;                // e is larger than the caches
 };
 
 // m = class, n = row: a lane holds classes of one row per fragment, so that maxima and sums run inside lanes and then over four of them.
@@ -164,11 +175,11 @@ __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
           const long at = (long)n * o.pitch + c;
           if (F32) {
             f32x4* p = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(o.e) + at);
-            p[0] = f32x4{v[0], v[1], v[2], v[3]};
-            p[1] = f32x4{v[4], v[5], v[6], v[7]};
+            store_out(f32x4{v[0], v[1], v[2], v[3]}, p, o.past);
+            store_out(f32x4{v[4], v[5], v[6], v[7]}, p + 1, o.past);
           } else
-            *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(o.e) + at) =
-                u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+            store_out(u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])},
+                      reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(o.e) + at), o.past);
         }
       });
   }
@@ -226,6 +237,7 @@ struct TurnArgs {
   const float2* stats; const float* lse; const float* target_score; const int64_t* target; const float* row_weight; const float* inv;
   uint16_t* d; long plane;               // [planes][rows, whole tiles of 64][pitch]; e itself for bfloat16
   int rows, V, strip;                    // strip: classes that share a maximum
+  bool past;                             // d is larger than the caches
 };
 
 // 16 rows x 512 classes a workgroup, 8 classes a thread and row: d_tv = e_tv * exp(max_strip - lse_t) * w_t / n, the row's own class from its float32
@@ -287,10 +299,10 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
       for (int k = 0; k < 8; ++k) split3(x[k], s[k]);
 #pragma unroll
       for (int p = 0; p < P; ++p)
-        *reinterpret_cast<u32x4*>(a.d + p * a.plane + to) = u32x4{s[0][p] | (uint32_t)s[1][p] << 16, s[2][p] | (uint32_t)s[3][p] << 16,
-                                                                s[4][p] | (uint32_t)s[5][p] << 16, s[6][p] | (uint32_t)s[7][p] << 16};
+        store_out(u32x4{s[0][p] | (uint32_t)s[1][p] << 16, s[2][p] | (uint32_t)s[3][p] << 16, s[4][p] | (uint32_t)s[5][p] << 16, s[6][p] | (uint32_t)s[7][p] << 16},
+                  reinterpret_cast<u32x4*>(a.d + p * a.plane + to), a.past);
     } else
-      *reinterpret_cast<u32x4*>(a.d + to) = u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+      store_out(u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])}, reinterpret_cast<u32x4*>(a.d + to), a.past);
   }
 }
 
@@ -358,13 +370,13 @@ struct GradOut {
   void* c; long ldc;          // [N][ldc], M values a row
   const float* add;           // float32 [N][ldc] that is added first, or null
   float* part; long part_stride;   // with splits: float32 [splits][N][ldc] instead
-  int c_bf16, wide;           // wide: rows of c start on 16 bytes and M is a multiple of 8
+  int c_bf16, past, wide;     // past: c is larger than the caches; wide: rows of c start on 16 bytes and M is a multiple of 8
 };
 
 __device__ __forceinline__ void put8(const GradOut& o, long at, int left, const float (&v)[8]) {
   if (o.c_bf16) {
     uint16_t* p = reinterpret_cast<uint16_t*>(o.c) + at;
-    if (o.wide) *reinterpret_cast<u32x4*>(p) = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+    if (o.wide) store_out(u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])}, reinterpret_cast<u32x4*>(p), o.past);
     else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -533,7 +545,7 @@ int launch_grad(TnArgs g, const GradOut& o, hipStream_t st) {
 template <bool TRA, bool TRB>
 int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, size_t part_bytes, hipStream_t st) {
   GradOut o{};
-  o.c = c; o.ldc = g.M; o.add = add; o.c_bf16 = c_bf16;
+  o.c = c; o.ldc = g.M; o.add = add; o.c_bf16 = c_bf16; o.past = (size_t)g.M * g.N * (c_bf16 ? 2 : 4) > CACHED;
   o.wide = g.M % 8 == 0 && (uintptr_t)c % 16 == 0;
   const Shape shape = shape_of(g.M, g.N, (long)g.ksteps * g.pairs, true);
   g.splits = shape.splits;
@@ -612,6 +624,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     g.K = (int)D; g.ksteps = cdiv(D, 64); g.pairs = p.pairs; g.splits = 1;
     ScoreOut o{};
     o.stats = stats; o.target_score = f(p.tscore); o.target = target + t0; o.e = grad ? ws + p.e : nullptr; o.pitch = p.Vp; o.V = (int)V;
+    o.past = (size_t)rows * p.Vp * (p.f32 ? 4 : 2) > CACHED;
     if (p.tile_scores == 0) DPPM_TRY(p.f32 ? (launch_scores<Wide, true>(g, o, st)) : (launch_scores<Wide, false>(g, o, st)));
     else if (p.tile_scores == 1) DPPM_TRY(p.f32 ? (launch_scores<Mid, true>(g, o, st)) : (launch_scores<Mid, false>(g, o, st)));
     else DPPM_TRY(p.f32 ? (launch_scores<Narrow, true>(g, o, st)) : (launch_scores<Narrow, false>(g, o, st)));
@@ -623,7 +636,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     TurnArgs a{};
     a.e = ws + p.e; a.pitch = p.Vp; a.stats = stats; a.lse = f(p.lse); a.target_score = f(p.tscore); a.target = target + t0;
     a.row_weight = row_weight ? row_weight + t0 : nullptr; a.inv = f(p.inv);
-    a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip;
+    a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip; a.past = (size_t)p.planes * a.plane * 2 > CACHED;
     const dim3 grid((unsigned)cdiv(p.Vp, 512), (unsigned)(whole / 16));
     if (p.f32) hipLaunchKernelGGL((turn_kernel<true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((turn_kernel<false>), grid, dim3(256), 0, st, a);
