@@ -171,8 +171,8 @@ __global__ __launch_bounds__(256) void grad_sq_kernel(const dppm_tensor_entry* _
   if (threadIdx.x == 0) part[blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
 }
 
-__global__ __launch_bounds__(256) void grad_norm_kernel(const double* __restrict__ part, int n, double gscale, double max_norm, float* __restrict__ norm_out,
-                                                        NormOut* __restrict__ out) {
+// The partial sums of all workgroups, by 256 threads in a fixed order: the norm, and what the step reads.  All threads get the result.
+__device__ __forceinline__ NormOut clip_of(const double* part, int n, double gscale, double max_norm, float* norm_out) {
   __shared__ double w[4];
   double s = 0.0;
   for (int i = threadIdx.x; i < n; i += 256) s += part[i];
@@ -180,13 +180,16 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const double* __restrict
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const double norm = sqrt((w[0] + w[1]) + (w[2] + w[3])) * fabs(gscale);
-    const double coef = max_norm / (norm + 1e-6);
-    *norm_out = (float)norm;
-    out->ok = norm <= 1.7e308;                                     // false for infinity and NaN: the step leaves everything as it was
-    out->mult = (float)(gscale * (coef < 1.0 ? coef : 1.0));
-  }
+  const double norm = sqrt((w[0] + w[1]) + (w[2] + w[3])) * fabs(gscale);
+  const double coef = max_norm / (norm + 1e-6);
+  if (norm_out && threadIdx.x == 0) *norm_out = (float)norm;
+  return NormOut{(float)(gscale * (coef < 1.0 ? coef : 1.0)), norm <= 1.7e308};     // not ok for infinity and NaN: the step leaves everything as it was
+}
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(const double* __restrict__ part, int n, double gscale, double max_norm, float* __restrict__ norm_out,
+                                                        NormOut* __restrict__ out) {
+  const NormOut o = clip_of(part, n, gscale, max_norm, norm_out);
+  if (threadIdx.x == 0) *out = o;
 }
 
 template <bool GBF, int BITS, bool FULL>
@@ -276,15 +279,19 @@ __device__ __forceinline__ void adamw_chunk(const dppm_tensor_entry& e, long bas
   }
 }
 
+// clip: what grad_norm_kernel left; or null, and with parts > 0 every workgroup sums the few partial sums itself, which spares the launch
+struct Clip { const NormOut* clip; const double* part; int parts; double gscale, max_norm; float* norm_out; };
+constexpr int FEW_PARTS = 256;
+
 template <bool GBF, int BITS>
-__global__ __launch_bounds__(256) void adamw_kernel(const dppm_tensor_entry* __restrict__ tab, const int2* __restrict__ chunks, const NormOut* __restrict__ clip,
-                                                    StepArgs a) {
+__global__ __launch_bounds__(256) void adamw_kernel(const dppm_tensor_entry* __restrict__ tab, const int2* __restrict__ chunks, Clip clip, StepArgs a) {
   const int2 ch = chunks[blockIdx.x];
   const dppm_tensor_entry e = tab[ch.x];
   float mult = a.gscale;
-  if (clip) {
-    if (!clip->ok) return;
-    mult = clip->mult;
+  if (clip.clip || clip.parts > 0) {
+    const NormOut o = clip.clip ? *clip.clip : clip_of(clip.part, clip.parts, clip.gscale, clip.max_norm, blockIdx.x == 0 ? clip.norm_out : nullptr);
+    if (!o.ok) return;
+    mult = o.mult;
   }
   const long base = (long)ch.y * CHUNK;
   if (base + CHUNK <= e.numel) adamw_chunk<GBF, BITS, true>(e, base, (uint32_t)ch.x, mult, a);
@@ -314,16 +321,21 @@ extern "C" int dppm_adamw_step(const dppm_tensor_entry* table, const int32_t* ch
   }
   const hipStream_t st = as_stream(stream);
   const int2* ch = reinterpret_cast<const int2*>(chunks);
-  NormOut* no = nullptr;
+  Clip no{};
   if (clip) {
     double* part = reinterpret_cast<double*>(workspace);
-    no = reinterpret_cast<NormOut*>(part + NORM_GRID);
+    NormOut* out = reinterpret_cast<NormOut*>(part + NORM_GRID);
     const int grid = n_chunks < NORM_GRID ? n_chunks : NORM_GRID;
     if (grid > 0) {
       if (grad_bf16) hipLaunchKernelGGL((grad_sq_kernel<true>), dim3(grid), dim3(256), 0, st, table, ch, n_chunks, part);
       else hipLaunchKernelGGL((grad_sq_kernel<false>), dim3(grid), dim3(256), 0, st, table, ch, n_chunks, part);
     }
-    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, st, part, grid, grad_scale, max_norm, norm_out, no);
+    if (grid > 0 && grid <= FEW_PARTS) {
+      no.part = part; no.parts = grid; no.gscale = grad_scale; no.max_norm = max_norm; no.norm_out = norm_out;
+    } else {
+      hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, st, part, grid, grad_scale, max_norm, norm_out, out);
+      no.clip = out;
+    }
   }
   if (n_chunks > 0) {
     StepArgs a;

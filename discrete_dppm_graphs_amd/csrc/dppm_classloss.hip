@@ -58,49 +58,44 @@ __device__ __forceinline__ void store_out(V v, V* p, bool past) {
 constexpr size_t CACHED = 256u << 20;
 
 // ------------------------------------------------------------------------------------------------ counting rows, losses
-// 1 / denom, or 1 / (rows with a class) where none is given; every thread of the 1024 gets it
+// 1 / denom, or 1 / (rows with a class) where none is given; all NT threads get it
+template <int NT>
 __device__ __forceinline__ float inverse_of_rows(const int64_t* target, long T, long V, float denom) {
-  __shared__ uint32_t w[16];
+  __shared__ uint32_t w[NT / 64];
   uint32_t n = 0;
   if (!(denom > 0.f)) {
-#pragma unroll 4
-    for (long t = threadIdx.x; t < T; t += 1024) n += target[t] >= 0 && target[t] < V;
+#pragma unroll 8
+    for (long t = threadIdx.x; t < T; t += NT) n += target[t] >= 0 && target[t] < V;
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = n;
   __syncthreads();
   uint32_t all = 0;
-  for (int i = 0; i < 16; ++i) all += w[i];
+  for (int i = 0; i < NT / 64; ++i) all += w[i];
   return 1.f / (denom > 0.f ? denom : (float)(all ? all : 1u));
 }
 
-__global__ __launch_bounds__(1024) void count_kernel(const int64_t* __restrict__ target, long T, long V, float denom, float* __restrict__ inv) {
-  const float x = inverse_of_rows(target, T, V, denom);
-  if (threadIdx.x == 0) *inv = x;
-}
+struct LossArgs { const float *row_loss, *row_weight; const int64_t* target; long T, V; float denom; float* loss; };   // loss null: nothing to do
 
-// `inv`: what count_kernel left, or null (no gradients: nothing needed it before)
-__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ row_loss, const float* __restrict__ row_weight, const int64_t* __restrict__ target, long V,
-                                                    float denom, const float* __restrict__ inv, long T, float* __restrict__ loss) {
-  __shared__ double w[16];
+// The loss of all rows, by one workgroup of 256, in float64 and a fixed order.  `inv`: 1 / n, or null where nothing needed it before.
+__device__ __forceinline__ void sum_loss(const LossArgs& a, const float* inv) {
+  __shared__ double w[4];
   double s = 0.0;
-#pragma unroll 4
-  for (long t = threadIdx.x; t < T; t += 1024) {
-    const float l = row_loss[t];
-    if (l != 0.f) s += (double)l * (row_weight ? row_weight[t] : 1.f);      // rows without a class have 0, whatever their weight
+#pragma unroll 8
+  for (long t = threadIdx.x; t < a.T; t += 256) {
+    const float l = a.row_loss[t];
+    if (l != 0.f) s += (double)l * (a.row_weight ? a.row_weight[t] : 1.f);      // rows without a class have 0, whatever their weight
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
-  const float scale = inv ? *inv : inverse_of_rows(target, T, V, denom);
+  const float scale = inv ? *inv : inverse_of_rows<256>(a.target, a.T, a.V, a.denom);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double all = 0.0;
-    for (int i = 0; i < 16; ++i) all += w[i];
-    *loss = (float)(all * scale);
-  }
+  if (threadIdx.x == 0) *a.loss = (float)(((w[0] + w[1]) + (w[2] + w[3])) * scale);
 }
+
+__global__ __launch_bounds__(256) void loss_kernel(LossArgs a) { sum_loss(a, nullptr); }
 
 // ------------------------------------------------------------------------------------------------ scores
 struct ScoreOut {
@@ -243,7 +238,11 @@ struct TurnArgs {
 // 16 rows x 512 classes a workgroup, 8 classes a thread and row: d_tv = e_tv * exp(max_strip - lse_t) * w_t / n, the row's own class from its float32
 // score.  Rows behind the last (to whole tiles of 64) and without a class are zeros; so are classes behind the last, to the pitch.
 template <bool F32>
-__global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
+__global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
+  if (blockIdx.y == gridDim.y - 1) {      // one more row of workgroups: its first sums the loss, with the last block of rows
+    if (blockIdx.x == 0 && l.loss) sum_loss(l, a.inv);
+    return;
+  }
   constexpr int P = F32 ? 3 : 1, ROWS = 16;
   __shared__ float factor[16][ROWS];     // of each 32 classes: strips of 32 are the shortest
   __shared__ float own[ROWS];
@@ -309,13 +308,24 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a) {
 // ------------------------------------------------------------------------------------------------ operands
 // [rows][cols] of the caller, contiguous -> bfloat16 planes, as they stand [rows][pitch] (cols .. pitch zero) and/or transposed [cols][pitch_t]
 // (rows .. pitch_t zero).  target, V (or null): rows without a class are zeros.  64 x 64 a workgroup.
-// WIDE: cols and the source's address allow 16-byte reads (4 or 8 values).
+struct LayOut {
+  const void* src; int rows, cols;
+  uint16_t* as_is; long pitch, plane;
+  uint16_t* turned; long pitch_t, plane_t;
+  const int64_t* target; long V;
+  int across, wide;      // tiles across; wide: cols and the source's address allow 16-byte reads (4 or 8 values)
+};
+
 template <bool F32, bool WIDE>
-__global__ __launch_bounds__(256) void lay_out_kernel(const void* __restrict__ src, int rows, int cols, uint16_t* __restrict__ as_is, long pitch, long plane,
-                                                      uint16_t* __restrict__ turned, long pitch_t, long plane_t, const int64_t* __restrict__ target, long V) {
+__device__ __forceinline__ void lay_out_tile(const LayOut& a, int id) {
+  const void* src = a.src;
+  const int rows = a.rows, cols = a.cols;
+  uint16_t *as_is = a.as_is, *turned = a.turned;
+  const long pitch = a.pitch, plane = a.plane, pitch_t = a.pitch_t, plane_t = a.plane_t, V = a.V;
+  const int64_t* target = a.target;
   constexpr int P = F32 ? 3 : 1, VEC = WIDE ? (F32 ? 4 : 8) : 1, PER_ROW = 64 / VEC;
   __shared__ uint16_t tile[P][64][66];
-  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
+  const int c0 = id % a.across * 64, r0 = id / a.across * 64;
 #pragma unroll 4
   for (int i = threadIdx.x; i < 64 * PER_ROW; i += 256) {
     const int r = i / PER_ROW, c = i % PER_ROW * VEC;
@@ -363,6 +373,24 @@ __global__ __launch_bounds__(256) void lay_out_kernel(const void* __restrict__ s
       for (int k = 0; k < 4; ++k) w[k] = (uint32_t)tile[p][r + 2 * k][c] | ((uint32_t)tile[p][r + 2 * k + 1][c] << 16);
       *reinterpret_cast<u32x4*>(turned + p * plane_t + (long)(c0 + c) * pitch_t + r0 + r) = u32x4{w[0], w[1], w[2], w[3]};
     }
+}
+
+// Everything that can be laid out before the products, in one launch: `first` workgroups for a, `second` for b, and one more that leaves
+// 1 / n in inv (null: not wanted).
+template <bool F32>
+__global__ __launch_bounds__(256) void prepare_kernel(LayOut a, int first, LayOut b, int second, const int64_t* __restrict__ target, long T, long V, float denom,
+                                                      float* __restrict__ inv) {
+  const int id = blockIdx.x;
+  if (id < first) {
+    if (a.wide) lay_out_tile<F32, true>(a, id);
+    else lay_out_tile<F32, false>(a, id);
+  } else if (id < first + second) {
+    if (b.wide) lay_out_tile<F32, true>(b, id - first);
+    else lay_out_tile<F32, false>(b, id - first);
+  } else if (inv) {
+    const float x = inverse_of_rows<256>(target, T, V, denom);
+    if (threadIdx.x == 0) *inv = x;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
@@ -560,17 +588,12 @@ int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, 
   return DPPM_OK;
 }
 
-template <bool F32>
-void lay_out(const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, const int64_t* target, long V, hipStream_t st) {
-  const long r = turned ? (pitch_t > rows ? pitch_t : rows) : rows, c = as_is ? pitch : cols;
-  const dim3 grid((unsigned)cdiv(c, 64), (unsigned)cdiv(r, 64));
-  const bool wide = (uintptr_t)src % 16 == 0 && cols % (F32 ? 4 : 8) == 0;
-  if (wide) hipLaunchKernelGGL((lay_out_kernel<F32, true>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t, target, V);
-  else hipLaunchKernelGGL((lay_out_kernel<F32, false>), grid, dim3(256), 0, st, src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t, target, V);
-}
-void lay_out(bool f32, const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, const int64_t* target, long V, hipStream_t st) {
-  if (f32) lay_out<true>(src, rows, cols, as_is, pitch, turned, pitch_t, target, V, st);
-  else lay_out<false>(src, rows, cols, as_is, pitch, turned, pitch_t, target, V, st);
+// -> workgroups for it
+int lay_out(LayOut& a, bool f32, const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, const int64_t* target, long V) {
+  const long r = turned && pitch_t > rows ? pitch_t : rows, c = as_is ? pitch : cols;
+  a = LayOut{src, (int)rows, (int)cols, as_is, pitch, rows * pitch, turned, pitch_t, cols * pitch_t, target, V, cdiv(c, 64),
+             (uintptr_t)src % 16 == 0 && cols % (f32 ? 4 : 8) == 0};
+  return a.across * cdiv(r, 64);
 }
 
 bool sizes_ok(int64_t T, int64_t V, int64_t D) { return T >= 0 && V >= 1 && D >= 1 && T < (1L << 30) && V <= (1L << 23) && D <= (1L << 16); }   // 255 rows of any operand lie within 2^32 bytes
@@ -609,12 +632,24 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
   const auto h = [&](size_t at) { return reinterpret_cast<uint16_t*>(ws + at); };
   const auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
   float2* stats = reinterpret_cast<float2*>(ws + p.stats);
-  if (grad) hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, st, target, (long)T, (long)V, (float)denom, f(p.inv));
   const uint16_t *xp = reinterpret_cast<const uint16_t*>(x), *wp = reinterpret_cast<const uint16_t*>(weight);
-  if (!p.direct) {
-    lay_out(p.f32, weight, V, D, h(p.wp), p.Kp, nullptr, 0, nullptr, 0, st);
-    lay_out(p.f32, x, T, D, h(p.xp), p.Kp, nullptr, 0, nullptr, 0, st);
-    xp = h(p.xp); wp = h(p.wp);
+  const size_t es = bf16 ? 2 : 4;
+  const LossArgs loss{row_loss, row_weight, target, (long)T, (long)V, (float)denom, loss_out};
+  const auto prepare = [&](const LayOut& a, int first, const LayOut& b, int second, float* inv) {
+    const int grid = first + second + (inv ? 1 : 0);
+    if (grid == 0) return;
+    if (p.f32) hipLaunchKernelGGL((prepare_kernel<true>), dim3(grid), dim3(256), 0, st, a, first, b, second, target, (long)T, (long)V, (float)denom, inv);
+    else hipLaunchKernelGGL((prepare_kernel<false>), dim3(grid), dim3(256), 0, st, a, first, b, second, target, (long)T, (long)V, (float)denom, inv);
+  };
+  {
+    // a single block's transposed x is made here too; rows of x without a class are zeros in both, which changes nothing that counts
+    LayOut w{}, xs{};
+    int first = 0, second = 0;
+    const bool turn_x = grad && p.blocks == 1;
+    if (!p.direct) first = lay_out(w, p.f32, weight, V, D, h(p.wp), p.Kp, nullptr, 0, nullptr, 0);
+    if (!p.direct || turn_x) second = lay_out(xs, p.f32, x, T, D, p.direct ? nullptr : h(p.xp), p.Kp, turn_x ? h(p.xt) : nullptr, p.Rp, target, V);
+    prepare(w, first, xs, second, grad ? f(p.inv) : nullptr);
+    if (!p.direct) { xp = h(p.xp); wp = h(p.wp); }
   }
   for (int b = 0; b < p.blocks; ++b) {
     const long t0 = b * p.R, rows = T - t0 < p.R ? T - t0 : p.R, Rp = pitch_of(rows);
@@ -637,11 +672,17 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     a.e = ws + p.e; a.pitch = p.Vp; a.stats = stats; a.lse = f(p.lse); a.target_score = f(p.tscore); a.target = target + t0;
     a.row_weight = row_weight ? row_weight + t0 : nullptr; a.inv = f(p.inv);
     a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip; a.past = (size_t)p.planes * a.plane * 2 > CACHED;
-    const dim3 grid((unsigned)cdiv(p.Vp, 512), (unsigned)(whole / 16));
-    if (p.f32) hipLaunchKernelGGL((turn_kernel<true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((turn_kernel<false>), grid, dim3(256), 0, st, a);
-    const size_t es = bf16 ? 2 : 4;
-    lay_out(p.f32, reinterpret_cast<const char*>(x) + t0 * D * es, rows, D, nullptr, 0, h(p.xt), Rp, target + t0, V, st);
+    const bool last = b == p.blocks - 1;
+    LossArgs sum = loss;
+    if (!last) sum.loss = nullptr;
+    const dim3 grid((unsigned)cdiv(p.Vp, 512), (unsigned)(whole / 16 + 1));
+    if (p.f32) hipLaunchKernelGGL((turn_kernel<true>), grid, dim3(256), 0, st, a, sum);
+    else hipLaunchKernelGGL((turn_kernel<false>), grid, dim3(256), 0, st, a, sum);
+    if (p.blocks > 1) {
+      LayOut xs{};
+      const int n = lay_out(xs, p.f32, reinterpret_cast<const char*>(x) + t0 * D * es, rows, D, nullptr, 0, h(p.xt), Rp, target + t0, V);
+      prepare(xs, n, xs, 0, nullptr);
+    }
     TnArgs gx{};       // dx[t][d] = sum_v d[t][v] W[v][d]
     gx.A = wp; gx.lda = p.Kp; gx.plane_a = V * p.Kp; gx.M = (int)D;
     gx.B = a.d; gx.ldb = p.Vp; gx.plane_b = a.plane; gx.N = (int)rows;
@@ -651,10 +692,9 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     gw.A = h(p.xt); gw.lda = Rp; gw.plane_a = D * Rp; gw.M = (int)D;
     gw.B = a.d; gw.ldb = p.Vp; gw.plane_b = a.plane; gw.N = (int)V;
     gw.K = whole; gw.ksteps = cdiv(rows, 64); gw.pairs = p.pairs;      // d has zeros to whole steps
-    const bool last = b == p.blocks - 1;
-    float* sum = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
-    DPPM_TRY((grad_product<false, true>)(gw, last || p.f32 ? dweight : (void*)sum, bf16 && last, b == 0 ? nullptr : sum, f(p.part), p.part_bytes, st));
+    float* total = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
+    DPPM_TRY((grad_product<false, true>)(gw, last || p.f32 ? dweight : (void*)total, bf16 && last, b == 0 ? nullptr : total, f(p.part), p.part_bytes, st));
   }
-  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, target, (long)V, (float)denom, grad ? f(p.inv) : nullptr, (long)T, loss_out);
+  if (!grad) hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(256), 0, st, loss);
   return check_launch("dppm_loss_ce_fwd_bwd");
 }
