@@ -1,0 +1,49 @@
+"""Differentiable fronts of the operators for categorical states: classes looked up in a table on the way into a network, and the softmax
+cross entropy over classes on the way out (the counterpart of ppgn_simple.loss_func_bce and ppgn_vlb.loss_func_kld where a state has more
+than two values).  The reference's states are binary; nothing in it corresponds."""
+import torch
+
+from . import ops
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale = weight.shape[0], scale
+        return ops.embedding_fwd(weight, ids, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        return ops.embedding_wgrad(g.contiguous(), ids, ctx.rows, ctx.scale), None, None
+
+
+def embedding(weight, ids, scale=1.0):
+    """scale * weight[ids], differentiable with respect to weight [V, D] (float32 or bfloat16); an id outside [0, V) gives zeros and no
+    gradient."""
+    return _Embedding.apply(weight.contiguous(), ids.contiguous(), float(scale))
+
+
+class _ClassLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, row_weight, denom):
+        loss, _, dx, dweight = ops.loss_ce(x, weight, target, row_weight, denom, want_grad=any(ctx.needs_input_grad[:2]))
+        ctx.save_for_backward(dx, dweight)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        dx, dweight = ctx.saved_tensors
+        return (dx * g.to(dx.dtype) if ctx.needs_input_grad[0] else None, dweight * g.to(dweight.dtype) if ctx.needs_input_grad[1] else None,
+                None, None, None)
+
+
+def loss_func_ce(x, weight, target, row_weight=None, denom=None):
+    """Softmax cross entropy of the classes' rows weight [V, D] against the last hidden layer x [..., D] (float32 scalar, differentiable
+    with respect to x and weight): ops.loss_ce over the flattened positions; target [...] int64, outside [0, V): no class."""
+    d = x.shape[-1]
+    return _ClassLoss.apply(x.reshape(-1, d).contiguous(), weight.contiguous(), target.reshape(-1).contiguous(),
+                            None if row_weight is None else row_weight.reshape(-1).contiguous(), denom)

@@ -49,9 +49,19 @@ class FlatState:
     """Trained parameters of a `Powerful` (or a conditioning variant) re-homed into one contiguous float32 buffer (each nn.Parameter becomes a view,
     names and shapes unchanged), plus a flat gradient bucket and Adam moments.  Unused parameters (time_mlp,
     feature_extractors) never receive gradients in the reference either and are left alone, exactly as
-    torch.optim.Adam skips parameters whose .grad is None."""
+    torch.optim.Adam skips parameters whose .grad is None.
 
-    def __init__(self, model, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0):
+    optimizer: "adam" (the reference's: L2 weight decay), "adamw" (decoupled weight decay, ops.adamw_step over all tensors) or "adamw8" (the
+    same with moments in 8 bits, rounded with random bits keyed by `seed`).  max_grad_norm (adamw, adamw8): the gradients' norm over all
+    tensors is clipped to it; self.grad_norm is the last step's norm before clipping, on the device."""
+
+    OPTIMIZERS = ("adam", "adamw", "adamw8")
+
+    def __init__(self, model, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, optimizer="adam", max_grad_norm=None, seed=0):
+        if optimizer not in self.OPTIMIZERS:
+            raise ValueError(f"optimizer {optimizer!r}: expected one of {self.OPTIMIZERS}")
+        if max_grad_norm is not None and (optimizer == "adam" or not max_grad_norm > 0):
+            raise ValueError(f"max_grad_norm {max_grad_norm}: a positive number, with optimizer 'adamw' or 'adamw8'")
         self.model = model
         self.names = model.trainable_param_names()
         named = dict(model.named_parameters())
@@ -64,8 +74,10 @@ class FlatState:
         n = self.offsets[-1]
         self.flat = torch.zeros(n, device=dev)
         self.grad = torch.zeros(n, device=dev)
-        self.exp_avg = torch.zeros(n, device=dev)
-        self.exp_avg_sq = torch.zeros(n, device=dev)
+        self.optimizer, self.max_grad_norm, self.seed, self.grad_norm, self.tensors = optimizer, max_grad_norm, int(seed), None, None
+        if optimizer == "adam":
+            self.exp_avg = torch.zeros(n, device=dev)
+            self.exp_avg_sq = torch.zeros(n, device=dev)
         grads = {}
         for name, p, off in zip(self.names, params, self.offsets):
             view = self.flat[off:off + p.numel()].view_as(p)
@@ -76,6 +88,9 @@ class FlatState:
         self.grad_pack = model.make_grad_pack(grads)
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         self.step_count = 0
+        if optimizer != "adam":
+            self.tensors = ops.TensorSet([p.data for p in params], [grads[name] for name in self.names], weight_decay=weight_decay,
+                                         state_bits=8 if optimizer == "adamw8" else 32)
         model._pack_cache = None
 
     def numel(self):
@@ -89,38 +104,57 @@ class FlatState:
 
     def adam_step(self, lr=None):
         self.step_count += 1
+        if self.tensors is not None:
+            self.grad_norm = ops.adamw_step(self.tensors, self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps, self.step_count,
+                                            max_norm=self.max_grad_norm, seed=self.seed)
+            return
         ops.adam_step(self.flat, self.grad, self.exp_avg, self.exp_avg_sq, self.lr if lr is None else lr, self.betas[0],
                       self.betas[1], self.eps, self.weight_decay, self.step_count)
 
     def state_dict(self):
         """Optimizer state as saved in the checkpoint's 'optimizer_state_dict' (flat moments + hyper-parameters)."""
-        return {'step': self.step_count, 'exp_avg': self.exp_avg, 'exp_avg_sq': self.exp_avg_sq, 'lr': self.lr,
-                'betas': list(self.betas), 'eps': self.eps, 'weight_decay': self.weight_decay, 'names': list(self.names),
-                'offsets': list(self.offsets)}
+        sd = {'step': self.step_count, 'lr': self.lr, 'betas': list(self.betas), 'eps': self.eps, 'weight_decay': self.weight_decay,
+              'names': list(self.names), 'offsets': list(self.offsets)}
+        if self.tensors is not None:
+            return {**sd, **self.tensors.state, 'optimizer': self.optimizer, 'offsets': list(self.tensors.offsets), 'seed': self.seed}
+        return {**sd, 'exp_avg': self.exp_avg, 'exp_avg_sq': self.exp_avg_sq}
 
     def load_state_dict(self, sd):
         """Restore what state_dict() saved.  The moments must belong to the same parameter layout (names / offsets are
         checked when present); a reference checkpoint's torch.optim.Adam state is not accepted here - its per-parameter
         tensors are keyed by index over ALL parameters, not by name."""
-        if 'exp_avg' not in sd or 'exp_avg_sq' not in sd:
+        if sd.get('optimizer', 'adam') != self.optimizer:
+            raise ValueError("FlatState.load_state_dict: a state of optimizer %r, this one is %r" % (sd.get('optimizer', 'adam'), self.optimizer))
+        moments = self.tensors.state if self.tensors is not None else {'exp_avg': self.exp_avg, 'exp_avg_sq': self.exp_avg_sq}
+        if any(k not in sd for k in moments):
             raise ValueError("FlatState.load_state_dict: not a flat optimizer state (a torch.optim.Adam state_dict cannot be resumed)")
         if 'names' in sd and list(sd['names']) != list(self.names):
             raise ValueError("FlatState.load_state_dict: parameter names differ from this model's")
-        if sd['exp_avg'].numel() != self.exp_avg.numel():
-            raise ValueError("FlatState.load_state_dict: moment size %d != %d" % (sd['exp_avg'].numel(), self.exp_avg.numel()))
-        self.exp_avg.copy_(sd['exp_avg'].to(self.exp_avg.device))
-        self.exp_avg_sq.copy_(sd['exp_avg_sq'].to(self.exp_avg_sq.device))
+        for k, m in moments.items():
+            if sd[k].numel() != m.numel() or sd[k].dtype != m.dtype:
+                raise ValueError("FlatState.load_state_dict: moment size %d (%s) != %d (%s)" % (sd[k].numel(), sd[k].dtype, m.numel(), m.dtype))
+        for k, m in moments.items():
+            m.copy_(sd[k].to(m.device))
+        self.seed = int(sd.get('seed', self.seed))
         self.step_count = int(sd['step'])
         self.lr = float(sd.get('lr', self.lr))
         self.betas = tuple(sd.get('betas', self.betas))
         self.eps = float(sd.get('eps', self.eps))
         self.weight_decay = float(sd.get('weight_decay', self.weight_decay))
+        if self.tensors is not None:
+            self.tensors.set_weight_decay(self.weight_decay)
 
     def publish_grads(self):
         """Expose the flat bucket as .grad on the parameters (for callers that want to inspect or clip)."""
         named = dict(self.model.named_parameters())
         for name in self.names:
             named[name].grad = self.grad_views[name]
+
+
+def optimizer_options(config):
+    """FlatState's optimizer arguments from a configuration: train.optimizer ("adam" unless given) and train.max_grad_norm."""
+    return {"optimizer": getattr(config.train, "optimizer", "adam"), "max_grad_norm": getattr(config.train, "max_grad_norm", None),
+            "seed": int(getattr(config, "seed", 0))}
 
 
 # ---------------------------------------------------------------------------------------------- training steps

@@ -513,10 +513,9 @@ class TensorSet:
             if p.device != self.params[0].device:
                 raise ValueError(f"params[{i}]: on {p.device}, params[0] on {self.params[0].device}")
         self.copies = [None] * n if copies is None else list(copies)
-        self.weight_decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
-        for name, v in (("copies", self.copies), ("weight_decay", self.weight_decay)):
-            if len(v) != n:
-                raise ValueError(f"{name}: {len(v)} entries for {n} tensors")
+        if len(self.copies) != n:
+            raise ValueError(f"copies: {len(self.copies)} entries for {n} tensors")
+        self.weight_decay = self._per_tensor(weight_decay)
         for i, c in enumerate(self.copies):
             if c is not None:
                 _chk(c, f"copies[{i}]", None, torch.bfloat16)
@@ -536,6 +535,17 @@ class TensorSet:
         self.table = torch.empty(n, 9, device=self.device, dtype=torch.int64)
         self.workspace = torch.empty(lib.dppm_adamw_workspace_bytes() // 8, device=self.device, dtype=torch.float64)
         self.set_grads(grads)
+
+    def _per_tensor(self, weight_decay):
+        w = [float(weight_decay)] * len(self.params) if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        if len(w) != len(self.params):
+            raise ValueError(f"weight_decay: {len(w)} entries for {len(self.params)} tensors")
+        return w
+
+    def set_weight_decay(self, weight_decay):
+        """One number, or one for each tensor (and the table is laid out again)."""
+        self.weight_decay = self._per_tensor(weight_decay)
+        self.set_grads(self.grads)
 
     def _state(self, given):
         total = self.offsets[-1]

@@ -207,7 +207,8 @@ def train_main(config, args):
     model = get_score_model(config)
     total_params = sum(p.numel() for p in model.parameters())
     logging.info(f"Parameters Count: {total_params}, Trainable: {sum(p.numel() for p in model.parameters() if p.requires_grad)}")
-    state = engine.FlatState(model, lr=config.train.lr_init, betas=(0.9, 0.999), eps=1e-8, weight_decay=config.train.weight_decay)
+    state = engine.FlatState(model, lr=config.train.lr_init, betas=(0.9, 0.999), eps=1e-8, weight_decay=config.train.weight_decay,
+                             **engine.optimizer_options(config))
     return fit(model, state, None, train_dl, max_node_number=config.dataset.max_node_num, max_epoch=config.train.max_epoch,
                config=config, save_interval=config.train.save_interval, sample_interval=config.train.sample_interval,
                sigma_length=len(config.train.sigmas), sample_from_sigma_delta=0.0, test_dl=test_dl,

@@ -121,7 +121,8 @@ def train_main(config, args):
     set_seed_and_logger(config, args)
     train_dl, test_dl = load_data(config)
     model = get_score_model(config)
-    state = engine.FlatState(model, lr=config.train.lr_init, betas=(0.9, 0.999), eps=1e-8, weight_decay=config.train.weight_decay)
+    state = engine.FlatState(model, lr=config.train.lr_init, betas=(0.9, 0.999), eps=1e-8, weight_decay=config.train.weight_decay,
+                             **engine.optimizer_options(config))
     return fit(model, state, None, train_dl, max_node_number=config.dataset.max_node_num, max_epoch=config.train.max_epoch,
                config=config, save_interval=config.train.save_interval, sample_interval=config.train.sample_interval,
                test_dl=test_dl, resume=getattr(args, "resume", None) or None)

@@ -102,3 +102,18 @@ def test_loss_ce_entry_refuses():
     # beside a copy of x, memory is that of one block of rows, whatever their number
     many, more = lib.dppm_loss_ce_workspace_bytes(1 << 16, 1 << 17, 1024, 1, 1), lib.dppm_loss_ce_workspace_bytes(1 << 17, 1 << 17, 1024, 1, 1)
     assert more - many <= (1 << 16) * 1088 * 2 + 4096 and more < 8 << 30
+
+
+def test_optimizer_options_come_from_the_configuration():
+    from discrete_dppm_graphs_amd import engine
+    from discrete_dppm_graphs_amd.utils.easydict import EasyDict
+    assert engine.optimizer_options(EasyDict(train=dict(lr_init=0.1))) == {"optimizer": "adam", "max_grad_norm": None, "seed": 0}
+    assert engine.optimizer_options(EasyDict(seed=7, train=dict(optimizer="adamw8", max_grad_norm=1.0))) == {"optimizer": "adamw8", "max_grad_norm": 1.0, "seed": 7}
+
+
+def test_differentiable_fronts_refuse_cpu_tensors():
+    from discrete_dppm_graphs_amd.categorical import embedding, loss_func_ce
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        embedding(torch.zeros(4, 2), torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        loss_func_ce(torch.zeros(3, 2), torch.zeros(4, 2), torch.zeros(3, dtype=torch.int64))
