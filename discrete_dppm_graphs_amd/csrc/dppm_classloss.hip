@@ -78,24 +78,29 @@ __device__ __forceinline__ float inverse_of_rows(const int64_t* target, long T, 
 
 struct LossArgs { const float *row_loss, *row_weight; const int64_t* target; long T, V; float denom; float* loss; };   // loss null: nothing to do
 
-// The loss of all rows, by one workgroup of 256, in float64 and a fixed order.  `inv`: 1 / n, or null where nothing needed it before.
+// The loss of all rows, by one workgroup, in float64 and a fixed order.  `inv`: 1 / n, or null where nothing needed it before.
+template <int NT>
 __device__ __forceinline__ void sum_loss(const LossArgs& a, const float* inv) {
-  __shared__ double w[4];
+  __shared__ double w[NT / 64];
   double s = 0.0;
 #pragma unroll 8
-  for (long t = threadIdx.x; t < a.T; t += 256) {
+  for (long t = threadIdx.x; t < a.T; t += NT) {
     const float l = a.row_loss[t];
     if (l != 0.f) s += (double)l * (a.row_weight ? a.row_weight[t] : 1.f);      // rows without a class have 0, whatever their weight
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
-  const float scale = inv ? *inv : inverse_of_rows<256>(a.target, a.T, a.V, a.denom);
+  const float scale = inv ? *inv : inverse_of_rows<NT>(a.target, a.T, a.V, a.denom);
   __syncthreads();
-  if (threadIdx.x == 0) *a.loss = (float)(((w[0] + w[1]) + (w[2] + w[3])) * scale);
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    for (int i = 0; i < NT / 64; ++i) all += w[i];
+    *a.loss = (float)(all * scale);
+  }
 }
 
-__global__ __launch_bounds__(256) void loss_kernel(LossArgs a) { sum_loss(a, nullptr); }
+__global__ __launch_bounds__(256) void loss_kernel(LossArgs a) { sum_loss<256>(a, nullptr); }
 
 // ------------------------------------------------------------------------------------------------ scores
 struct ScoreOut {
@@ -181,11 +186,11 @@ __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-// ROWS rows a workgroup, 256 / ROWS threads each over the strips: 32, so that a strip's line is read whole, or 2 for few rows
-template <int ROWS>
-__global__ __launch_bounds__(256) void rows_kernel(const float2* __restrict__ stats, int strips, int rows, const int64_t* __restrict__ target, long V,
+// ROWS rows a workgroup, NT / ROWS threads each over the strips: 32, so that a strip's line is read whole, or 2 for few rows
+template <int NT, int ROWS>
+__device__ __forceinline__ void reduce_rows(const float2* __restrict__ stats, int strips, int rows, const int64_t* __restrict__ target, long V,
                                                    const float* __restrict__ target_score, float* __restrict__ lse, float* __restrict__ row_loss) {
-  constexpr int LANES = 256 / ROWS, AHEAD = 8;
+  constexpr int LANES = NT / ROWS, AHEAD = 8;
   __shared__ float2 part[LANES][ROWS];
   const int r = threadIdx.x % ROWS, q = threadIdx.x / ROWS, n = blockIdx.x * ROWS + r;
   float top = -INFINITY, sum = 0.f;
@@ -226,6 +231,21 @@ __global__ __launch_bounds__(256) void rows_kernel(const float2* __restrict__ st
   }
 }
 
+template <int ROWS>
+__global__ __launch_bounds__(256) void rows_kernel(const float2* __restrict__ stats, int strips, int rows, const int64_t* __restrict__ target, long V,
+                                                   const float* __restrict__ target_score, float* __restrict__ lse, float* __restrict__ row_loss) {
+  reduce_rows<256, ROWS>(stats, strips, rows, target, V, target_score, lse, row_loss);
+}
+
+// Up to 8 rows and no gradients: rows and loss by one workgroup with 128 threads a row, which spares a launch (for 5 rows against 32768 classes;
+// with 32 threads a row, for up to 32 rows, it took 4 us longer than two launches)
+__global__ __launch_bounds__(1024) void rows_and_loss_kernel(const float2* __restrict__ stats, int strips, const float* __restrict__ target_score,
+                                                             float* __restrict__ lse, float* row_loss, LossArgs a) {
+  reduce_rows<1024, 8>(stats, strips, (int)a.T, a.target, a.V, target_score, lse, row_loss);
+  __syncthreads();
+  sum_loss<1024>(a, nullptr);
+}
+
 // ------------------------------------------------------------------------------------------------ turn
 struct TurnArgs {
   const void* e; long pitch;             // exponentials [rows][pitch]
@@ -240,7 +260,7 @@ struct TurnArgs {
 template <bool F32>
 __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
   if (blockIdx.y == gridDim.y - 1) {      // one more row of workgroups: its first sums the loss, with the last block of rows
-    if (blockIdx.x == 0 && l.loss) sum_loss(l, a.inv);
+    if (blockIdx.x == 0 && l.loss) sum_loss<256>(l, a.inv);
     return;
   }
   constexpr int P = F32 ? 3 : 1, ROWS = 16;
@@ -489,11 +509,13 @@ struct Plan {
 // memory (written and read once more, at 4 TB/s, and a launch).
 struct Shape { int wide; int splits; };
 Shape shape_of(long M, long N, long steps, bool may_split) {
+  static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
   Shape best{1, 1};
   double least = 1e300;
   for (int wide = 0; wide < 2; ++wide) {
     const long t = wide ? 256 : 128, tiles = cdiv(M, t) * (long)cdiv(N, t), slots = wide ? CUS : 2 * CUS;
-    for (long s = 1; s <= 64 && (s == 1 || (may_split && s * 8 <= steps && s * M * N <= (1L << 28))); ++s) {
+    for (const long s : kSplits) {
+      if (s > 1 && !(may_split && s * 8 <= steps && s * M * N <= (1L << 28))) break;
       const double us = (double)((tiles * s + slots - 1) / slots) * (double)((steps + s - 1) / s) * (wide ? 1.15 : 0.95) + (s > 1 ? 4.0 + (double)s * M * N * 8e-6 / 4.0 : 0.0);
       if (us < least) { least = us; best = Shape{wide, (int)s}; }
     }
@@ -597,12 +619,6 @@ int lay_out(LayOut& a, bool f32, const void* src, long rows, long cols, uint16_t
 }
 
 bool sizes_ok(int64_t T, int64_t V, int64_t D) { return T >= 0 && V >= 1 && D >= 1 && T < (1L << 30) && V <= (1L << 23) && D <= (1L << 16); }   // 255 rows of any operand lie within 2^32 bytes
-// the layout is the same whether or not the operands can be used where they are, so that the size does not depend on addresses
-Plan plan_for(int64_t T, int64_t V, int64_t D, bool bf16, bool grad, bool aligned) {
-  Plan p = plan_of(T, V, D, !bf16, grad, true);
-  if (p.direct && !aligned) p = plan_of(T, V, D, !bf16, grad, false);
-  return p;
-}
 
 }  // namespace
 }  // namespace dppm
@@ -611,8 +627,7 @@ using namespace dppm;
 
 extern "C" size_t dppm_loss_ce_workspace_bytes(int64_t T, int64_t V, int64_t D, int bf16, int want_grad) {
   if (!sizes_ok(T, V, D) || T == 0) return 0;
-  const size_t a = plan_for(T, V, D, bf16, want_grad, true).total, b = plan_for(T, V, D, bf16, want_grad, false).total;
-  return a > b ? a : b;
+  return plan_of(T, V, D, !bf16, want_grad, false).total;      // the larger of the two layouts, so that the size does not depend on addresses
 }
 
 extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16, const int64_t* target, const float* row_weight, double denom, int64_t T,
@@ -625,7 +640,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
   DPPM_REQUIRE((dx == nullptr) == (dweight == nullptr), "dppm_loss_ce_fwd_bwd: dx and dweight come together");
   DPPM_REQUIRE((uintptr_t)workspace % 16 == 0, "dppm_loss_ce_fwd_bwd: the workspace must be 16-byte aligned");
   const bool grad = dx != nullptr, aligned = ((uintptr_t)x | (uintptr_t)weight) % 16 == 0;
-  const Plan p = plan_for(T, V, D, bf16, grad, aligned);
+  const Plan p = plan_of(T, V, D, !bf16, grad, aligned);
   DPPM_REQUIRE(workspace_bytes >= p.total, "dppm_loss_ce_fwd_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
   const hipStream_t st = as_stream(stream);
   char* ws = reinterpret_cast<char*>(workspace);
@@ -664,6 +679,10 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     else if (p.tile_scores == 1) DPPM_TRY(p.f32 ? (launch_scores<Mid, true>(g, o, st)) : (launch_scores<Mid, false>(g, o, st)));
     else DPPM_TRY(p.f32 ? (launch_scores<Narrow, true>(g, o, st)) : (launch_scores<Narrow, false>(g, o, st)));
     // a thread's share of the strips is what takes the time: with few rows, more threads a row
+    if (!grad && T <= 8) {
+      hipLaunchKernelGGL(rows_and_loss_kernel, dim3(1), dim3(1024), 0, st, stats, p.strips, f(p.tscore), f(p.lse), row_loss, loss);
+      break;
+    }
     if (rows <= 64) hipLaunchKernelGGL((rows_kernel<2>), dim3(cdiv(rows, 2)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
     else hipLaunchKernelGGL((rows_kernel<32>), dim3(cdiv(rows, 32)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
     if (!grad) continue;
@@ -695,6 +714,6 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     float* total = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
     DPPM_TRY((grad_product<false, true>)(gw, last || p.f32 ? dweight : (void*)total, bf16 && last, b == 0 ? nullptr : total, f(p.part), p.part_bytes, st));
   }
-  if (!grad) hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(256), 0, st, loss);
+  if (!grad && T > 8) hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(256), 0, st, loss);
   return check_launch("dppm_loss_ce_fwd_bwd");
 }

@@ -15,16 +15,15 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _on(device):
-    """Context in which a launch goes to `device` and its current stream, whichever device is current."""
-    return _NO_CONTEXT if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-_NO_CONTEXT = contextlib.nullcontext()
-
-
-def _raw_stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _launch(index, fn, name, *args):
+    """fn(*args, stream) with the current stream of GPU `index`, which is made the current device if it is not."""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(rc, name)
 
 
 def _chk(t, name, shape=None, dtype=torch.float32):
@@ -396,37 +395,38 @@ def adam_step(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, weight_de
 
 
 # ------------------------------------------------------------------------------------------------- categorical states
-_FLOATS = (torch.float32, torch.bfloat16)
+_BF16 = torch.bfloat16
 
 
 def _chk_float(t, name, shape=None):
-    """A contiguous float32 or bfloat16 tensor on the GPU."""
-    if isinstance(t, torch.Tensor) and t.dtype not in _FLOATS:
+    """A contiguous float32 or bfloat16 tensor on a GPU."""
+    if isinstance(t, torch.Tensor) and t.dtype is not torch.float32 and t.dtype is not _BF16:
         raise TypeError(f"{name}: dtype {t.dtype}, expected float32 or bfloat16")
     return _chk(t, name, shape, t.dtype if isinstance(t, torch.Tensor) else None)
 
 
-def _chk_device(t, name, like, like_name):
-    if t.device != like.device:
-        raise ValueError(f"{name}: on {t.device}, {like_name} on {like.device}")
-    return t
+def _chk_at(t, name, shape, dtype, index):
+    """... of this type, on GPU `index`."""
+    _chk(t, name, shape, dtype)
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on {t.device}, expected cuda:{index}")
 
 
 def embedding_fwd(weight, ids, scale=1.0, out=None):
     """scale * weight[ids]: weight [V, D] float32 or bfloat16, ids int64 of any shape -> [*ids.shape, D] in weight's type.  An id
-    outside [0, V) (a padded position) gives a row of zeros."""
-    weight = _chk_float(weight, "weight")
+    outside [0, V) (a padded position) gives a row of zeros.  out: where it goes; it must not overlap weight."""
+    _chk_float(weight, "weight")
     if weight.dim() != 2:
         raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [V, D]")
-    ids = _chk_device(_chk(ids, "ids", None, torch.int64), "ids", weight, "weight")
-    shape = (*ids.shape, weight.shape[1])
+    index = weight.get_device()
+    _chk_at(ids, "ids", None, torch.int64, index)
+    V, D = weight.shape
     if out is None:
-        out = torch.empty(shape, device=weight.device, dtype=weight.dtype)
+        out = weight.new_empty((*ids.shape, D))
     else:
-        _chk_device(_chk(out, "out", shape, weight.dtype), "out", weight, "weight")
-    with _on(weight.device):
-        check(lib.dppm_embedding_fwd(weight.data_ptr(), weight.dtype == torch.bfloat16, ids.data_ptr(), scale, out.data_ptr(), ids.numel(),
-                                     weight.shape[0], weight.shape[1], _raw_stream(weight.device)), "dppm_embedding_fwd")
+        _chk_at(out, "out", (*ids.shape, D), weight.dtype, index)
+    _launch(index, lib.dppm_embedding_fwd, "dppm_embedding_fwd", weight.data_ptr(), weight.dtype is _BF16, ids.data_ptr(), scale,
+            out.data_ptr(), ids.numel(), V, D)
     return out
 
 
@@ -434,23 +434,23 @@ def embedding_wgrad(dout, ids, num_rows, scale=1.0, out=None, accumulate=False):
     """Gradient of embedding_fwd: dout [*ids.shape, D] -> [num_rows, D], scale times the sum of dout over the positions of each class,
     the same bits from call to call.  out: where it goes (float32 or bfloat16; default: dout's type); accumulate=True adds to it and
     leaves rows without a position as they are."""
-    dout = _chk_float(dout, "dout")
-    ids = _chk_device(_chk(ids, "ids", None, torch.int64), "ids", dout, "dout")
+    _chk_float(dout, "dout")
+    index = dout.get_device()
+    _chk_at(ids, "ids", None, torch.int64, index)
     if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:
         raise ValueError(f"dout: shape {tuple(dout.shape)}, expected [*{tuple(ids.shape)}, D]")
     T, V, D = ids.numel(), int(num_rows), dout.shape[-1]
     if out is None:
         if accumulate:
             raise ValueError("embedding_wgrad: accumulate needs an out")
-        out = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
+        out = dout.new_empty((max(V, 0), D))
     else:
-        _chk_device(_chk_float(out, "out", (V, D)), "out", dout, "dout")
+        _chk_float(out, "out", (V, D))
+        _chk_at(out, "out", None, out.dtype, index)
     nbytes = lib.dppm_embedding_wgrad_workspace_bytes(T, V, D)
-    with _on(dout.device):
-        ws = torch.empty(nbytes, device=dout.device, dtype=torch.uint8)
-        check(lib.dppm_embedding_wgrad(dout.data_ptr(), dout.dtype == torch.bfloat16, ids.data_ptr(), scale, out.data_ptr(),
-                                       out.dtype == torch.bfloat16, accumulate, T, V, D, ws.data_ptr(), nbytes, _raw_stream(dout.device)),
-              "dppm_embedding_wgrad")
+    ws = torch.empty(nbytes, device=dout.device, dtype=torch.uint8)
+    _launch(index, lib.dppm_embedding_wgrad, "dppm_embedding_wgrad", dout.data_ptr(), dout.dtype is _BF16, ids.data_ptr(), scale, out.data_ptr(),
+            out.dtype is _BF16, accumulate, T, V, D, ws.data_ptr(), nbytes)
     return out
 
 
@@ -459,32 +459,31 @@ def loss_ce(x, weight, target, row_weight=None, denom=None, want_grad=True):
     [0, V) means none: the row counts for nothing), row_weight None or [T] float32, denom a positive number (default: the number of rows
     that have a class).  Returns (loss float32 0-d, row_loss [T] float32, dx or None, dweight or None), gradients in x's type, of
     loss = sum(row_weight * row_loss) / denom (include/dppm_hip.h, dppm_loss_ce_fwd_bwd)."""
-    x = _chk_float(x, "x")
+    _chk_float(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x: shape {tuple(x.shape)}, expected [T, D]")
     T, D = x.shape
     if isinstance(weight, torch.Tensor) and (weight.dim() != 2 or weight.shape[1] != D):
         raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [V, {D}]")
-    _chk_device(_chk(weight, "weight", None, x.dtype), "weight", x, "x")
-    _chk_device(_chk(target, "target", (T,), torch.int64), "target", x, "x")
+    index = x.get_device()
+    _chk_at(weight, "weight", None, x.dtype, index)
+    _chk_at(target, "target", (T,), torch.int64, index)
     if row_weight is not None:
-        _chk_device(_chk(row_weight, "row_weight", (T,)), "row_weight", x, "x")
+        _chk_at(row_weight, "row_weight", (T,), torch.float32, index)
     if denom is not None and not 0 < float(denom) < float("inf"):
         raise ValueError(f"denom {denom}: expected a positive number or None")
-    V, bf16 = weight.shape[0], x.dtype == torch.bfloat16
+    V, bf16 = weight.shape[0], x.dtype is _BF16
     if T == 0:
         zero = torch.zeros((), device=x.device, dtype=torch.float32)
         return (zero, zero.new_zeros(0), torch.empty_like(x), torch.zeros_like(weight)) if want_grad else (zero, zero.new_zeros(0), None, None)
     nbytes = lib.dppm_loss_ce_workspace_bytes(T, V, D, bf16, want_grad)
-    with _on(x.device):
-        out = torch.empty(T + 1, device=x.device, dtype=torch.float32)
-        loss, row_loss = out[T], out[:T]
-        dx, dweight = (torch.empty_like(x), torch.empty_like(weight)) if want_grad else (None, None)
-        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-        check(lib.dppm_loss_ce_fwd_bwd(x.data_ptr(), weight.data_ptr(), bf16, target.data_ptr(), None if row_weight is None else row_weight.data_ptr(),
-                                       0.0 if denom is None else float(denom), T, V, D, loss.data_ptr(), row_loss.data_ptr(),
-                                       None if dx is None else dx.data_ptr(), None if dx is None else dweight.data_ptr(), ws.data_ptr(), nbytes,
-                                       _raw_stream(x.device)), "dppm_loss_ce_fwd_bwd")
+    out = torch.empty(T + 1, device=x.device, dtype=torch.float32)
+    loss, row_loss = out[T], out[:T]
+    dx, dweight = (torch.empty_like(x), torch.empty_like(weight)) if want_grad else (None, None)
+    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+    _launch(index, lib.dppm_loss_ce_fwd_bwd, "dppm_loss_ce_fwd_bwd", x.data_ptr(), weight.data_ptr(), bf16, target.data_ptr(),
+            None if row_weight is None else row_weight.data_ptr(), 0.0 if denom is None else float(denom), T, V, D, loss.data_ptr(),
+            row_loss.data_ptr(), None if dx is None else dx.data_ptr(), None if dx is None else dweight.data_ptr(), ws.data_ptr(), nbytes)
     return loss, row_loss, dx, dweight
 
 
@@ -618,12 +617,10 @@ def adamw_step(tensors, lr, beta1, beta2, eps, step, max_norm=None, grad_scale=1
     if max_norm is not None and not max_norm > 0:
         raise ValueError(f"max_norm {max_norm}: expected a positive number or None")
     s = tensors
-    with _on(s.device):
-        norm = torch.empty((), device=s.device, dtype=torch.float32) if max_norm is not None else None
-        check(lib.dppm_adamw_step(s.table.data_ptr(), s.chunks.data_ptr(), s.n_chunks, s.grad_bf16, s.state_bits, lr, beta1, beta2, eps,
-                                  int(step), grad_scale, 0.0 if norm is None else float(max_norm), int(seed) & (2 ** 64 - 1),
-                                  None if norm is None else norm.data_ptr(), s.workspace.data_ptr(), s.workspace.numel() * 8,
-                                  _raw_stream(s.device)), "dppm_adamw_step")
+    norm = torch.empty((), device=s.device, dtype=torch.float32) if max_norm is not None else None
+    _launch(s.device.index, lib.dppm_adamw_step, "dppm_adamw_step", s.table.data_ptr(), s.chunks.data_ptr(), s.n_chunks, s.grad_bf16, s.state_bits,
+            lr, beta1, beta2, eps, int(step), grad_scale, 0.0 if norm is None else float(max_norm), int(seed) & (2 ** 64 - 1),
+            None if norm is None else norm.data_ptr(), s.workspace.data_ptr(), s.workspace.numel() * 8)
     return norm
 
 
