@@ -325,7 +325,8 @@ extern "C" int dppm_adamw_step(const dppm_tensor_entry* table, const int32_t* ch
   if (clip) {
     double* part = reinterpret_cast<double*>(workspace);
     NormOut* out = reinterpret_cast<NormOut*>(part + NORM_GRID);
-    const int grid = n_chunks < NORM_GRID ? n_chunks : NORM_GRID;
+    // two chunks are read at a time: with few, two for each workgroup, so that the step can sum the parts itself
+    const int grid = n_chunks <= 2 * FEW_PARTS ? (n_chunks + 1) / 2 : n_chunks < NORM_GRID ? n_chunks : NORM_GRID;
     if (grid > 0) {
       if (grad_bf16) hipLaunchKernelGGL((grad_sq_kernel<true>), dim3(grid), dim3(256), 0, st, table, ch, n_chunks, part);
       else hipLaunchKernelGGL((grad_sq_kernel<false>), dim3(grid), dim3(256), 0, st, table, ch, n_chunks, part);
