@@ -251,7 +251,7 @@ struct TurnArgs {
   const void* e; long pitch;             // exponentials [rows][pitch]
   const float2* stats; const float* lse; const float* target_score; const int64_t* target; const float* row_weight; const float* inv;
   uint16_t* d; long plane;               // [planes][rows, whole tiles of 64][pitch]; e itself for bfloat16
-  int rows, V, strip;                    // strip: classes that share a maximum
+  int rows, V, strip, across;            // strip: classes that share a maximum; across: workgroups for the classes
   bool past;                             // d is larger than the caches
 };
 
@@ -259,15 +259,15 @@ struct TurnArgs {
 // score.  Rows behind the last (to whole tiles of 64) and without a class are zeros; so are classes behind the last, to the pitch.
 template <bool F32>
 __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
-  if (blockIdx.y == gridDim.y - 1) {      // one more row of workgroups: its first sums the loss, with the last block of rows
-    if (blockIdx.x == 0 && l.loss) sum_loss<256>(l, a.inv);
+  if (blockIdx.x == gridDim.x - 1) {      // one more workgroup, which sums the loss, with the last block of rows
+    if (l.loss) sum_loss<256>(l, a.inv);
     return;
   }
   constexpr int P = F32 ? 3 : 1, ROWS = 16;
   __shared__ float factor[16][ROWS];     // of each 32 classes: strips of 32 are the shortest
   __shared__ float own[ROWS];
   __shared__ int at[ROWS];
-  const int v0 = blockIdx.x * 512, t0 = blockIdx.y * ROWS;
+  const int v0 = blockIdx.x % a.across * 512, t0 = blockIdx.x / a.across * ROWS;
   {
     const int r = threadIdx.x & 15, k = threadIdx.x >> 4, t = t0 + r, v = v0 + 32 * k;
     float f = 0.f, mine = 0.f;
@@ -694,7 +694,8 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     const bool last = b == p.blocks - 1;
     LossArgs sum = loss;
     if (!last) sum.loss = nullptr;
-    const dim3 grid((unsigned)cdiv(p.Vp, 512), (unsigned)(whole / 16 + 1));
+    a.across = cdiv(p.Vp, 512);
+    const dim3 grid((unsigned)((long)a.across * (whole / 16) + 1));      // (a second dimension of a grid ends at 65535)
     if (p.f32) hipLaunchKernelGGL((turn_kernel<true>), grid, dim3(256), 0, st, a, sum);
     else hipLaunchKernelGGL((turn_kernel<false>), grid, dim3(256), 0, st, a, sum);
     if (p.blocks > 1) {

@@ -468,7 +468,7 @@ using namespace dppm;
 
 #define DPPM_REQUIRE_TABLE(what)                                                                                                       \
   DPPM_REQUIRE(T >= 0 && V >= 1 && D >= 1, what ": T=%ld V=%ld D=%ld", (long)T, (long)V, (long)D);                                     \
-  DPPM_REQUIRE(T < (1L << 31) && V < (1L << 31) && D < (1L << 24), what ": T=%ld V=%ld D=%ld are too large", (long)T, (long)V, (long)D)
+  DPPM_REQUIRE(T < (1L << 31) && V < (1L << 31) && D <= (1L << 21), what ": T=%ld V=%ld D=%ld are too large", (long)T, (long)V, (long)D)
 
 extern "C" int dppm_embedding_fwd(const void* weight, int bf16, const int64_t* ids, float scale, void* out, int64_t T, int64_t V, int64_t D,
                                   void* stream) {
@@ -494,7 +494,7 @@ extern "C" int dppm_embedding_fwd(const void* weight, int bf16, const int64_t* i
 }
 
 extern "C" size_t dppm_embedding_wgrad_workspace_bytes(int64_t T, int64_t V, int64_t D) {
-  if (T < 1 || V < 1 || D < 1 || T >= (1L << 31) || V >= (1L << 31) || D >= (1L << 24)) return 0;
+  if (T < 1 || V < 1 || D < 1 || T >= (1L << 31) || V >= (1L << 31) || D > (1L << 21)) return 0;
   return layout_of(T, V, D).total;
 }
 

@@ -412,9 +412,16 @@ def _chk_at(t, name, shape, dtype, index):
         raise ValueError(f"{name}: on {t.device}, expected cuda:{index}")
 
 
+def _refuse_overlap(out, t, name):
+    """Workgroups read t while others write out."""
+    a, b = out.data_ptr(), t.data_ptr()
+    if a < b + t.numel() * t.element_size() and b < a + out.numel() * out.element_size():
+        raise ValueError(f"out: shares memory with {name}")
+
+
 def embedding_fwd(weight, ids, scale=1.0, out=None):
     """scale * weight[ids]: weight [V, D] float32 or bfloat16, ids int64 of any shape -> [*ids.shape, D] in weight's type.  An id
-    outside [0, V) (a padded position) gives a row of zeros.  out: where it goes; it must not overlap weight."""
+    outside [0, V) (a padded position) gives a row of zeros.  out: where it goes."""
     _chk_float(weight, "weight")
     if weight.dim() != 2:
         raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [V, D]")
@@ -425,6 +432,8 @@ def embedding_fwd(weight, ids, scale=1.0, out=None):
         out = weight.new_empty((*ids.shape, D))
     else:
         _chk_at(out, "out", (*ids.shape, D), weight.dtype, index)
+        _refuse_overlap(out, weight, "weight")
+        _refuse_overlap(out, ids, "ids")
     _launch(index, lib.dppm_embedding_fwd, "dppm_embedding_fwd", weight.data_ptr(), weight.dtype is _BF16, ids.data_ptr(), scale,
             out.data_ptr(), ids.numel(), V, D)
     return out
@@ -447,6 +456,8 @@ def embedding_wgrad(dout, ids, num_rows, scale=1.0, out=None, accumulate=False):
     else:
         _chk_float(out, "out", (V, D))
         _chk_at(out, "out", None, out.dtype, index)
+        _refuse_overlap(out, dout, "dout")
+        _refuse_overlap(out, ids, "ids")
     nbytes = lib.dppm_embedding_wgrad_workspace_bytes(T, V, D)
     ws = torch.empty(nbytes, device=dout.device, dtype=torch.uint8)
     _launch(index, lib.dppm_embedding_wgrad, "dppm_embedding_wgrad", dout.data_ptr(), dout.dtype is _BF16, ids.data_ptr(), scale, out.data_ptr(),

@@ -270,14 +270,15 @@ int dppm_adam_step(float* param, const float* grad, float* exp_avg, float* exp_a
  * ---------------------------------------------------------------------------------------------- */
 
 /* out[t][:] = scale * weight[ids[t]][:] for t in [0, T): weight [V][D] and out [T][D] float32, or bfloat16 with bf16 != 0 (product in
- * float32, rounded once).  An id outside [0, V) stands for no class: its row of out is zero.  out must not overlap weight. */
+ * float32, rounded once).  An id outside [0, V) stands for no class: its row of out is zero.  out must not overlap weight.
+ * T, V < 2^31, D <= 2^21. */
 int dppm_embedding_fwd(const void* weight, int bf16, const int64_t* ids, float scale, void* out, int64_t T, int64_t V, int64_t D,
                        void* stream);
 
 /* Its gradient: dweight[v][:] = scale * sum over t with ids[t] = v of dout[t][:], every row written (zero without a position); with
  * accumulate != 0 it is added to dweight and rows without a position stay as they are.  dout [T][D], dweight [V][D], each float32 or
  * bfloat16; sums in float32, in the order of t within chunks of the sorted positions: the same bits from call to call.
- * T, V < 2^31.  workspace: dppm_embedding_wgrad_workspace_bytes(T, V, D), 16-byte aligned (0 bytes: invalid sizes). */
+ * T, V < 2^31, D <= 2^21.  workspace: dppm_embedding_wgrad_workspace_bytes(T, V, D), 16-byte aligned (0 bytes: invalid sizes). */
 size_t dppm_embedding_wgrad_workspace_bytes(int64_t T, int64_t V, int64_t D);
 int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64_t* ids, float scale, void* dweight, int dweight_bf16, int accumulate,
                          int64_t T, int64_t V, int64_t D, void* workspace, size_t workspace_bytes, void* stream);

@@ -162,6 +162,7 @@ def test_refusals(ops):
                  (lambda: ops.embedding_fwd(w.t(), ids), ValueError), (lambda: ops.embedding_fwd(w[0], ids), ValueError),
                  (lambda: ops.embedding_fwd(w, ids, out=torch.zeros(6, 5, device="cuda")), ValueError), (lambda: ops.embedding_fwd(w, ids.cpu()), RuntimeError),
                  (lambda: ops.embedding_fwd(w, ids, out=d.bfloat16()), TypeError), (lambda: ops.embedding_fwd(w[:0], ids), RuntimeError),
+                 (lambda: ops.embedding_fwd(w, ids[:5], out=w), ValueError), (lambda: ops.embedding_wgrad(d, ids, 6, out=d), ValueError),
                  (lambda: ops.embedding_wgrad(d[:5], ids, 5), ValueError), (lambda: ops.embedding_wgrad(d, ids, 5, accumulate=True), ValueError),
                  (lambda: ops.embedding_wgrad(d, ids, 0), RuntimeError), (lambda: ops.embedding_wgrad(d, ids, 5, out=torch.zeros(4, 4, device="cuda")), ValueError),
                  (lambda: ops.embedding_wgrad(d.t(), ids, 5), ValueError), (lambda: ops.embedding_wgrad(d.double(), ids, 5), TypeError)):

@@ -90,6 +90,44 @@ def test_tiles_of_256(ops, T, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+def test_very_many_rows_of_few_classes(ops, dtype):
+    """more than 65535 workgroups of 16 rows"""
+    x, w, y, rw = make(1_100_003, 3, 8, dtype, 9)
+    check(ops, x, w, y, rw)
+
+
+@pytest.mark.parametrize("dtype,T,V", [(F32, 2500, 60000), (BF16, 9000, 131100)])
+def test_several_blocks_of_rows(ops, dtype, T, V):
+    """T V over 2^27 (float32) or 2^30 (bfloat16): the rows go in blocks whose parts of dweight add up in float32 (one more u a block, within
+    the T-term sum's allowance); compared on the device against float64 there, with the tolerances of `bounds` for its largest entries"""
+    x, w, y, rw = (t.cuda() for t in make(T, V, 64, dtype, 10))
+    loss, row_loss, dx, dw = ops.loss_ce(x, w, y, rw)
+    h = H if dtype == BF16 else 0.0
+    ok = y >= 0
+    share = (torch.where(ok, rw, torch.zeros(()).cuda()).double() / ok.sum()).unsqueeze(1)
+    xd, wd = x.double(), w.double()
+    want_dw, mag_dw = torch.zeros_like(wd), torch.zeros_like(wd)
+    for rows in torch.arange(T, device="cuda").split(1500):
+        s = xd[rows] @ wd.t()
+        mag = (xd[rows].abs() @ wd.abs().t()).amax(1, keepdim=True)
+        lse = torch.logsumexp(s, 1, keepdim=True)
+        at = y[rows].clamp(min=0).unsqueeze(1)
+        e = 2 * (64 + 16) * U * mag + 64 * U + 4 * mag * U
+        off = (row_loss[rows].double() - torch.where(ok[rows], (lse - s.gather(1, at)).squeeze(1), torch.zeros(()).cuda().double())).abs()
+        assert (off <= (2 * e + 8 * U * (mag + np.log(V) + 1)).squeeze(1)).all()
+        p = (s - lse).exp()
+        d = p.clone().scatter_add_(1, at, torch.full_like(lse, -1.0)) * share[rows]
+        dd = (2 * h + 16 * U) * d.abs() + e * p * share[rows] * (1 + 2 * h) + 1e-37
+        tol = dd @ wd.abs() + (V + 64) * U * (d.abs() @ wd.abs())
+        want = d @ wd
+        last = h if h else 4 * U
+        assert ((dx[rows].double() - want).abs() <= tol * (1 + last) + last * want.abs() + 1e-37).all()
+        want_dw += d.t() @ xd[rows]
+        mag_dw += dd.t() @ xd[rows].abs() + (T + 64) * U * (d.abs().t() @ xd[rows].abs())
+    assert ((dw.double() - want_dw).abs() <= mag_dw * (1 + last) + last * want_dw.abs() + 1e-37).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_certain_and_hopeless_rows(ops, dtype):
     x, w, y, rw = make(200, 300, 64, dtype, 2, missing=0.0)
     x = (x.float() * 30).to(dtype)                       # scores of +-100: most probabilities are 0 or 1
