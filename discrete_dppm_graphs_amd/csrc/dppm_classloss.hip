@@ -8,7 +8,9 @@
 //
 // Three matrix products, each 2 T V D operations, and the exponentials between them:
 //  * scores: tiles of s on the matrix cores; from the accumulators each strip of classes gives its maximum and its sum of exponentials per
-//    row, and (with gradients) the exponentials relative to the strip's maximum, bfloat16 for bfloat16 inputs and float32 for float32;
+//    row, and (with gradients) the exponentials relative to the strip's maximum, in half precision for bfloat16 inputs -- they lie in [0, 1], where
+//    its 11 bits keep 2^-11 of each down to 2^-14 of the maximum and 2^-25 of the maximum below, so that the only rounding of d that counts
+//    is its own -- and in float32 for float32;
 //  * rows: lse, the rows' losses;
 //  * turn: exponentials to d, rounded once to the operands' type;
 //  * dx = d W and dW = d^T x: W and d are read transposed from LDS where the contracted dimension is not the contiguous one; x, the smallest,
@@ -29,6 +31,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {   // round t
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
 }
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {   // round to nearest even
+  typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, halfx2{(_Float16)lo, (_Float16)hi});
+}
+__device__ __forceinline__ float half_lo(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)w); }
+__device__ __forceinline__ float half_hi(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)); }
 __device__ __forceinline__ uint16_t to_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 __device__ __forceinline__ float from_bf16(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 
@@ -178,7 +186,7 @@ __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
             store_out(f32x4{v[0], v[1], v[2], v[3]}, p, o.past);
             store_out(f32x4{v[4], v[5], v[6], v[7]}, p + 1, o.past);
           } else
-            store_out(u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])},
+            store_out(u32x4{pack_half(v[0], v[1]), pack_half(v[2], v[3]), pack_half(v[4], v[5]), pack_half(v[6], v[7])},
                       reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(o.e) + at), o.past);
         }
       });
@@ -250,20 +258,21 @@ __global__ __launch_bounds__(1024) void rows_and_loss_kernel(const float2* __res
 struct TurnArgs {
   const void* e; long pitch;             // exponentials [rows][pitch]
   const float2* stats; const float* lse; const float* target_score; const int64_t* target; const float* row_weight; const float* inv;
-  uint16_t* d; long plane;               // [planes][rows, whole tiles of 64][pitch]; e itself for bfloat16
+  uint16_t* d; long plane;               // [planes][rows, whole tiles of 64][pitch]; in e's place for bfloat16
   int rows, V, strip, across;            // strip: classes that share a maximum; across: workgroups for the classes
   bool past;                             // d is larger than the caches
 };
 
 // 16 rows x 512 classes a workgroup, 8 classes a thread and row: d_tv = e_tv * exp(max_strip - lse_t) * w_t / n, the row's own class from its float32
 // score.  Rows behind the last (to whole tiles of 64) and without a class are zeros; so are classes behind the last, to the pitch.
-template <bool F32>
+// P planes of d: 3 for float32; 1 for bfloat16, or 2 for few rows (plan_of).
+template <bool F32, int P>
 __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
   if (blockIdx.x == gridDim.x - 1) {      // one more workgroup, which sums the loss, with the last block of rows
     if (l.loss) sum_loss<256>(l, a.inv);
     return;
   }
-  constexpr int P = F32 ? 3 : 1, ROWS = 16;
+  constexpr int ROWS = 16;
   __shared__ float factor[16][ROWS];     // of each 32 classes: strips of 32 are the shortest
   __shared__ float own[ROWS];
   __shared__ int at[ROWS];
@@ -301,7 +310,7 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
       } else {
         const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.e) + to);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { x[2 * k] = __uint_as_float(w[k] << 16); x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u); }
+        for (int k = 0; k < 4; ++k) { x[2 * k] = half_lo(w[k]); x[2 * k + 1] = half_hi(w[k]); }
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[k] *= f;
@@ -312,7 +321,7 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
       for (int k = 0; k < 8; ++k)
         if (y == k) x[k] = own[r];
     }
-    if (F32) {
+    if (P > 1) {
       uint16_t s[8][3];
 #pragma unroll
       for (int k = 0; k < 8; ++k) split3(x[k], s[k]);
@@ -501,6 +510,7 @@ struct Plan {
   bool f32, grad, direct;        // direct: x and W are used where they are
   long T, V, D, Kp, Vp, R, Rp;   // pitches for D and V values; rows of a block, pitch for them
   int blocks, planes, pairs, tile_scores, strips, strip;
+  int d_planes, d_pairs;         // of d, and products of pairs of planes in the gradients
   size_t inv, stats, lse, tscore, xp, wp, xt, e, d, dw, part, total, part_bytes;
 };
 
@@ -532,6 +542,12 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
   p.f32 = f32; p.grad = grad; p.T = T; p.V = V; p.D = D;
   p.planes = f32 ? 3 : 1;
   p.pairs = f32 ? 6 : 1;
+  // d of bfloat16 inputs: one bfloat16 plane, whose rounding adds to the gradients' error about as much as their own does, or two for few rows,
+  // over which one large entry's rounding does not average out (8 rows, 25840 classes: off by 0.0029 instead of 0.0016 of the gradient; 47 and
+  // 58 us with one plane and with two; 1024 rows, 1024 x 1024: 74 and 80 us, and no more than 1.4 times the plain rounding either way).
+  const bool exact_d = !f32 && T <= 64;
+  p.d_planes = f32 ? 3 : exact_d ? 2 : 1;
+  p.d_pairs = f32 ? 6 : p.d_planes;
   p.direct = direct && !f32 && D % 64 == 0;
   p.Kp = p.direct ? D : pitch_of(D);
   p.Vp = pitch_of(V);
@@ -562,9 +578,9 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
     p.xt = take((size_t)p.planes * D * p.Rp * 2);
     const size_t held = (size_t)((p.R + 63) / 64 * 64) * p.Vp;
     p.e = take(held * (f32 ? 4 : 2));
-    p.d = f32 ? take(3 * held * 2) : p.e;
+    p.d = p.d_planes > 1 ? take(p.d_planes * held * 2) : p.e;
     if (p.blocks > 1 && !f32) p.dw = take((size_t)V * D * 4);
-    const int s1 = shape_of(D, p.R, (long)cdiv(V, 64) * p.pairs, true).splits, s2 = shape_of(D, V, (long)cdiv(p.R, 64) * p.pairs, true).splits;
+    const int s1 = shape_of(D, p.R, (long)cdiv(V, 64) * p.d_pairs, true).splits, s2 = shape_of(D, V, (long)cdiv(p.R, 64) * p.d_pairs, true).splits;
     const size_t b1 = s1 > 1 ? (size_t)s1 * D * p.R * 4 : 0, b2 = s2 > 1 ? (size_t)s2 * D * V * 4 : 0;
     p.part_bytes = b1 > b2 ? b1 : b2;
     p.part = take(p.part_bytes);
@@ -690,14 +706,15 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     TurnArgs a{};
     a.e = ws + p.e; a.pitch = p.Vp; a.stats = stats; a.lse = f(p.lse); a.target_score = f(p.tscore); a.target = target + t0;
     a.row_weight = row_weight ? row_weight + t0 : nullptr; a.inv = f(p.inv);
-    a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip; a.past = (size_t)p.planes * a.plane * 2 > CACHED;
+    a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip; a.past = (size_t)p.d_planes * a.plane * 2 > CACHED;
     const bool last = b == p.blocks - 1;
     LossArgs sum = loss;
     if (!last) sum.loss = nullptr;
     a.across = cdiv(p.Vp, 512);
     const dim3 grid((unsigned)((long)a.across * (whole / 16) + 1));      // (a second dimension of a grid ends at 65535)
-    if (p.f32) hipLaunchKernelGGL((turn_kernel<true>), grid, dim3(256), 0, st, a, sum);
-    else hipLaunchKernelGGL((turn_kernel<false>), grid, dim3(256), 0, st, a, sum);
+    if (p.f32) hipLaunchKernelGGL((turn_kernel<true, 3>), grid, dim3(256), 0, st, a, sum);
+    else if (p.d_planes == 2) hipLaunchKernelGGL((turn_kernel<false, 2>), grid, dim3(256), 0, st, a, sum);
+    else hipLaunchKernelGGL((turn_kernel<false, 1>), grid, dim3(256), 0, st, a, sum);
     if (p.blocks > 1) {
       LayOut xs{};
       const int n = lay_out(xs, p.f32, reinterpret_cast<const char*>(x) + t0 * D * es, rows, D, nullptr, 0, h(p.xt), Rp, target + t0, V);
@@ -706,12 +723,12 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     TnArgs gx{};       // dx[t][d] = sum_v d[t][v] W[v][d]
     gx.A = wp; gx.lda = p.Kp; gx.plane_a = V * p.Kp; gx.M = (int)D;
     gx.B = a.d; gx.ldb = p.Vp; gx.plane_b = a.plane; gx.N = (int)rows;
-    gx.K = (int)V; gx.ksteps = cdiv(V, 64); gx.pairs = p.pairs;
+    gx.K = (int)V; gx.ksteps = cdiv(V, 64); gx.pairs = p.d_pairs;
     DPPM_TRY((grad_product<true, false>(gx, reinterpret_cast<char*>(dx) + t0 * D * es, bf16, nullptr, f(p.part), p.part_bytes, st)));
     TnArgs gw{};       // dW[v][d] = sum_t d[t][v] x^T[d][t]
     gw.A = h(p.xt); gw.lda = Rp; gw.plane_a = D * Rp; gw.M = (int)D;
     gw.B = a.d; gw.ldb = p.Vp; gw.plane_b = a.plane; gw.N = (int)V;
-    gw.K = whole; gw.ksteps = cdiv(rows, 64); gw.pairs = p.pairs;      // d has zeros to whole steps
+    gw.K = whole; gw.ksteps = cdiv(rows, 64); gw.pairs = p.d_pairs;      // d has zeros to whole steps
     float* total = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
     DPPM_TRY((grad_product<false, true>)(gw, last || p.f32 ? dweight : (void*)total, bf16 && last, b == 0 ? nullptr : total, f(p.part), p.part_bytes, st));
   }

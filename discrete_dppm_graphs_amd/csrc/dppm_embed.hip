@@ -170,6 +170,8 @@ __device__ __forceinline__ void place(RankShared<NT, BITS>& s, const int64_t* id
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < PER; ++r) {
+    rank[r] = 0;
+    if (at0 - lane + r * 64 >= n) continue;      // the whole wave is behind the end
     const bool in = at0 + r * 64 < n;
     const uint32_t d = (key[r] >> shift) & low;
     uint64_t same = __ballot(in);
@@ -291,6 +293,17 @@ __device__ __forceinline__ void finish_row(const SumArgs& a, uint32_t k, int c, 
   store_vec<OBF, VEC>(a.dw, at, acc);
 }
 
+// `bytes` zeros from p (2-byte aligned) by `lanes` (8 or 64) lanes: 16 at a time between the aligned ends
+__device__ __forceinline__ void zero_bytes(char* p, long bytes, int lane, int lanes) {
+  long head = (16 - ((uintptr_t)p & 15)) & 15;
+  if (head > bytes) head = bytes;
+  if (lane * 2 < head) *(glb<uint16_t>)(p + lane * 2) = 0;
+  const long wide = (bytes - head) / 16;
+  for (long i = lane; i < wide; i += lanes) *(glb<u32x4>)(p + head + i * 16) = u32x4{0, 0, 0, 0};
+  const long done = head + wide * 16;
+  if (done + lane * 2 < bytes) *(glb<uint16_t>)(p + done + lane * 2) = 0;
+}
+
 // One group of `lanes` lanes sums the rows of `cp` consecutive sorted positions over lanes * VEC columns.  Workgroups behind those
 // write zeros to the rows that have no position (found by bisection: the sorted classes are in L2).
 constexpr int FILL_ROWS = 64;
@@ -310,13 +323,10 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a, int sum_block
       absent[threadIdx.x] = row < a.V && !(lo < a.T && (long)a.key[lo] == row);
     }
     __syncthreads();
-    float zero[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) zero[i] = 0.f;
-    const int lane = threadIdx.x & 63;
-    for (int r = threadIdx.x >> 6; r < FILL_ROWS; r += 4)
-      if (absent[r])
-        for (int c = lane * VEC; c < a.D; c += 64 * VEC) store_vec<OBF, VEC>(a.dw, (r0 + r) * a.D + c, zero);
+    constexpr int ES = OBF ? 2 : 4;
+    const int zl = a.D * ES <= 256 ? 8 : 64;      // short rows: eight lanes each
+    for (int r = threadIdx.x / zl; r < FILL_ROWS; r += 256 / zl)
+      if (absent[r]) zero_bytes(reinterpret_cast<char*>(a.dw) + (r0 + r) * a.D * ES, (long)a.D * ES, threadIdx.x & (zl - 1), zl);
     return;
   }
   const int lanes = 1 << a.lanes_log2;

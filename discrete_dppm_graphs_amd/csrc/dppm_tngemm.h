@@ -29,7 +29,7 @@ struct TnArgs {
   long lda, ldb;          // elements between rows (of m or n, or of k); multiples of 8, as the planes' distance
   long plane_a, plane_b;  // elements between planes
   int M, N, K, ksteps;       // ksteps = k / 64: operands contiguous in k are padded with zeros to whole steps
-  int pairs;              // 1, or 6 for float32 operands in three planes
+  int pairs;              // 1; 6 for float32 operands in three planes; 2 for one plane of A with two of B
   int splits;             // parts that the steps of k are dealt to
   int tiles_m, tiles_n;
 };

@@ -4,8 +4,8 @@ Tolerances, with u = 2^-24 and h = 2^-8 for bfloat16 inputs (half a step), 0 for
   a score is a sum of D products; each float32 product is three-piece split work, under 2^-21 of it: |ds| <= (D + 16) u sum_k |x_k w_k|;
   an exponential of it: relative error |ds| + (8 + |s|) u at both ends of the subtraction, so e_t = 2 max_v |ds| + 64 u + 4 max |s| u for a row;
   row_loss: 2 e_t + 4 u |lse| + 4 u |s|;
-  a gradient of the scores: the stored exponential and d are each rounded once to the operands' type: |dd| <= (2 h + 8 u) |d| + e_t p g,
-  for float32 three pieces keep 2^-23: 16 u |d|;
+  a gradient of the scores: for bfloat16 the stored exponential is rounded to half precision (2^-11 of it, or 2^-25 of the strip's largest where
+  it is subnormal) and d to bfloat16 (h): |dd| <= (2^-11 + h + 16 u) |d| (1 + h) + 2^-25 max p g + e_t p g; for float32 three pieces keep 2^-23: 16 u |d|;
   dx: sum_v |dd| |W| + V-term sum in float32 + splits (V + 64) u sum |d| |W|, then its rounding (h or u); dW likewise over the rows."""
 import numpy as np
 import pytest
@@ -45,7 +45,7 @@ def bounds(x, w, y, rw, denom, want):
     e = 2 * s_err + 64 * U + 4 * mag * U
     row_tol = torch.where(ok, (2 * e + 8 * U * (mag + np.log(V) + 1)).squeeze(1), torch.zeros(()).double())
     loss_tol = (row_tol * g.squeeze(1)).sum() + 8 * U * (row_loss * g.squeeze(1)).sum()
-    dd = (2 * h + 16 * U) * d.abs() + e * p * g * (1 + 2 * h) + 1e-37
+    dd = ((2.0 ** -11 + h if h else 0) + 16 * U) * d.abs() * (1 + h) + (2.0 ** -25 * (1 + h) * p.amax(1, keepdim=True) * g if h else 0) + e * p * g * (1 + 2 * h) + 1e-37
     dx_tol = dd @ wd + (V + 64) * U * (d.abs() @ wd)
     dw_tol = dd.t() @ xd + (T + 64) * U * (d.abs().t() @ xd)
     last = h if h else 4 * U
@@ -117,7 +117,9 @@ def test_several_blocks_of_rows(ops, dtype, T, V):
         assert (off <= (2 * e + 8 * U * (mag + np.log(V) + 1)).squeeze(1)).all()
         p = (s - lse).exp()
         d = p.clone().scatter_add_(1, at, torch.full_like(lse, -1.0)) * share[rows]
-        dd = (2 * h + 16 * U) * d.abs() + e * p * share[rows] * (1 + 2 * h) + 1e-37
+        dd = ((2.0 ** -11 + h if h else 0) + 16 * U) * d.abs() * (1 + h) + e * p * share[rows] * (1 + 2 * h) + 1e-37
+        if h:
+            dd = dd + 2.0 ** -25 * (1 + h) * p.amax(1, keepdim=True) * share[rows]
         tol = dd @ wd.abs() + (V + 64) * U * (d.abs() @ wd.abs())
         want = d @ wd
         last = h if h else 4 * U
