@@ -176,20 +176,22 @@ __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
   }
   if (o.e) {
 #pragma unroll
-    for (int j = 0; j < T::WN / 32; ++j)
-      tn_rows<T>(lds, acc, j, [&](int row, int m, const float (&v)[8]) {
-        const int n = ns + j * 32 + row, c = ms + m;
-        if (n < g.N && c < o.pitch) {
-          const long at = (long)n * o.pitch + c;
-          if (F32) {
-            f32x4* p = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(o.e) + at);
+    for (int j = 0; j < T::WN / 32; ++j) {
+      if constexpr (F32)
+        tn_rows<T>(lds, acc, j, [&](int row, int m, const float (&v)[8]) {
+          const int n = ns + j * 32 + row, c = ms + m;
+          if (n < g.N && c < o.pitch) {
+            f32x4* p = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(o.e) + (long)n * o.pitch + c);
             store_out(f32x4{v[0], v[1], v[2], v[3]}, p, o.past);
             store_out(f32x4{v[4], v[5], v[6], v[7]}, p + 1, o.past);
-          } else
-            store_out(u32x4{pack_half(v[0], v[1]), pack_half(v[2], v[3]), pack_half(v[4], v[5]), pack_half(v[6], v[7])},
-                      reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(o.e) + at), o.past);
-        }
-      });
+          }
+        });
+      else
+        tn_rows16<T>(lds, acc, j, pack_half, [&](int row, int m, u32x4 w) {
+          const int n = ns + j * 32 + row, c = ms + m;
+          if (n < g.N && c < o.pitch) store_out(w, reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(o.e) + (long)n * o.pitch + c), o.past);
+        });
+    }
   }
 }
 
@@ -464,6 +466,15 @@ __global__ __launch_bounds__(T::NT) void grad_kernel(TnArgs g, GradOut o) {
   tn_product<T, TRA, TRB>(g, lds, m0, n0, (int)(steps * split / g.splits), (int)(steps * (split + 1) / g.splits), acc);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;
+  if (o.c_bf16 && o.wide && !o.part && !o.add) {
+#pragma unroll
+    for (int j = 0; j < T::WN / 32; ++j)
+      tn_rows16<T>(lds, acc, j, pack_bf16, [&](int row, int m, u32x4 w) {
+        const int n = ns + j * 32 + row;
+        if (n < g.N && ms + m < g.M) store_out(w, reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(o.c) + (long)n * o.ldc + ms + m), o.past);
+      });
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < T::WN / 32; ++j)
     tn_rows<T>(lds, acc, j, [&](int row, int m, const float (&v)[8]) {
@@ -650,7 +661,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
                                     int64_t V, int64_t D, float* loss_out, float* row_loss, void* dx, void* dweight, void* workspace,
                                     size_t workspace_bytes, void* stream) {
   DPPM_REQUIRE(sizes_ok(T, V, D), "dppm_loss_ce_fwd_bwd: T=%ld V=%ld D=%ld", (long)T, (long)V, (long)D);
-  DPPM_REQUIRE(denom >= 0, "dppm_loss_ce_fwd_bwd: denom=%g", denom);
+  DPPM_REQUIRE(denom == 0 || (denom >= 1e-37 && denom <= 1e37), "dppm_loss_ce_fwd_bwd: denom=%g", denom);
   DPPM_REQUIRE(T >= 1, "dppm_loss_ce_fwd_bwd: no rows");
   DPPM_REQUIRE(x && weight && target && loss_out && row_loss && workspace, "dppm_loss_ce_fwd_bwd: null pointer");
   DPPM_REQUIRE((dx == nullptr) == (dweight == nullptr), "dppm_loss_ce_fwd_bwd: dx and dweight come together");

@@ -272,4 +272,31 @@ __device__ __forceinline__ void tn_rows(char* lds, const tn_acc (&acc)[T::MI][T:
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
+// The same with the values packed to 16 bits on the way in, which halves the LDS traffic
+// (4099 x 1000 bfloat16, 50001 classes: 1.49 -> 1.47 ms): pack(lo, hi) makes a word of two,
+// emit(row, m, word[4]) gets eight values.
+template <class T, class Pack, class Emit>
+__device__ __forceinline__ void tn_rows16(char* lds, const tn_acc (&acc)[T::MI][T::NI], int block, Pack pack, Emit emit) {
+  typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+  constexpr int PITCH = T::WM * 2 + 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char* img = lds + wave * 32 * PITCH;
+#pragma unroll
+  for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j)
+      if (j / 2 == block)
+        *reinterpret_cast<u32x2v*>(img + ((j & 1) * 16 + (lane & 15)) * PITCH + (16 * i + 4 * (lane >> 4)) * 2) =
+            u32x2v{pack(acc[i][j][0], acc[i][j][1]), pack(acc[i][j][2], acc[i][j][3])};
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  constexpr int PER_ROW = T::WM / 8, ROWS = 64 / PER_ROW;
+#pragma unroll
+  for (int r = 0; r < 32; r += ROWS) {
+    const int row = r + lane / PER_ROW, m = (lane % PER_ROW) * 8;
+    emit(row, m, *reinterpret_cast<const u32x4v*>(img + row * PITCH + m * 2));
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 }  // namespace dppm

@@ -94,7 +94,7 @@ def test_loss_ce_entry_refuses():
     one = C.c_void_p(16)
     good = dict(x=one, w=one, bf=1, target=one, rw=None, denom=0.0, T=4, V=5, D=8, loss=one, row=one, dx=one, dw=one, ws=one, n=1 << 40, st=None)
     for bad in ({"x": None}, {"w": None}, {"target": None}, {"loss": None}, {"row": None}, {"ws": None}, {"dx": None}, {"dw": None}, {"T": 0}, {"T": -1},
-                {"T": 1 << 30}, {"V": 0}, {"V": (1 << 23) + 1}, {"D": 0}, {"D": (1 << 16) + 1}, {"denom": -1.0}, {"denom": float("nan")}, {"ws": C.c_void_p(8)}):
+                {"T": 1 << 30}, {"V": 0}, {"V": (1 << 23) + 1}, {"D": 0}, {"D": (1 << 16) + 1}, {"denom": -1.0}, {"denom": float("nan")}, {"denom": 1e-50}, {"denom": float("inf")}, {"ws": C.c_void_p(8)}):
         assert lib.dppm_loss_ce_fwd_bwd(*{**good, **bad}.values()) == -1, bad
     need = lib.dppm_loss_ce_workspace_bytes(4, 5, 8, 1, 1)
     assert need > lib.dppm_loss_ce_workspace_bytes(4, 5, 8, 1, 0) > 0
