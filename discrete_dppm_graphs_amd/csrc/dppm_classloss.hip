@@ -66,49 +66,53 @@ __device__ __forceinline__ void store_out(V v, V* p, bool past) {
 constexpr size_t CACHED = 256u << 20;
 
 // ------------------------------------------------------------------------------------------------ counting rows, losses
-// 1 / denom, or 1 / (rows with a class) where none is given; all NT threads get it
+// Of up to COUNTED rows, or of a workgroup of rows_kernel; one workgroup puts them together in a fixed order.  (One workgroup over all rows took
+// 0.28 ms to count a million and 1.3 ms to sum their losses.)
+struct RowsPart { double loss; uint32_t rows, pad; };
+constexpr long COUNTED = 4096;
+
+// 1 / denom, or 1 / (the sum of counts) where none is given; all NT threads get it
 template <int NT>
-__device__ __forceinline__ float inverse_of_rows(const int64_t* target, long T, long V, float denom) {
+__device__ __forceinline__ float inverse_of(const uint32_t* counts, int n, float denom) {
   __shared__ uint32_t w[NT / 64];
-  uint32_t n = 0;
+  uint32_t sum = 0;
   if (!(denom > 0.f)) {
 #pragma unroll 8
-    for (long t = threadIdx.x; t < T; t += NT) n += target[t] >= 0 && target[t] < V;
+    for (int i = threadIdx.x; i < n; i += NT) sum += counts[i];
   }
 #pragma unroll
-  for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
-  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = n;
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
   __syncthreads();
   uint32_t all = 0;
   for (int i = 0; i < NT / 64; ++i) all += w[i];
   return 1.f / (denom > 0.f ? denom : (float)(all ? all : 1u));
 }
 
-struct LossArgs { const float *row_loss, *row_weight; const int64_t* target; long T, V; float denom; float* loss; };   // loss null: nothing to do
+struct LossArgs { const RowsPart* parts; int n; float denom; float* loss; };   // loss null: nothing to do
 
 // The loss of all rows, by one workgroup, in float64 and a fixed order.  `inv`: 1 / n, or null where nothing needed it before.
 template <int NT>
 __device__ __forceinline__ void sum_loss(const LossArgs& a, const float* inv) {
-  __shared__ double w[NT / 64];
+  __shared__ double ws[NT / 64];
+  __shared__ uint32_t wn[NT / 64];
   double s = 0.0;
+  uint32_t n = 0;
 #pragma unroll 8
-  for (long t = threadIdx.x; t < a.T; t += NT) {
-    const float l = a.row_loss[t];
-    if (l != 0.f) s += (double)l * (a.row_weight ? a.row_weight[t] : 1.f);      // rows without a class have 0, whatever their weight
-  }
+  for (int i = threadIdx.x; i < a.n; i += NT) { s += a.parts[i].loss; n += a.parts[i].rows; }
 #pragma unroll
-  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
-  const float scale = inv ? *inv : inverse_of_rows<NT>(a.target, a.T, a.V, a.denom);
+  for (int o = 32; o; o >>= 1) { s += __shfl_xor(s, o, 64); n += __shfl_xor(n, o, 64); }
+  if ((threadIdx.x & 63) == 0) { ws[threadIdx.x >> 6] = s; wn[threadIdx.x >> 6] = n; }
   __syncthreads();
   if (threadIdx.x == 0) {
     double all = 0.0;
-    for (int i = 0; i < NT / 64; ++i) all += w[i];
-    *a.loss = (float)(all * scale);
+    uint32_t rows = 0;
+    for (int i = 0; i < NT / 64; ++i) { all += ws[i]; rows += wn[i]; }
+    *a.loss = (float)(all * (inv ? *inv : 1.f / (a.denom > 0.f ? a.denom : (float)(rows ? rows : 1u))));
   }
 }
 
-__global__ __launch_bounds__(256) void loss_kernel(LossArgs a) { sum_loss<256>(a, nullptr); }
+__global__ __launch_bounds__(1024) void loss_kernel(LossArgs a) { sum_loss<1024>(a, nullptr); }
 
 // ------------------------------------------------------------------------------------------------ scores
 struct ScoreOut {
@@ -196,13 +200,21 @@ __global__ __launch_bounds__(T::NT) void scores_kernel(TnArgs g, ScoreOut o) {
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-// ROWS rows a workgroup, NT / ROWS threads each over the strips: 32, so that a strip's line is read whole, or 2 for few rows
+struct RowsArgs {
+  const float2* stats; int strips, rows; const int64_t* target; long V; const float *target_score, *row_weight;
+  float *lse, *row_loss;
+  RowsPart* parts;          // one a workgroup
+};
+
+// ROWS rows a workgroup, NT / ROWS threads each over the strips: 32, so that a strip's line is read whole, or 2 for few rows.  Threads 0 ..
+// ROWS - 1 get their row's loss times its weight, thread 0 the sum of them and how many have a class.
 template <int NT, int ROWS>
-__device__ __forceinline__ void reduce_rows(const float2* __restrict__ stats, int strips, int rows, const int64_t* __restrict__ target, long V,
-                                                   const float* __restrict__ target_score, float* __restrict__ lse, float* __restrict__ row_loss) {
+__device__ __forceinline__ RowsPart reduce_rows(const RowsArgs& a) {
   constexpr int LANES = NT / ROWS, AHEAD = 8;
   __shared__ float2 part[LANES][ROWS];
   const int r = threadIdx.x % ROWS, q = threadIdx.x / ROWS, n = blockIdx.x * ROWS + r;
+  const float2* __restrict__ stats = a.stats;
+  const int strips = a.strips, rows = a.rows;
   float top = -INFINITY, sum = 0.f;
   if (n < rows) {
     for (int s0 = q; s0 < strips; s0 += AHEAD * LANES) {
@@ -232,28 +244,40 @@ __device__ __forceinline__ void reduce_rows(const float2* __restrict__ stats, in
       part[q][r] = make_float2(t, sx + sy);
     }
   }
+  RowsPart mine{0.0, 0u, 0u};
   if (q == 0 && n < rows) {
     const float t = part[0][r].x, s = part[0][r].y;
     const float l = t + logf(s);
-    lse[n] = l;
-    const int64_t y = target[n];
-    row_loss[n] = (y >= 0 && y < V) ? l - target_score[n] : 0.f;
+    a.lse[n] = l;
+    const int64_t y = a.target[n];
+    const bool counts = y >= 0 && y < a.V;
+    const float loss = counts ? l - a.target_score[n] : 0.f;
+    a.row_loss[n] = loss;
+    mine.rows = counts;
+    if (loss != 0.f) mine.loss = (double)loss * (a.row_weight ? a.row_weight[n] : 1.f);      // rows without a class have 0, whatever their weight
   }
+#pragma unroll
+  for (int o = ROWS / 2; o; o >>= 1) { mine.loss += __shfl_xor(mine.loss, o, 64); mine.rows += __shfl_xor(mine.rows, o, 64); }
+  return mine;
 }
 
+// counts not null: one more workgroup, which puts them together
 template <int ROWS>
-__global__ __launch_bounds__(256) void rows_kernel(const float2* __restrict__ stats, int strips, int rows, const int64_t* __restrict__ target, long V,
-                                                   const float* __restrict__ target_score, float* __restrict__ lse, float* __restrict__ row_loss) {
-  reduce_rows<256, ROWS>(stats, strips, rows, target, V, target_score, lse, row_loss);
+__global__ __launch_bounds__(256) void rows_kernel(RowsArgs a, const uint32_t* __restrict__ counts, int n, float denom, float* __restrict__ inv) {
+  if (counts && blockIdx.x == gridDim.x - 1) {
+    const float x = inverse_of<256>(counts, n, denom);
+    if (threadIdx.x == 0) *inv = x;
+    return;
+  }
+  const RowsPart part = reduce_rows<256, ROWS>(a);
+  if (threadIdx.x == 0) a.parts[blockIdx.x] = part;
 }
 
 // Up to 8 rows and no gradients: rows and loss by one workgroup with 128 threads a row, which spares a launch (for 5 rows against 32768 classes;
 // with 32 threads a row, for up to 32 rows, it took 4 us longer than two launches)
-__global__ __launch_bounds__(1024) void rows_and_loss_kernel(const float2* __restrict__ stats, int strips, const float* __restrict__ target_score,
-                                                             float* __restrict__ lse, float* row_loss, LossArgs a) {
-  reduce_rows<1024, 8>(stats, strips, (int)a.T, a.target, a.V, target_score, lse, row_loss);
-  __syncthreads();
-  sum_loss<1024>(a, nullptr);
+__global__ __launch_bounds__(1024) void rows_and_loss_kernel(RowsArgs a, float denom, float* __restrict__ loss) {
+  const RowsPart all = reduce_rows<1024, 8>(a);
+  if (threadIdx.x == 0) *loss = (float)(all.loss * (1.f / (denom > 0.f ? denom : (float)(all.rows ? all.rows : 1u))));
 }
 
 // ------------------------------------------------------------------------------------------------ turn
@@ -261,26 +285,26 @@ struct TurnArgs {
   const void* e; long pitch;             // exponentials [rows][pitch]
   const float2* stats; const float* lse; const float* target_score; const int64_t* target; const float* row_weight; const float* inv;
   uint16_t* d; long plane;               // [planes][rows, whole tiles of 64][pitch]; in e's place for bfloat16
-  int rows, V, strip, across;            // strip: classes that share a maximum; across: workgroups for the classes
+  int rows, whole, V, strip, across;     // whole: rows, to whole tiles of 64; strip: classes that share a maximum; across: workgroups for the classes
   bool past;                             // d is larger than the caches
 };
 
-// 16 rows x 512 classes a workgroup, 8 classes a thread and row: d_tv = e_tv * exp(max_strip - lse_t) * w_t / n, the row's own class from its float32
-// score.  Rows behind the last (to whole tiles of 64) and without a class are zeros; so are classes behind the last, to the pitch.
-// P planes of d: 3 for float32; 1 for bfloat16, or 2 for few rows (plan_of).
-template <bool F32, int P>
+// 16 rows x 512 classes a workgroup -- or, where the pitch is 64, 128 rows x 64 --, 8 classes a thread and row: d_tv = e_tv * exp(max_strip - lse_t)
+// * w_t / n, the row's own class from its float32 score.  Rows behind the last (to whole tiles of 64) and without a class are zeros; so are classes
+// behind the last, to the pitch.  P planes of d: 3 for float32; 1 for bfloat16, or 2 for few rows (plan_of).  LANES: threads a row.
+template <bool F32, int P, int LANES>
 __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
-  if (blockIdx.x == gridDim.x - 1) {      // one more workgroup, which sums the loss, with the last block of rows
+  if (blockIdx.x == 0) {                  // one more workgroup, which sums the loss, with the last block of rows
     if (l.loss) sum_loss<256>(l, a.inv);
     return;
   }
-  constexpr int ROWS = 16;
-  __shared__ float factor[16][ROWS];     // of each 32 classes: strips of 32 are the shortest
+  constexpr int ROWS = 1024 / LANES, GROUPS = LANES / 4;
+  __shared__ float factor[GROUPS][ROWS + 1];     // of each 32 classes: strips of 32 are the shortest
   __shared__ float own[ROWS];
   __shared__ int at[ROWS];
-  const int v0 = blockIdx.x % a.across * 512, t0 = blockIdx.x / a.across * ROWS;
+  const int v0 = (blockIdx.x - 1) % a.across * (8 * LANES), t0 = (blockIdx.x - 1) / a.across * ROWS;
   {
-    const int r = threadIdx.x & 15, k = threadIdx.x >> 4, t = t0 + r, v = v0 + 32 * k;
+    const int r = threadIdx.x % ROWS, k = threadIdx.x / ROWS, t = t0 + r, v = v0 + 32 * k;
     float f = 0.f, mine = 0.f;
     int where = -1;
     if (t < a.rows) {
@@ -296,11 +320,12 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
     if (k == 0) { own[r] = mine; at[r] = where; }
   }
   __syncthreads();
-  const int c = (threadIdx.x & 63) * 8, v = v0 + c;
+  const int c = threadIdx.x % LANES * 8, v = v0 + c;
   if (v >= a.pitch) return;
 #pragma unroll
-  for (int r = threadIdx.x >> 6; r < ROWS; r += 4) {
+  for (int r = threadIdx.x / LANES; r < ROWS; r += 256 / LANES) {
     const int t = t0 + r;
+    if (t >= a.whole) return;
     const long to = (long)t * a.pitch + v;
     const float f = factor[c >> 5][r];
     float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -409,8 +434,8 @@ __device__ __forceinline__ void lay_out_tile(const LayOut& a, int id) {
 // Everything that can be laid out before the products, in one launch: `first` workgroups for a, `second` for b, and one more that leaves
 // 1 / n in inv (null: not wanted).
 template <bool F32>
-__global__ __launch_bounds__(256) void prepare_kernel(LayOut a, int first, LayOut b, int second, const int64_t* __restrict__ target, long T, long V, float denom,
-                                                      float* __restrict__ inv) {
+__global__ __launch_bounds__(256) void prepare_kernel(LayOut a, int first, LayOut b, int second, const int64_t* __restrict__ target, long T, long V,
+                                                      uint32_t* __restrict__ counts) {
   const int id = blockIdx.x;
   if (id < first) {
     if (a.wide) lay_out_tile<F32, true>(a, id);
@@ -418,9 +443,18 @@ __global__ __launch_bounds__(256) void prepare_kernel(LayOut a, int first, LayOu
   } else if (id < first + second) {
     if (b.wide) lay_out_tile<F32, true>(b, id - first);
     else lay_out_tile<F32, false>(b, id - first);
-  } else if (inv) {
-    const float x = inverse_of_rows<256>(target, T, V, denom);
-    if (threadIdx.x == 0) *inv = x;
+  } else {
+    __shared__ uint32_t w[4];
+    const long t0 = (id - first - second) * COUNTED;
+    const int n = (int)(T - t0 < COUNTED ? T - t0 : COUNTED);
+    uint32_t sum = 0;
+#pragma unroll 8
+    for (int t = threadIdx.x; t < n; t += 256) { const int64_t y = target[t0 + t]; sum += y >= 0 && y < V; }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[id - first - second] = w[0] + w[1] + w[2] + w[3];
   }
 }
 
@@ -501,6 +535,7 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
                                                     int c_bf16) {
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
     float s = add ? add[i] : 0.f;
+#pragma unroll 8
     for (int k = 0; k < splits; ++k) s += part[k * stride + i];
     if (c_bf16) reinterpret_cast<uint16_t*>(c)[i] = to_bf16(s);
     else reinterpret_cast<float*>(c)[i] = s;
@@ -521,8 +556,9 @@ struct Plan {
   bool f32, grad, direct;        // direct: x and W are used where they are
   long T, V, D, Kp, Vp, R, Rp;   // pitches for D and V values; rows of a block, pitch for them
   int blocks, planes, pairs, tile_scores, strips, strip;
+  int counters;                  // workgroups that count rows
   int d_planes, d_pairs;         // of d, and products of pairs of planes in the gradients
-  size_t inv, stats, lse, tscore, xp, wp, xt, e, d, dw, part, total, part_bytes;
+  size_t inv, counts, rparts, stats, lse, tscore, xp, wp, xt, e, d, dw, part, total, part_bytes;
 };
 
 // Which tile, and how many parts of k: the choice with the shortest time by what one step of 64 in k takes a full chip of workgroups --
@@ -530,7 +566,7 @@ struct Plan {
 // memory (written and read once more, at 4 TB/s, and a launch).
 struct Shape { int wide; int splits; };
 Shape shape_of(long M, long N, long steps, bool may_split) {
-  static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
+  static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256};
   Shape best{1, 1};
   double least = 1e300;
   for (int wide = 0; wide < 2; ++wide) {
@@ -578,6 +614,9 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
   size_t at = 0;
   const auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   p.inv = take(4);
+  p.counters = grad ? cdiv(T, COUNTED) : 0;
+  p.counts = take((size_t)p.counters * 4);
+  p.rparts = take((size_t)(cdiv(T, 32) + 32) * sizeof(RowsPart));
   p.stats = take((size_t)p.strips * p.R * 8);
   p.lse = take((size_t)p.R * 4);
   p.tscore = take((size_t)p.R * 4);
@@ -676,12 +715,14 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
   float2* stats = reinterpret_cast<float2*>(ws + p.stats);
   const uint16_t *xp = reinterpret_cast<const uint16_t*>(x), *wp = reinterpret_cast<const uint16_t*>(weight);
   const size_t es = bf16 ? 2 : 4;
-  const LossArgs loss{row_loss, row_weight, target, (long)T, (long)V, (float)denom, loss_out};
-  const auto prepare = [&](const LayOut& a, int first, const LayOut& b, int second, float* inv) {
-    const int grid = first + second + (inv ? 1 : 0);
+  RowsPart* const parts = reinterpret_cast<RowsPart*>(ws + p.rparts);
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(ws + p.counts);
+  int sums = 0;      // parts written so far
+  const auto prepare = [&](const LayOut& a, int first, const LayOut& b, int second, int counters) {
+    const int grid = first + second + counters;
     if (grid == 0) return;
-    if (p.f32) hipLaunchKernelGGL((prepare_kernel<true>), dim3(grid), dim3(256), 0, st, a, first, b, second, target, (long)T, (long)V, (float)denom, inv);
-    else hipLaunchKernelGGL((prepare_kernel<false>), dim3(grid), dim3(256), 0, st, a, first, b, second, target, (long)T, (long)V, (float)denom, inv);
+    if (p.f32) hipLaunchKernelGGL((prepare_kernel<true>), dim3(grid), dim3(256), 0, st, a, first, b, second, target, (long)T, (long)V, counts);
+    else hipLaunchKernelGGL((prepare_kernel<false>), dim3(grid), dim3(256), 0, st, a, first, b, second, target, (long)T, (long)V, counts);
   };
   {
     // a single block's transposed x is made here too; rows of x without a class are zeros in both, which changes nothing that counts
@@ -690,7 +731,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     const bool turn_x = grad && p.blocks == 1;
     if (!p.direct) first = lay_out(w, p.f32, weight, V, D, h(p.wp), p.Kp, nullptr, 0, nullptr, 0);
     if (!p.direct || turn_x) second = lay_out(xs, p.f32, x, T, D, p.direct ? nullptr : h(p.xp), p.Kp, turn_x ? h(p.xt) : nullptr, p.Rp, target, V);
-    prepare(w, first, xs, second, grad ? f(p.inv) : nullptr);
+    prepare(w, first, xs, second, p.counters);
     if (!p.direct) { xp = h(p.xp); wp = h(p.wp); }
   }
   for (int b = 0; b < p.blocks; ++b) {
@@ -705,13 +746,17 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     if (p.tile_scores == 0) DPPM_TRY(p.f32 ? (launch_scores<Wide, true>(g, o, st)) : (launch_scores<Wide, false>(g, o, st)));
     else if (p.tile_scores == 1) DPPM_TRY(p.f32 ? (launch_scores<Mid, true>(g, o, st)) : (launch_scores<Mid, false>(g, o, st)));
     else DPPM_TRY(p.f32 ? (launch_scores<Narrow, true>(g, o, st)) : (launch_scores<Narrow, false>(g, o, st)));
-    // a thread's share of the strips is what takes the time: with few rows, more threads a row
+    const RowsArgs r{stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), row_weight ? row_weight + t0 : nullptr, f(p.lse), row_loss + t0, parts + sums};
     if (!grad && T <= 8) {
-      hipLaunchKernelGGL(rows_and_loss_kernel, dim3(1), dim3(1024), 0, st, stats, p.strips, f(p.tscore), f(p.lse), row_loss, loss);
+      hipLaunchKernelGGL(rows_and_loss_kernel, dim3(1), dim3(1024), 0, st, r, (float)denom, loss_out);
       break;
     }
-    if (rows <= 64) hipLaunchKernelGGL((rows_kernel<2>), dim3(cdiv(rows, 2)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
-    else hipLaunchKernelGGL((rows_kernel<32>), dim3(cdiv(rows, 32)), dim3(256), 0, st, stats, p.strips, (int)rows, target + t0, (long)V, f(p.tscore), f(p.lse), row_loss + t0);
+    // a thread's share of the strips is what takes the time: with few rows, more threads a row
+    const int by = rows <= 64 ? 2 : 32, n = cdiv(rows, by);
+    const bool join = grad && b == 0;
+    if (by == 2) hipLaunchKernelGGL((rows_kernel<2>), dim3(n + join), dim3(256), 0, st, r, join ? counts : nullptr, p.counters, (float)denom, f(p.inv));
+    else hipLaunchKernelGGL((rows_kernel<32>), dim3(n + join), dim3(256), 0, st, r, join ? counts : nullptr, p.counters, (float)denom, f(p.inv));
+    sums += n;
     if (!grad) continue;
     const int whole = cdiv(rows, 64) * 64;
     TurnArgs a{};
@@ -719,17 +764,21 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     a.row_weight = row_weight ? row_weight + t0 : nullptr; a.inv = f(p.inv);
     a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip; a.past = (size_t)p.d_planes * a.plane * 2 > CACHED;
     const bool last = b == p.blocks - 1;
-    LossArgs sum = loss;
-    if (!last) sum.loss = nullptr;
-    a.across = cdiv(p.Vp, 512);
-    const dim3 grid((unsigned)((long)a.across * (whole / 16) + 1));      // (a second dimension of a grid ends at 65535)
-    if (p.f32) hipLaunchKernelGGL((turn_kernel<true, 3>), grid, dim3(256), 0, st, a, sum);
-    else if (p.d_planes == 2) hipLaunchKernelGGL((turn_kernel<false, 2>), grid, dim3(256), 0, st, a, sum);
-    else hipLaunchKernelGGL((turn_kernel<false, 1>), grid, dim3(256), 0, st, a, sum);
+    const LossArgs sum{parts, sums, (float)denom, last ? loss_out : nullptr};
+    const int lanes = p.Vp <= 64 && p.d_planes != 2 ? 8 : 64;
+    a.whole = whole;
+    a.across = cdiv(p.Vp, 8 * lanes);
+    const dim3 grid((unsigned)((long)a.across * cdiv(whole, 1024 / lanes) + 1));      // (a second dimension of a grid ends at 65535)
+    if (p.f32) {
+      if (lanes == 8) hipLaunchKernelGGL((turn_kernel<true, 3, 8>), grid, dim3(256), 0, st, a, sum);
+      else hipLaunchKernelGGL((turn_kernel<true, 3, 64>), grid, dim3(256), 0, st, a, sum);
+    } else if (p.d_planes == 2) hipLaunchKernelGGL((turn_kernel<false, 2, 64>), grid, dim3(256), 0, st, a, sum);
+    else if (lanes == 8) hipLaunchKernelGGL((turn_kernel<false, 1, 8>), grid, dim3(256), 0, st, a, sum);
+    else hipLaunchKernelGGL((turn_kernel<false, 1, 64>), grid, dim3(256), 0, st, a, sum);
     if (p.blocks > 1) {
       LayOut xs{};
       const int n = lay_out(xs, p.f32, reinterpret_cast<const char*>(x) + t0 * D * es, rows, D, nullptr, 0, h(p.xt), Rp, target + t0, V);
-      prepare(xs, n, xs, 0, nullptr);
+      prepare(xs, n, xs, 0, 0);
     }
     TnArgs gx{};       // dx[t][d] = sum_v d[t][v] W[v][d]
     gx.A = wp; gx.lda = p.Kp; gx.plane_a = V * p.Kp; gx.M = (int)D;
@@ -743,6 +792,6 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     float* total = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
     DPPM_TRY((grad_product<false, true>)(gw, last || p.f32 ? dweight : (void*)total, bf16 && last, b == 0 ? nullptr : total, f(p.part), p.part_bytes, st));
   }
-  if (!grad && T > 8) hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(256), 0, st, loss);
+  if (!grad && T > 8) hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, LossArgs{parts, sums, (float)denom, loss_out});
   return check_launch("dppm_loss_ce_fwd_bwd");
 }

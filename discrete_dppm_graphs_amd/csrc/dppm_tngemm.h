@@ -273,7 +273,7 @@ __device__ __forceinline__ void tn_rows(char* lds, const tn_acc (&acc)[T::MI][T:
 }
 
 // The same with the values packed to 16 bits on the way in, which halves the LDS traffic
-// (4099 x 1000 bfloat16, 50001 classes: 1.49 -> 1.47 ms): pack(lo, hi) makes a word of two,
+// (4099 x 1000 bfloat16, 50001 classes: 1.525 -> 1.510 ms): pack(lo, hi) makes a word of two,
 // emit(row, m, word[4]) gets eight values.
 template <class T, class Pack, class Emit>
 __device__ __forceinline__ void tn_rows16(char* lds, const tn_acc (&acc)[T::MI][T::NI], int block, Pack pack, Emit emit) {
