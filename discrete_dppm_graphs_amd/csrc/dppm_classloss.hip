@@ -16,7 +16,7 @@
 //  * dx = d W and dW = d^T x: W and d are read transposed from LDS where the contracted dimension is not the contiguous one; x, the smallest,
 //    is transposed in memory, with zeros for rows that have no class.
 // The exponentials held at a time are those of one block of rows, at most 2^30 (bfloat16) or 2^27 (float32) of them: memory does not grow
-// with T.  Several blocks add up dW in float32.
+// with T.  Several blocks add up dW in float32.  Few classes go another way, in one pass (few_kernel).
 #include "dppm_common.h"
 #include "dppm_tngemm.h"
 
@@ -71,22 +71,42 @@ constexpr size_t CACHED = 256u << 20;
 struct RowsPart { double loss; uint32_t rows, pad; };
 constexpr long COUNTED = 4096;
 
-// 1 / denom, or 1 / (the sum of counts) where none is given; all NT threads get it
+// 1 / denom, or 1 / (the sum of all threads' rows) where none is given; all NT threads get it
 template <int NT>
-__device__ __forceinline__ float inverse_of(const uint32_t* counts, int n, float denom) {
+__device__ __forceinline__ float inverse_of(uint32_t rows, float denom) {
   __shared__ uint32_t w[NT / 64];
-  uint32_t sum = 0;
-  if (!(denom > 0.f)) {
-#pragma unroll 8
-    for (int i = threadIdx.x; i < n; i += NT) sum += counts[i];
-  }
 #pragma unroll
-  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
+  for (int o = 32; o; o >>= 1) rows += __shfl_xor(rows, o, 64);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = rows;
   __syncthreads();
   uint32_t all = 0;
   for (int i = 0; i < NT / 64; ++i) all += w[i];
   return 1.f / (denom > 0.f ? denom : (float)(all ? all : 1u));
+}
+// a thread's share of the rows with a class, from the targets or from what workgroups counted
+template <int NT>
+__device__ __forceinline__ uint32_t rows_with_class(const int64_t* target, long T, long V) {
+  uint32_t n = 0;
+#pragma unroll 8
+  for (int t = threadIdx.x; t < T; t += NT) n += target[t] >= 0 && target[t] < V;
+  return n;
+}
+template <int NT>
+__device__ __forceinline__ uint32_t rows_counted(const uint32_t* counts, int n) {
+  uint32_t sum = 0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += NT) sum += counts[i];
+  return sum;
+}
+__device__ __forceinline__ void count_rows(const int64_t* target, long T, long V, int part, uint32_t* counts) {    // 256 threads
+  __shared__ uint32_t w[4];
+  const long t0 = part * COUNTED;
+  uint32_t sum = rows_with_class<256>(target + t0, T - t0 < COUNTED ? T - t0 : COUNTED, V);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) counts[part] = w[0] + w[1] + w[2] + w[3];
 }
 
 struct LossArgs { const RowsPart* parts; int n; float denom; float* loss; };   // loss null: nothing to do
@@ -265,7 +285,7 @@ __device__ __forceinline__ RowsPart reduce_rows(const RowsArgs& a) {
 template <int ROWS>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a, const uint32_t* __restrict__ counts, int n, float denom, float* __restrict__ inv) {
   if (counts && blockIdx.x == gridDim.x - 1) {
-    const float x = inverse_of<256>(counts, n, denom);
+    const float x = inverse_of<256>(denom > 0.f ? 0u : rows_counted<256>(counts, n), denom);
     if (threadIdx.x == 0) *inv = x;
     return;
   }
@@ -443,19 +463,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(LayOut a, int first, LayOu
   } else if (id < first + second) {
     if (b.wide) lay_out_tile<F32, true>(b, id - first);
     else lay_out_tile<F32, false>(b, id - first);
-  } else {
-    __shared__ uint32_t w[4];
-    const long t0 = (id - first - second) * COUNTED;
-    const int n = (int)(T - t0 < COUNTED ? T - t0 : COUNTED);
-    uint32_t sum = 0;
-#pragma unroll 8
-    for (int t = threadIdx.x; t < n; t += 256) { const int64_t y = target[t0 + t]; sum += y >= 0 && y < V; }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) counts[id - first - second] = w[0] + w[1] + w[2] + w[3];
-  }
+  } else
+    count_rows(target, T, V, id - first - second, counts);
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
@@ -540,6 +549,307 @@ __global__ __launch_bounds__(256) void parts_kernel(const float* __restrict__ pa
     if (c_bf16) reinterpret_cast<uint16_t*>(c)[i] = to_bf16(s);
     else reinterpret_cast<float*>(c)[i] = s;
   }
+}
+
+// ------------------------------------------------------------------------------------------------ few classes
+// Up to 32 classes of up to 512 values: all of W lies in LDS and a row's scores in the registers of four lanes, so that one pass over x gives the
+// losses, dx and each workgroup's part of dW, and neither scores nor d reach memory.  x is read twice (the second time from the caches), dx
+// written once.  A wave takes 16 rows at a time, in three products on the matrix cores:
+//   s = W x^T    k = dims: lane i + 16 g holds row i, dims 32 step + 8 g .. + 7 (16 or 32 bytes of x); out come classes 4 g .. 4 g + 3 of row i,
+//   dx^T = W^T d k = classes: those four are the operand as they stand; out come the same dims of row i as were read,
+//   dW += d x    k = rows: d turned in LDS, x read again with a lane's four dims of row 4 t + g.
+// float32: all three by v_mfma_f32_16x16x4_f32, 96 operations a value with the classes padded to 16.  bfloat16: scores in one exact product
+// of the operands, dx with d in two bfloat16 planes, which hold 2^-17 of it; dW in float32 as well, its operands being a row's dims and not a dim's rows.
+// LDS holds W twice, in the order of each product's fragments; slot 2 step + u, place q holds dim 32 step + 8 (q / 4) + 4 u + q % 4.
+struct FewArgs {
+  const void *x, *weight; const int64_t* target; const float* row_weight;
+  const uint32_t* counts; int counters;            // 0: every workgroup counts for itself
+  long T; int V, D; float denom;
+  float* row_loss; void* dx;                       // dx null: losses only
+  float* part; RowsPart* parts;                    // [workgroups][V][D], [workgroups]
+};
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+constexpr int FEW_CLASSES = 32, FEW_VALUES = 512;  // (padded classes / 16) * padded D at most FEW_VALUES: dW fits in 128 registers
+
+template <bool F32>
+__device__ __forceinline__ void load8(const void* x, long at, float (&v)[8]) {
+  if (F32) {
+    const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x) + at);
+    const f32x4 a = p[0], b = p[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+  } else {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(x) + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+  }
+}
+template <bool F32>
+__device__ __forceinline__ f32x4 load4(const void* x, long at) {
+  if (F32) return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x) + at);
+  const u32x2 w = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint16_t*>(x) + at);
+  return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
+}
+
+// CT: sixteens of classes, NC: sixty-fours of dims
+template <bool F32, int CT, int NC>
+__global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : 2) void few_kernel(FewArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ __attribute__((aligned(16))) float turned[4][CT][16][20];
+  __shared__ RowsPart sums[4];
+  float* const wk = reinterpret_cast<float*>(lds);       // float32: [slot][ct][class][q]
+  float* const wc = wk + NC * CT * 1024;                 //          [slot][ct][q][class]
+  uint16_t* const hk = reinterpret_cast<uint16_t*>(lds); // bfloat16: [step][ct][class][dim]
+  uint16_t* const hc = hk + NC * CT * 1024;              //           [slot][q][class / 4][ct][class % 4]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+  for (int k = threadIdx.x; k < 16 * CT * 8 * NC; k += 256) {
+    const int v = k / (8 * NC), d = k % (8 * NC) * 8, st = d / 32, o = d % 32 / 8, ct = v / 16, c = v % 16;
+    const bool in = v < a.V && d < a.D;
+    const long from = in ? (long)v * a.D + d : 0;
+    if constexpr (F32) {
+      float w[8];
+      load8<F32>(a.weight, from, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = in ? w[e] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int at = (2 * st + u) * CT + ct;
+        *reinterpret_cast<f32x4*>(wk + (at * 16 + c) * 16 + 4 * o) = f32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wc[(at * 16 + 4 * o + e) * 16 + c] = w[4 * u + e];
+      }
+    } else {
+      u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.weight) + from);
+      if (!in) w = u32x4{0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4*>(hk + ((st * CT + ct) * 16 + c) * 32 + 8 * o) = w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hc[((((2 * st + e / 4) * 16 + 4 * o + e % 4) * 4 + c / 4) * CT + ct) * 4 + c % 4] = (uint16_t)(w[e / 2] >> e % 2 * 16);
+    }
+  }
+  float inv = 0.f;
+  if (a.dx)
+    inv = inverse_of<256>(a.denom > 0.f ? 0u : a.counters ? rows_counted<256>(a.counts, a.counters) : rows_with_class<256>(a.target, a.T, a.V), a.denom);
+  __syncthreads();
+
+  f32x4 dw[CT][NC][4];                                   // classes 4 g .. + 3 of dim 64 c + 4 i + e
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dw[ct][c][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  RowsPart mine{0.0, 0u, 0u};
+  constexpr int AHEAD = NC == 1 ? 2 : 4;                 // steps of 32 dims that are read together
+  const int steps = (a.D + 31) / 32;
+  for (long t0 = ((long)blockIdx.x * 4 + wave) * 16; t0 < a.T; t0 += (long)gridDim.x * 64) {
+    const long t = t0 + i < a.T ? t0 + i : a.T - 1;      // rows behind the last repeat it and count for nothing
+    const int64_t y = a.target[t];
+    const bool in = t0 + i < a.T, counts = in && y >= 0 && y < a.V;
+    f32x4 s[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) s[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; 32 * s0 < a.D; s0 += AHEAD) {
+      if constexpr (F32) {
+        float v[AHEAD][8];
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h) {
+          const int d = 32 * (s0 + h) + 8 * g;
+          load8<F32>(a.x, t * a.D + (d < a.D ? d : 0), v[h]);
+          if (d >= a.D) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[h][e] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const f32x4 w = *reinterpret_cast<const f32x4*>(wk + (((2 * (s0 + h) + u) * CT + ct) * 16 + i) * 16 + 4 * g);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], v[h][4 * u + e], s[ct], 0, 0, 0);
+            }
+      } else {
+        u32x4 v[AHEAD];
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h) {
+          const int d = 32 * (s0 + h) + 8 * g;
+          v[h] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.x) + t * a.D + (d < a.D ? d : 0));
+          if (d >= a.D) v[h] = u32x4{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            s[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const tn_frag*>(hk + (((s0 + h) * CT + ct) * 16 + i) * 32 + 8 * g),
+                                                            __builtin_bit_cast(tn_frag, v[h]), s[ct], 0, 0, 0);
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (16 * ct + 4 * g + j < a.V) top = fmaxf(top, s[ct][j]);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    float sum = 0.f, own = 0.f;
+    f32x4 p[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int v = 16 * ct + 4 * g + j;
+        p[ct][j] = v < a.V ? exp_of<F32>(s[ct][j] - top) : 0.f;
+        sum += p[ct][j];
+        if (v == y) own = s[ct][j];
+      }
+    sum += __shfl_xor(sum, 16, 64);
+    own += __shfl_xor(own, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    own += __shfl_xor(own, 32, 64);
+    const float loss = counts ? top + logf(sum) - own : 0.f;
+    const float weight = counts && a.row_weight ? a.row_weight[t] : 1.f;
+    if (g == 0) {
+      if (in) a.row_loss[t] = loss;
+      if (counts) { mine.rows += 1; mine.loss += loss != 0.f ? (double)loss * weight : 0.0; }
+    }
+    if (!a.dx) continue;
+
+    const float share = weight * inv, r = 1.f / sum;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[ct][j] = counts ? (p[ct][j] * r - (16 * ct + 4 * g + j == y ? 1.f : 0.f)) * share : 0.f;      // d
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<f32x4*>(&turned[wave][ct][i][4 * g]) = p[ct];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    u32x4 plane[2];      // bfloat16: d in two planes, class 4 g + j of the first sixteen, then of the second
+    if (!F32) {
+      f32x4 rest[CT];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            uint32_t w = 0;
+            if (ct < CT) {
+              const float lo = k ? rest[ct][j] : p[ct][j], hi = k ? rest[ct][j + 1] : p[ct][j + 1];
+              w = pack_bf16(lo, hi);
+              if (k == 0) { rest[ct][j] = lo - __uint_as_float(w << 16); rest[ct][j + 1] = hi - __uint_as_float(w & 0xffff0000u); }
+            }
+            plane[k][2 * ct + j / 2] = w;
+          }
+    }
+#pragma unroll 1
+    for (int st = 0; st < steps; ++st) {
+      f32x4 o[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (!F32) {
+          const uint16_t* w = hc + (((2 * st + u) * 16 + i) * 4 + g) * CT * 4;
+#pragma unroll
+          for (int k = 1; k >= 0; --k) {
+            if constexpr (CT == 2)
+              o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const tn_frag*>(w), __builtin_bit_cast(tn_frag, plane[k]), o[u], 0, 0, 0);
+            else
+              o[u] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(*reinterpret_cast<const s16x4*>(w), __builtin_bit_cast(s16x4, u32x2{plane[k].x, plane[k].y}), o[u], 0, 0, 0);
+          }
+        } else
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const f32x4 w = *reinterpret_cast<const f32x4*>(wc + (((2 * st + u) * CT + ct) * 16 + i) * 16 + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], p[ct][j], o[u], 0, 0, 0);
+        }
+      }
+      const int d = 32 * st + 8 * g;
+      if (in && d < a.D) {
+        if (F32) {
+          f32x4* to = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.dx) + t * a.D + d);
+          to[0] = o[0];
+          to[1] = o[1];
+        } else
+          *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(a.dx) + t * a.D + d) =
+              u32x4{pack_bf16(o[0][0], o[0][1]), pack_bf16(o[0][2], o[0][3]), pack_bf16(o[1][0], o[1][1]), pack_bf16(o[1][2], o[1][3])};
+      }
+    }
+    const uint32_t have = (uint32_t)__ballot(counts);    // bit i: row i; what a row without a class holds is not looked at
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = 4 * k + g;
+      const bool has = have >> row & 1;
+      const long from = (t0 + row < a.T ? t0 + row : a.T - 1) * a.D;
+      float d[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) d[ct] = turned[wave][ct][row][i];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int at = 64 * c + 4 * i;
+        f32x4 v = load4<F32>(a.x, from + (at < a.D ? at : 0));
+        if (!has || at >= a.D) v = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dw[ct][c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(d[ct], v[e], dw[ct][c][e], 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+
+#pragma unroll
+  for (int o = 8; o; o >>= 1) { mine.loss += __shfl_xor(mine.loss, o, 64); mine.rows += __shfl_xor(mine.rows, o, 64); }
+  if (lane == 0) sums[wave] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    RowsPart all = sums[0];
+    for (int w = 1; w < 4; ++w) { all.loss += sums[w].loss; all.rows += sums[w].rows; }
+    a.parts[blockIdx.x] = all;
+  }
+  if (!a.dx) return;
+  for (int w = 0; w < 4; ++w) {                          // the waves' parts of dW in turn, in the place of W
+    if (wave == w) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f32x4* to = reinterpret_cast<f32x4*>(wk + (16 * ct + 4 * g + j) * 64 * NC + 64 * c + 4 * i);
+            const f32x4 v{dw[ct][c][0][j], dw[ct][c][1][j], dw[ct][c][2][j], dw[ct][c][3][j]};
+            *to = w ? *to + v : v;
+          }
+    }
+    __syncthreads();
+  }
+  const int n = a.V * a.D;
+  for (int k = threadIdx.x; k < n; k += 256) a.part[(long)blockIdx.x * n + k] = wk[k / a.D * 64 * NC + k % a.D];
+}
+
+__global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ target, long T, long V, uint32_t* __restrict__ counts) { count_rows(target, T, V, blockIdx.x, counts); }
+
+// dW from the workgroups' parts: 64 values a workgroup, 16 threads each over the parts; and one more workgroup for the loss
+__global__ __launch_bounds__(1024) void few_join_kernel(const float* __restrict__ part, int parts, int n, void* __restrict__ dweight, int bf16, LossArgs l) {
+  if (blockIdx.x == 0) {
+    sum_loss<1024>(l, nullptr);
+    return;
+  }
+  __shared__ float w[16][64];
+  const int c = threadIdx.x & 63, q = threadIdx.x >> 6, k = (blockIdx.x - 1) * 64 + c;
+  float s = 0.f;
+  if (k < n) {
+#pragma unroll 8
+    for (int p = q; p < parts; p += 16) s += part[(long)p * n + k];
+  }
+  w[q][c] = s;
+  __syncthreads();
+  if (q || k >= n) return;
+  for (int p = 1; p < 16; ++p) s += w[p][c];
+  if (bf16) reinterpret_cast<uint16_t*>(dweight)[k] = to_bf16(s);
+  else reinterpret_cast<float*>(dweight)[k] = s;
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -676,6 +986,53 @@ int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, 
   return DPPM_OK;
 }
 
+// few_kernel: the rule on sizes, and its workspace.  Losses and gradients in one pass and by the products in tiles, which pad the classes to 128 and
+// hold x^T, scores and d in memory, bfloat16 / float32: 2^20 rows x 64, 5 classes 87 / 137 us and 443 / 1289 (60 / 118 at a copy's rate); at its largest
+// sizes, 2^16 x 512, 16 classes 57 / 90 and 98 / 350, 300 x 256, 32 classes 20 / 24 and 35 / 68.
+struct FewPlan { bool fits; int ct, nc, grid, counters; size_t counts, parts, part, total; };
+FewPlan few_plan(long T, long V, long D, bool grad) {
+  FewPlan f{};
+  f.ct = V <= 16 ? 1 : 2;
+  f.nc = D <= 64 ? 1 : D <= 128 ? 2 : D <= 256 ? 4 : 8;
+  f.fits = V <= FEW_CLASSES && D % 8 == 0 && D <= FEW_VALUES && f.ct * f.nc * 64 <= FEW_VALUES;
+  if (!f.fits) return f;
+  const long groups = (T + 63) / 64, most = CUS * (f.ct * f.nc <= 2 ? 4 : 2);
+  f.grid = (int)(groups < most ? groups : most);
+  f.counters = grad && T > COUNTED ? cdiv(T, COUNTED) : 0;
+  f.parts = ((size_t)f.counters * 4 + 255) / 256 * 256;
+  f.part = f.parts + ((size_t)f.grid * sizeof(RowsPart) + 255) / 256 * 256;
+  f.total = f.part + (grad ? (size_t)f.grid * V * D * 4 : 0);
+  return f;
+}
+template <bool F32, int CT, int NC>
+int launch_few(const FewArgs& a, int grid, hipStream_t st) {
+  constexpr int LDS = NC * CT * (F32 ? 8192 : 4096);
+  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(few_kernel<F32, CT, NC>), LDS, "dppm_loss_ce"));
+  hipLaunchKernelGGL((few_kernel<F32, CT, NC>), dim3(grid), dim3(256), LDS, st, a);
+  return DPPM_OK;
+}
+template <bool F32>
+int few_classes(const FewPlan& f, FewArgs a, bool denominator, float* loss, void* dweight, char* ws, hipStream_t st) {
+  a.counts = reinterpret_cast<uint32_t*>(ws + f.counts);
+  a.parts = reinterpret_cast<RowsPart*>(ws + f.parts);
+  a.part = reinterpret_cast<float*>(ws + f.part);
+  a.counters = denominator ? 0 : f.counters;
+  if (a.counters) hipLaunchKernelGGL(count_kernel, dim3(a.counters), dim3(256), 0, st, a.target, a.T, (long)a.V, reinterpret_cast<uint32_t*>(ws + f.counts));
+  if (f.ct == 1) {
+    if (f.nc == 1) DPPM_TRY((launch_few<F32, 1, 1>(a, f.grid, st)));
+    else if (f.nc == 2) DPPM_TRY((launch_few<F32, 1, 2>(a, f.grid, st)));
+    else if (f.nc == 4) DPPM_TRY((launch_few<F32, 1, 4>(a, f.grid, st)));
+    else DPPM_TRY((launch_few<F32, 1, 8>(a, f.grid, st)));
+  } else {
+    if (f.nc == 1) DPPM_TRY((launch_few<F32, 2, 1>(a, f.grid, st)));
+    else if (f.nc == 2) DPPM_TRY((launch_few<F32, 2, 2>(a, f.grid, st)));
+    else DPPM_TRY((launch_few<F32, 2, 4>(a, f.grid, st)));
+  }
+  const int n = a.dx ? a.V * a.D : 0;
+  hipLaunchKernelGGL(few_join_kernel, dim3(1 + cdiv(n, 64)), dim3(1024), 0, st, a.part, f.grid, n, dweight, (int)!F32, LossArgs{a.parts, f.grid, a.denom, loss});
+  return DPPM_OK;
+}
+
 // -> workgroups for it
 int lay_out(LayOut& a, bool f32, const void* src, long rows, long cols, uint16_t* as_is, long pitch, uint16_t* turned, long pitch_t, const int64_t* target, long V) {
   const long r = turned && pitch_t > rows ? pitch_t : rows, c = as_is ? pitch : cols;
@@ -693,7 +1050,8 @@ using namespace dppm;
 
 extern "C" size_t dppm_loss_ce_workspace_bytes(int64_t T, int64_t V, int64_t D, int bf16, int want_grad) {
   if (!sizes_ok(T, V, D) || T == 0) return 0;
-  return plan_of(T, V, D, !bf16, want_grad, false).total;      // the larger of the two layouts, so that the size does not depend on addresses
+  const size_t tiles = plan_of(T, V, D, !bf16, want_grad, false).total, few = few_plan(T, V, D, want_grad).total;
+  return tiles > few ? tiles : few;      // the largest of the layouts, so that the size does not depend on addresses
 }
 
 extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16, const int64_t* target, const float* row_weight, double denom, int64_t T,
@@ -706,6 +1064,13 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
   DPPM_REQUIRE((dx == nullptr) == (dweight == nullptr), "dppm_loss_ce_fwd_bwd: dx and dweight come together");
   DPPM_REQUIRE((uintptr_t)workspace % 16 == 0, "dppm_loss_ce_fwd_bwd: the workspace must be 16-byte aligned");
   const bool grad = dx != nullptr, aligned = ((uintptr_t)x | (uintptr_t)weight) % 16 == 0;
+  const FewPlan few = few_plan(T, V, D, grad);
+  if (few.fits && aligned && (uintptr_t)dx % 16 == 0) {
+    DPPM_REQUIRE(workspace_bytes >= few.total, "dppm_loss_ce_fwd_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, few.total);
+    const FewArgs a{x, weight, target, row_weight, nullptr, 0, (long)T, (int)V, (int)D, (float)denom, row_loss, dx, nullptr, nullptr};
+    DPPM_TRY((bf16 ? few_classes<false> : few_classes<true>)(few, a, denom > 0, loss_out, dweight, reinterpret_cast<char*>(workspace), as_stream(stream)));
+    return check_launch("dppm_loss_ce_fwd_bwd");
+  }
   const Plan p = plan_of(T, V, D, !bf16, grad, aligned);
   DPPM_REQUIRE(workspace_bytes >= p.total, "dppm_loss_ce_fwd_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
   const hipStream_t st = as_stream(stream);

@@ -148,7 +148,6 @@ __device__ __forceinline__ void tn_product(const TnArgs& g, char* lds, int m0, i
   // The builtin for these reads makes the compiler wait for every global_load_lds in flight first, so they are written out, with their wait:
   // nothing is in flight when the block ends.  The other wave of the SIMD multiplies meanwhile.
   typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
-  typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
   const auto turned4 = [&](tn_frag* out, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, auto pitch) {
     u32x2v r0, r1, r2, r3, r4, r5, r6, r7;
     asm volatile(

@@ -96,6 +96,71 @@ def test_very_many_rows_of_few_classes(ops, dtype):
     check(ops, x, w, y, rw)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,V,D", [(1, 1, 8), (15, 16, 64), (16, 17, 64), (17, 32, 40), (300, 5, 128), (129, 20, 72), (1000, 16, 256), (4097, 31, 248), (65, 17, 256), (513, 7, 512),
+                                   (90, 1, 264), (9001, 2, 8), (70000, 5, 64), (50, 33, 64), (50, 5, 520), (50, 17, 264)])
+def test_few_classes(ops, T, V, D, dtype):
+    """up to 32 classes of up to 512 values go in one pass, every size of it; and the first sizes that do not"""
+    x, w, y, rw = make(T, V, D, dtype, T + V + D)
+    got = check(ops, x, w, y, rw)
+    check(ops, x, w, y, None, 2.5)
+    assert all(torch.equal(a, b) for a, b in zip(got, ops.loss_ce(x.cuda(), w.cuda(), y.cuda(), rw.cuda())))
+    odd = torch.zeros(T * D + 1, dtype=dtype).cuda()[1:].view(T, D).copy_(x)         # not on 16 bytes: in tiles
+    from oracle import classes
+    want = classes.cross_entropy(x, w, y, rw)
+    for a, b, t in zip(ops.loss_ce(odd, w.cuda(), y.cuda(), rw.cuda()), want, bounds(x, w, y, rw, None, want)):
+        assert ((a.cpu().double() - b).abs() <= t).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_classes_non_finite(ops, dtype):
+    x, w, y, rw = make(200, 5, 64, dtype, 12, missing=0.0)
+    clean = ops.loss_ce(x.cuda(), w.cuda(), y.cuda(), rw.cuda(), 200.0)
+    bad = torch.zeros(200, dtype=torch.bool)
+    bad[3] = bad[40] = bad[199] = True
+    x[3], x[40, 5], x[199] = float("inf"), float("nan"), float("-inf")
+    _, row_loss, dx, _ = ops.loss_ce(x.cuda(), w.cuda(), y.cuda(), rw.cuda(), 200.0)
+    assert torch.equal(torch.isfinite(row_loss.cpu()), ~bad) and torch.equal(torch.isfinite(dx.cpu().float()).all(1), ~bad)
+    assert torch.equal(dx.cpu()[~bad], clean[2].cpu()[~bad])
+    y[bad] = torch.tensor([-1, 5, 2 ** 40])              # nothing that such rows hold counts once they have no class
+    rw[bad] = torch.tensor([float("inf"), float("nan"), 1.0])
+    loss, row_loss, dx, dw = ops.loss_ce(x.cuda(), w.cuda(), y.cuda(), rw.cuda(), 200.0)
+    z = x.clone()
+    z[bad] = 0
+    ones = torch.where(bad, torch.ones(()), rw)
+    want = ops.loss_ce(z.cuda(), w.cuda(), y.cuda(), ones.cuda(), 200.0)
+    assert (row_loss[bad.cuda()] == 0).all() and (dx[bad.cuda()] == 0).all()
+    assert all(torch.equal(a, b) for a, b in zip((loss, row_loss, dx, dw), want))
+    none = ops.loss_ce(x.cuda(), w.cuda(), torch.full((200,), -1).cuda())
+    assert none[0].item() == 0 and all((t == 0).all() for t in none)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_classes_in_a_graph(ops, dtype):
+    x, w, y, rw = (t.cuda() for t in make(10000, 6, 48, dtype, 13))
+    eager = ops.loss_ce(x, w, y, rw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.loss_ce(x, w, y, rw)
+    other = make(10000, 6, 48, dtype, 14)
+    for k in range(4):
+        if k == 2:
+            x.copy_(other[0]), y.copy_(other[2])
+            eager = ops.loss_ce(x, w, y, rw)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager)), k
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,V,D", [(9001, 3, 9), (20000, 50, 24), (1_100_003, 3, 9)])
+def test_many_rows_in_tiles(ops, T, V, D, dtype):
+    """rows counted and losses summed by several workgroups; more than 65535 workgroups of the turn"""
+    x, w, y, rw = make(T, V, D, dtype, 15)
+    check(ops, x, w, y, rw)
+
+
 @pytest.mark.parametrize("dtype,T,V", [(F32, 2500, 60000), (BF16, 9000, 131100)])
 def test_several_blocks_of_rows(ops, dtype, T, V):
     """T V over 2^27 (float32) or 2^30 (bfloat16): the rows go in blocks whose parts of dweight add up in float32 (one more u a block, within
