@@ -12,7 +12,7 @@
 //    its 11 bits keep 2^-11 of each down to 2^-14 of the maximum and 2^-25 of the maximum below, so that the only rounding of d that counts
 //    is its own -- and in float32 for float32;
 //  * rows: lse, the rows' losses;
-//  * turn: exponentials to d, rounded once to the operands' type;
+//  * turn: exponentials to n d, rounded once to the operands' type (bfloat16: the own class's entry without loss in dx);
 //  * dx = d W and dW = d^T x: W and d are read transposed from LDS where the contracted dimension is not the contiguous one; x, the smallest,
 //    is transposed in memory, with zeros for rows that have no class.
 // The exponentials held at a time are those of one block of rows, at most 2^30 (bfloat16) or 2^27 (float32) of them: memory does not grow
@@ -304,14 +304,16 @@ __global__ __launch_bounds__(1024) void rows_and_loss_kernel(RowsArgs a, float d
 struct TurnArgs {
   const void* e; long pitch;             // exponentials [rows][pitch]
   const float2* stats; const float* lse; const float* target_score; const int64_t* target; const float* row_weight; const float* inv;
+  float* residual;                       // [rows], P == 1: what the row's own entry lost to bfloat16
   uint16_t* d; long plane;               // [planes][rows, whole tiles of 64][pitch]; in e's place for bfloat16
   int rows, whole, V, strip, across;     // whole: rows, to whole tiles of 64; strip: classes that share a maximum; across: workgroups for the classes
   bool past;                             // d is larger than the caches
 };
 
-// 16 rows x 512 classes a workgroup -- or, where the pitch is 64, 128 rows x 64 --, 8 classes a thread and row: d_tv = e_tv * exp(max_strip - lse_t)
-// * w_t / n, the row's own class from its float32 score.  Rows behind the last (to whole tiles of 64) and without a class are zeros; so are classes
-// behind the last, to the pitch.  P planes of d: 3 for float32; 1 for bfloat16, or 2 for few rows (plan_of).  LANES: threads a row.
+// 16 rows x 512 classes a workgroup -- or, where the pitch is 64, 128 rows x 64 --, 8 classes a thread and row: n d_tv = e_tv * exp(max_strip - lse_t)
+// * w_t, the row's own class from its float32 score.  1 / n is left to the gradients' float32 sums: without weights, the own entry of a class that is
+// not yet likely is then next to -1 and loses nothing in bfloat16.  Rows behind the last (to whole tiles of 64) and without a class are zeros; so are
+// classes behind the last, to the pitch.  P planes of d: 3 for float32; 1 for bfloat16, or 2 for few rows (plan_of).  LANES: threads a row.
 template <bool F32, int P, int LANES>
 __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
   if (blockIdx.x == 0) {                  // one more workgroup, which sums the loss, with the last block of rows
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
     if (t < a.rows) {
       const int64_t y = a.target[t];
       if (y >= 0 && y < a.V) {
-        const float g = (a.row_weight ? a.row_weight[t] : 1.f) * *a.inv;
+        const float g = a.row_weight ? a.row_weight[t] : 1.f;
         if (v < a.V) f = expf(a.stats[(long)(v / a.strip) * a.rows + t].x - a.lse[t]) * g;
         where = (int)y;
         if (k == 0) mine = (expf(a.target_score[t] - a.lse[t]) - 1.f) * g;
@@ -338,6 +340,7 @@ __global__ __launch_bounds__(256) void turn_kernel(TurnArgs a, LossArgs l) {
     }
     factor[k][r] = f;
     if (k == 0) { own[r] = mine; at[r] = where; }
+    if (P == 1 && k == 0 && v0 == 0 && t < a.rows) a.residual[t] = mine - from_bf16(to_bf16(mine));
   }
   __syncthreads();
   const int c = threadIdx.x % LANES * 8, v = v0 + c;
@@ -472,6 +475,8 @@ struct GradOut {
   void* c; long ldc;          // [N][ldc], M values a row
   const float* add;           // float32 [N][ldc] that is added first, or null
   float* part; long part_stride;   // with splits: float32 [splits][N][ldc] instead
+  const float* scale;         // what the products are multiplied with
+  const float* residual; const int64_t* target;    // dx, one plane of d: += residual[n] * A's row of target[n]; or null
   int c_bf16, past, wide;     // past: c is larger than the caches; wide: rows of c start on 16 bytes and M is a multiple of 8
 };
 
@@ -507,7 +512,28 @@ __global__ __launch_bounds__(T::NT) void grad_kernel(TnArgs g, GradOut o) {
   const long steps = (long)g.ksteps * g.pairs;
   tn_acc acc[T::MI][T::NI];
   tn_product<T, TRA, TRB>(g, lds, m0, n0, (int)(steps * split / g.splits), (int)(steps * (split + 1) / g.splits), acc);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (TRA && o.residual && split == 0) {
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      const int n = n0 + (wave / T::WGM) * T::WN + 16 * j + (lane & 15), m = m0 + (wave % T::WGM) * T::WM + 4 * (lane >> 4);
+      const float r = n < g.N ? o.residual[n] : 0.f;
+      const uint16_t* row = g.A + (r != 0.f ? o.target[n] : 0) * g.lda + m;
+      if (r != 0.f) {
+#pragma unroll
+        for (int i = 0; i < T::MI; ++i)
+          if (m + 16 * i < g.M) {        // a row's pitch is a multiple of 64
+            const u32x2 w = *reinterpret_cast<const u32x2*>(row + 16 * i);
+            acc[i][j] += r * tn_acc{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
+          }
+      }
+    }
+  }
+  const float scale = *o.scale;
+#pragma unroll
+  for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) acc[i][j] *= scale;
   const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;
   if (o.c_bf16 && o.wide && !o.part && !o.add) {
 #pragma unroll
@@ -868,7 +894,7 @@ struct Plan {
   int blocks, planes, pairs, tile_scores, strips, strip;
   int counters;                  // workgroups that count rows
   int d_planes, d_pairs;         // of d, and products of pairs of planes in the gradients
-  size_t inv, counts, rparts, stats, lse, tscore, xp, wp, xt, e, d, dw, part, total, part_bytes;
+  size_t inv, counts, rparts, residual, stats, lse, tscore, xp, wp, xt, e, d, dw, part, total, part_bytes;
 };
 
 // Which tile, and how many parts of k: the choice with the shortest time by what one step of 64 in k takes a full chip of workgroups --
@@ -899,10 +925,11 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
   p.f32 = f32; p.grad = grad; p.T = T; p.V = V; p.D = D;
   p.planes = f32 ? 3 : 1;
   p.pairs = f32 ? 6 : 1;
-  // d of bfloat16 inputs: one bfloat16 plane, whose rounding adds to the gradients' error about as much as their own does, or two for few rows,
-  // over which one large entry's rounding does not average out (8 rows, 25840 classes: off by 0.0029 instead of 0.0016 of the gradient; 47 and
-  // 58 us with one plane and with two; 1024 rows, 1024 x 1024: 74 and 80 us, and no more than 1.4 times the plain rounding either way).
-  const bool exact_d = !f32 && T <= 64;
+  // d of bfloat16 inputs: one bfloat16 plane.  A row's own entry is most of its d, and what it loses would add as much to dx as dx's own rounding
+  // does (0.0024 of the gradient in place of 0.0017), so it is held back in float32 and added in dx's epilogue (4099 x 1000, 50001 classes: 1.484 ms
+  // without, 1.498 with it).  In dW it averages out over a class's rows, except where rows are few: there d has two planes (8 rows, 25840
+  // classes: off by 0.0029 with one plane, 0.0016 with two; 47 and 58 us; 100 rows x 512: 78 and 88 us).
+  const bool exact_d = !f32 && T <= 128;
   p.d_planes = f32 ? 3 : exact_d ? 2 : 1;
   p.d_pairs = f32 ? 6 : p.d_planes;
   p.direct = direct && !f32 && D % 64 == 0;
@@ -935,6 +962,7 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
     p.wp = take((size_t)p.planes * V * p.Kp * 2);
   }
   if (grad) {
+    p.residual = take((size_t)p.R * 4);
     p.xt = take((size_t)p.planes * D * p.Rp * 2);
     const size_t held = (size_t)((p.R + 63) / 64 * 64) * p.Vp;
     p.e = take(held * (f32 ? 4 : 2));
@@ -969,9 +997,9 @@ int launch_grad(TnArgs g, const GradOut& o, hipStream_t st) {
 
 // c[n][m] (+= add) = sum_k A[m][k] B[n][k]
 template <bool TRA, bool TRB>
-int grad_product(TnArgs g, void* c, bool c_bf16, const float* add, float* part, size_t part_bytes, hipStream_t st) {
+int grad_product(TnArgs g, void* c, bool c_bf16, const float* scale, const float* residual, const int64_t* target, const float* add, float* part, size_t part_bytes, hipStream_t st) {
   GradOut o{};
-  o.c = c; o.ldc = g.M; o.add = add; o.c_bf16 = c_bf16; o.past = (size_t)g.M * g.N * (c_bf16 ? 2 : 4) > CACHED;
+  o.c = c; o.ldc = g.M; o.scale = scale; o.residual = residual; o.target = target; o.add = add; o.c_bf16 = c_bf16; o.past = (size_t)g.M * g.N * (c_bf16 ? 2 : 4) > CACHED;
   o.wide = g.M % 8 == 0 && (uintptr_t)c % 16 == 0;
   const Shape shape = shape_of(g.M, g.N, (long)g.ksteps * g.pairs, true);
   g.splits = shape.splits;
@@ -1127,7 +1155,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     TurnArgs a{};
     a.e = ws + p.e; a.pitch = p.Vp; a.stats = stats; a.lse = f(p.lse); a.target_score = f(p.tscore); a.target = target + t0;
     a.row_weight = row_weight ? row_weight + t0 : nullptr; a.inv = f(p.inv);
-    a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip; a.past = (size_t)p.d_planes * a.plane * 2 > CACHED;
+    a.residual = f(p.residual); a.d = h(p.d); a.plane = whole * p.Vp; a.rows = (int)rows; a.V = (int)V; a.strip = p.strip; a.past = (size_t)p.d_planes * a.plane * 2 > CACHED;
     const bool last = b == p.blocks - 1;
     const LossArgs sum{parts, sums, (float)denom, last ? loss_out : nullptr};
     const int lanes = p.Vp <= 64 && p.d_planes != 2 ? 8 : 64;
@@ -1149,13 +1177,13 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     gx.A = wp; gx.lda = p.Kp; gx.plane_a = V * p.Kp; gx.M = (int)D;
     gx.B = a.d; gx.ldb = p.Vp; gx.plane_b = a.plane; gx.N = (int)rows;
     gx.K = (int)V; gx.ksteps = cdiv(V, 64); gx.pairs = p.d_pairs;
-    DPPM_TRY((grad_product<true, false>(gx, reinterpret_cast<char*>(dx) + t0 * D * es, bf16, nullptr, f(p.part), p.part_bytes, st)));
+    DPPM_TRY((grad_product<true, false>(gx, reinterpret_cast<char*>(dx) + t0 * D * es, bf16, f(p.inv), p.d_planes == 1 ? f(p.residual) : nullptr, target + t0, nullptr, f(p.part), p.part_bytes, st)));
     TnArgs gw{};       // dW[v][d] = sum_t d[t][v] x^T[d][t]
     gw.A = h(p.xt); gw.lda = Rp; gw.plane_a = D * Rp; gw.M = (int)D;
     gw.B = a.d; gw.ldb = p.Vp; gw.plane_b = a.plane; gw.N = (int)V;
     gw.K = whole; gw.ksteps = cdiv(rows, 64); gw.pairs = p.d_pairs;      // d has zeros to whole steps
     float* total = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
-    DPPM_TRY((grad_product<false, true>)(gw, last || p.f32 ? dweight : (void*)total, bf16 && last, b == 0 ? nullptr : total, f(p.part), p.part_bytes, st));
+    DPPM_TRY((grad_product<false, true>)(gw, last || p.f32 ? dweight : (void*)total, bf16 && last, f(p.inv), nullptr, nullptr, b == 0 ? nullptr : total, f(p.part), p.part_bytes, st));
   }
   if (!grad && T > 8) hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, LossArgs{parts, sums, (float)denom, loss_out});
   return check_launch("dppm_loss_ce_fwd_bwd");
