@@ -4,7 +4,8 @@
 // Both are HBM-bound.  The lookup reads and writes each row once, 16 bytes a lane.  The gradient sorts the positions by class (a stable
 // radix sort of (class, position) pairs), so that the rows of one class lie together and are summed in the order of their positions in
 // float32 registers: no atomics, the same bits from call to call, and one write per row of dW.  A class with many positions is split over
-// fixed chunks of the sorted order, whose partial rows a second launch joins, again in order.
+// fixed chunks of the sorted order, whose partial rows a second launch joins, again in order.  Small tables need no sorting: their sums lie in
+// LDS (embed_small_kernel).
 #include "dppm_common.h"
 
 namespace dppm {
@@ -434,6 +435,109 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, long chunks)
   }
 }
 
+// ------------------------------------------------------------------------------------------------ small tables
+// A table of few classes needs no sorting: every thread holds the sums of all classes over its VEC columns in LDS, [class][thread] -- free of bank
+// conflicts whatever the classes are -- and walks its rows in order.  Class V is the bin of rows without one.  Sums begin with -0, which no
+// addition tells from nothing: a sum that still is -0 at the end had no position (or only zeros of that sign).
+struct SmallArgs {
+  const void* dout; const int64_t* ids; float* part;       // part: [workgroups][V][D]
+  long T, per;                                             // per: rows of a workgroup
+  int V, D, lanes_log2, slices;
+};
+// VEC values as they lie in memory: float32, or bfloat16 by twos
+template <bool IBF, int VEC> struct Raw { typedef float type __attribute__((ext_vector_type(VEC))); };
+template <> struct Raw<true, 4> { typedef u32x2 type; };
+template <> struct Raw<true, 2> { typedef uint32_t type; };
+template <> struct Raw<true, 1> { typedef uint16_t type; };
+template <bool IBF, int VEC>
+__device__ __forceinline__ auto values_of(typename Raw<IBF, VEC>::type w) {
+  typedef float vec __attribute__((ext_vector_type(VEC)));
+  if constexpr (!IBF) return w;
+  else if constexpr (VEC == 4) return vec{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
+  else if constexpr (VEC == 2) return vec{bf16_lo(w), bf16_hi(w)};
+  else return vec(bf16_lo(w));
+}
+template <bool IBF, int VEC>
+__global__ __launch_bounds__(256) void embed_small_kernel(SmallArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float sums[];       // [V + 1][256][VEC]
+  typedef float vec __attribute__((ext_vector_type(VEC)));
+  typedef typename Raw<IBF, VEC>::type raw;
+  vec* const mine = reinterpret_cast<vec*>(sums) + threadIdx.x;
+  const int lanes = 1 << a.lanes_log2, streams = 256 >> a.lanes_log2;
+  const long block = blockIdx.x / a.slices, r0 = block * a.per, r1 = r0 + a.per < a.T ? r0 + a.per : a.T;
+  const int c = ((int)(blockIdx.x % a.slices) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
+  for (int v = 0; v <= a.V; ++v) mine[v * 256] = vec(-0.f);
+  constexpr int AHEAD = 8;
+  if (c < a.D) {
+    long id[AHEAD];
+    raw x[AHEAD];
+    const auto fetch = [&](long t0) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const long t = t0 + u * streams, r = t < r1 ? t : r1 - 1;
+        id[u] = ((glb<const int64_t>)a.ids)[r];
+        x[u] = *(glb<const raw>)((glb<const char>)a.dout + (r * a.D + c) * (IBF ? 2 : 4));
+      }
+      __builtin_amdgcn_sched_barrier(0);         // all of them on their way before the first is looked at
+    };
+    long t0 = r0 + (threadIdx.x >> a.lanes_log2);
+    if (t0 < r1) fetch(t0);
+    while (t0 < r1) {
+      int now[AHEAD];
+      raw y[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        now[u] = (t0 + u * streams < r1 && id[u] >= 0 && id[u] < a.V ? (int)id[u] : a.V) * 256;
+        y[u] = x[u];
+      }
+      t0 += AHEAD * streams;
+      if (t0 < r1) fetch(t0);
+#pragma unroll
+      for (int u = 0; u < AHEAD; u += 2) {       // two at a time, so that the second need not wait for the first's way through LDS
+        const vec first = mine[now[u]] + values_of<IBF, VEC>(y[u]), second = mine[now[u + 1]];
+        mine[now[u]] = first;
+        mine[now[u + 1]] = (now[u] == now[u + 1] ? first : second) + values_of<IBF, VEC>(y[u + 1]);
+      }
+    }
+  }
+  __syncthreads();
+  if (c >= a.D) return;
+  const vec* const all = reinterpret_cast<const vec*>(sums) + (threadIdx.x & (lanes - 1));
+#pragma unroll 4
+  for (int v = threadIdx.x >> a.lanes_log2; v < a.V; v += streams) {
+    vec sum = all[v * 256];
+    for (int q = 1; q < streams; ++q) sum += all[v * 256 + q * lanes];
+    *(glb<vec>)((glb<float>)a.part + (block * a.V + v) * a.D + c) = sum;
+  }
+}
+
+// 64 values a workgroup, 16 threads each over the parts
+template <bool OBF>
+__global__ __launch_bounds__(1024) void embed_small_join_kernel(const float* __restrict__ part, int parts, long n, float scale, int accumulate, void* __restrict__ dw) {
+  __shared__ float w[16][64];
+  const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const long k = (long)blockIdx.x * 64 + c;
+  float s = -0.f;
+  if (k < n) {
+#pragma unroll 8
+    for (int p = q; p < parts; p += 16) s += part[p * n + k];
+  }
+  w[q][c] = s;
+  __syncthreads();
+  if (q || k >= n) return;
+  for (int p = 1; p < 16; ++p) s += w[p][c];
+  const bool none = __float_as_uint(s) == 0x80000000u;
+  if (none && accumulate) return;
+  s = none ? 0.f : s * scale;
+  if constexpr (OBF) {
+    const glb<uint16_t> to = (glb<uint16_t>)dw + k;
+    *to = to_bf16(accumulate ? bf16_lo(*to) + s : s);
+  } else {
+    const glb<float> to = (glb<float>)dw + k;
+    *to = accumulate ? *to + s : s;
+  }
+}
+
 __global__ __launch_bounds__(256) void embed_zero_kernel(uint16_t* __restrict__ p, long halves) {   // a gradient without positions
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < halves; i += (long)gridDim.x * 256) p[i] = 0;
 }
@@ -460,6 +564,42 @@ Layout layout_of(long T, long V, long D) {
   L.part = take((size_t)L.chunks * 2 * L.pitch * 4);
   L.total = at;
   return L;
+}
+
+// The rule for small tables.  A thread takes as many columns (4, 2, 1) as leave its sums of all classes room in LDS.  Times in us, sorted and so:
+// 2^20 x 64 bfloat16, 5 classes 129 and 34 (31 at a copy's rate); 65536 x 512 float32, 38 classes 49 and 32, 60 classes 48 and 40; 1000 x 16, 2 classes 15
+// and 7.  One column a thread reads memory too slowly for large inputs (262144 x 128, 100 classes 61 and 56; 262144 x 512, 150 classes 189 and
+// 246), and the parts of a large table take longer than its sorting (200 x 2048, 140 classes 16 and 26; 2000 x 2048, 60 classes 22 and 26).
+struct SmallPlan { bool fits; int vec, lanes_log2, slices, blocks; long per; size_t lds, total; };
+SmallPlan small_plan(long T, long V, long D, bool fours) {
+  SmallPlan p{};
+  const long room = 156 << 10;
+  p.vec = 1;
+  while (fours && p.vec < 4 && (V + 1) * 2048 * p.vec <= room) p.vec *= 2;
+  p.fits = T >= 1 && (V + 1) * 1024 <= room && V * D <= (1L << 17) && (p.vec > 1 || V < 78 || T * D <= (1L << 25));
+  if (!p.fits) return p;
+  const long per_row = D / p.vec;
+  p.lanes_log2 = log2_ceil(per_row) < 8 ? log2_ceil(per_row) : 8;
+  p.slices = (int)((per_row + (1 << p.lanes_log2) - 1) >> p.lanes_log2);
+  p.lds = (size_t)(V + 1) * 1024 * p.vec;
+  long each = (160 << 10) / (long)p.lds;                     // workgroups of a CU
+  each = each < 1 ? 1 : each > 8 ? 8 : each;
+  // workgroups for the rows: their parts' way through memory (8 bytes a value, 4.6 TB/s) against the steps of a thread, 0.15 us each
+  const double steps = (double)T / (256 >> p.lanes_log2);
+  long blocks = (long)sqrt(0.15 * 4.6e6 * steps / (8.0 * V * D));
+  if (blocks > 256 * each / p.slices) blocks = 256 * each / p.slices;
+  if (blocks > (long)steps / 8) blocks = (long)steps / 8;
+  if (blocks < 1) blocks = 1;
+  p.per = (T + blocks - 1) / blocks;
+  p.blocks = (int)((T + p.per - 1) / p.per);
+  p.total = (size_t)p.blocks * V * D * 4;
+  return p;
+}
+template <bool IBF, int VEC>
+int launch_small(const SmallArgs& a, const SmallPlan& p, hipStream_t st) {
+  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(embed_small_kernel<IBF, VEC>), (int)p.lds, "dppm_embedding_wgrad"));
+  hipLaunchKernelGGL((embed_small_kernel<IBF, VEC>), dim3((unsigned)(p.blocks * p.slices)), dim3(256), p.lds, st, a);
+  return DPPM_OK;
 }
 
 template <bool IBF, bool OBF, int VEC>
@@ -505,7 +645,9 @@ extern "C" int dppm_embedding_fwd(const void* weight, int bf16, const int64_t* i
 
 extern "C" size_t dppm_embedding_wgrad_workspace_bytes(int64_t T, int64_t V, int64_t D) {
   if (T < 1 || V < 1 || D < 1 || T >= (1L << 31) || V >= (1L << 31) || D > (1L << 21)) return 0;
-  return layout_of(T, V, D).total;
+  const size_t sorted = layout_of(T, V, D).total, ones = small_plan(T, V, D, false).total, fours = D % 4 == 0 ? small_plan(T, V, D, true).total : 0;
+  const size_t small = ones > fours ? ones : fours;
+  return sorted > small ? sorted : small;      // the largest, so that the size does not depend on types and addresses
 }
 
 extern "C" int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64_t* ids, float scale, void* dweight, int dweight_bf16, int accumulate,
@@ -526,6 +668,17 @@ extern "C" int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64
   DPPM_REQUIRE(workspace_bytes >= L.total, "dppm_embedding_wgrad: workspace of %zu bytes, %zu needed", workspace_bytes, L.total);
   DPPM_REQUIRE((uintptr_t)workspace % 16 == 0, "dppm_embedding_wgrad: the workspace must be 16-byte aligned");
   char* ws = reinterpret_cast<char*>(workspace);
+  const SmallPlan few = small_plan(T, V, D, D % 4 == 0 && (uintptr_t)dout % (dout_bf16 ? 8 : 16) == 0);
+  if (few.fits && workspace_bytes >= few.total) {
+    const SmallArgs a{dout, ids, reinterpret_cast<float*>(ws), (long)T, few.per, (int)V, (int)D, few.lanes_log2, few.slices};
+    if (dout_bf16) DPPM_TRY(few.vec == 4 ? (launch_small<true, 4>(a, few, st)) : few.vec == 2 ? (launch_small<true, 2>(a, few, st)) : (launch_small<true, 1>(a, few, st)));
+    else DPPM_TRY(few.vec == 4 ? (launch_small<false, 4>(a, few, st)) : few.vec == 2 ? (launch_small<false, 2>(a, few, st)) : (launch_small<false, 1>(a, few, st)));
+    const long n = V * D;
+    const dim3 grid((unsigned)((n + 63) / 64)), block(1024);
+    if (dweight_bf16) hipLaunchKernelGGL((embed_small_join_kernel<true>), grid, block, 0, st, a.part, few.blocks, n, scale, accumulate, dweight);
+    else hipLaunchKernelGGL((embed_small_join_kernel<false>), grid, block, 0, st, a.part, few.blocks, n, scale, accumulate, dweight);
+    return check_launch("dppm_embedding_wgrad");
+  }
   SortBufs b;
   for (int i = 0; i < 2; ++i) {
     b.key[i] = reinterpret_cast<uint32_t*>(ws + L.key[i]);

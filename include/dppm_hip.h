@@ -277,7 +277,7 @@ int dppm_embedding_fwd(const void* weight, int bf16, const int64_t* ids, float s
 
 /* Its gradient: dweight[v][:] = scale * sum over t with ids[t] = v of dout[t][:], every row written (zero without a position); with
  * accumulate != 0 it is added to dweight and rows without a position stay as they are.  dout [T][D], dweight [V][D], each float32 or
- * bfloat16; sums in float32, in the order of t within chunks of the sorted positions: the same bits from call to call.
+ * bfloat16; sums in float32 in a fixed order: the same bits from call to call.
  * T, V < 2^31, D <= 2^21.  workspace: dppm_embedding_wgrad_workspace_bytes(T, V, D), 16-byte aligned (0 bytes: invalid sizes). */
 size_t dppm_embedding_wgrad_workspace_bytes(int64_t T, int64_t V, int64_t D);
 int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64_t* ids, float scale, void* dweight, int dweight_bf16, int accumulate,
@@ -288,8 +288,8 @@ int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64_t* ids, fl
  *   s = x weight^T;  row_loss[t] = log sum_v exp s[t][v] - s[t][target[t]];  *loss_out = sum_t row_weight[t] row_loss[t] / denom;
  *   dx = d weight, dweight = d^T x with d[t][v] = (softmax(s[t])[v] - [v = target[t]]) row_weight[t] / denom.
  * A row whose target lies outside [0, V) has no class: its row_loss and its row of dx are zero and it adds nothing else.  row_weight
- * (nullable) [T]; denom: 1e-37 .. 1e37, or 0, which
- * stands for the number of rows that have a class (1 if none has).  loss_out: one float; row_loss [T] float32.
+ * (nullable) [T]; denom: 1e-37 .. 1e37, or 0, which stands for the number of rows that have a class (1 if none has).  loss_out: one float;
+ * row_loss [T] float32.
  * dx [T][D] and dweight [V][D], in the inputs' type and overwritten, are both given or both NULL.  bfloat16: products of bfloat16 operands
  * (d is rounded to bfloat16 once, from exponentials held in half precision), sums in float32.  float32: operands split into three bfloat16 pieces, float32-grade products
  * (DPPM_PREC_F32X6).  The same bits from call to call.  T < 2^30, V <= 2^23, D <= 2^16.

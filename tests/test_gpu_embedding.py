@@ -169,3 +169,67 @@ def test_refusals(ops):
         with pytest.raises(e):
             f()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("T,V,D", [(1, 1, 1), (7, 2, 1), (2049, 1, 3), (5000, 5, 7), (3001, 38, 64), (3001, 39, 64), (2500, 77, 16), (2500, 78, 16), (2000, 155, 10), (2000, 156, 10),
+                                   (300, 64, 2048), (300, 64, 2052), (600000, 100, 60), (777, 5, 300), (60, 3, 2052),
+                                   (5, 9, 1025), (70000, 5, 64), (33000, 2, 512), (9000, 30, 128)])
+def test_small_tables(ops, T, V, D):
+    """tables whose sums lie in LDS, their first and last sizes, aligned and not, with rows added to and left alone"""
+    rng = np.random.default_rng(T + 3 * V + D)
+    ids = classes_of(rng, T, V, "padded")
+    if V > 2:
+        ids[ids == 1] = 0                              # class 1 never occurs
+    for dtype in (F32, BF16):
+        dout = torch.as_tensor(rng.normal(size=(T, D)).astype(np.float32)).to(dtype)
+        want, mag, n = sums(dout, ids, V)
+        s = float(np.float32(0.7))
+        odd = torch.zeros(T * D + 1, dtype=dtype).cuda()[1:].view(T, D).copy_(dout)
+        for rows in (dout.cuda(), odd):
+            for out_type in (F32, BF16):
+                out = torch.full((V, D), 5.0).to(out_type).cuda()
+                got = ops.embedding_wgrad(rows, ids.cuda(), V, scale=0.7, out=out)
+                tol = (n + 1) * U32 * mag * s + (U32 + (U16 if out_type == BF16 else 0)) * (want * s).abs() * 1.01 + 1e-38
+                assert ((got.cpu().double() - want * s).abs() <= tol).all()
+                assert torch.equal(ops.embedding_wgrad(rows, ids.cuda(), V, scale=0.7, out=torch.empty_like(out)), got)
+                old = torch.as_tensor(rng.normal(size=(V, D)).astype(np.float32)).to(out_type)
+                if V > 2:
+                    old[1] = -0.0
+                    old[1, 0] = float("nan")
+                more = ops.embedding_wgrad(rows, ids.cuda(), V, scale=0.7, out=old.clone().cuda(), accumulate=True).cpu()
+                present = n.squeeze(1) > 0
+                bits = torch.int32 if out_type == F32 else torch.int16
+                assert torch.equal(more[~present].view(bits), old[~present].view(bits))          # left as they are, to the bit
+                total = old.double() + want * s
+                tol = tol + 2 * U32 * total.abs() + (U16 if out_type == BF16 else 0) * total.abs()
+                assert ((more.double() - total).abs() <= tol)[present].all()
+
+
+def test_small_tables_of_zeros(ops):
+    """sums that are -0, and an infinite scale, for rows that do not occur"""
+    dout = torch.full((40, 8), -0.0).cuda()
+    ids = torch.full((40,), 2).cuda()
+    got = ops.embedding_wgrad(dout, ids, 4, scale=float("inf"))
+    assert (got[[0, 1, 3]] == 0).all()
+    old = torch.full((4, 8), -0.0).cuda()
+    ops.embedding_wgrad(dout, ids, 4, out=old, accumulate=True)
+    assert torch.equal(old.cpu().view(torch.int32), torch.full((4, 8), -0.0).view(torch.int32))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_small_tables_in_a_graph(ops, dtype):
+    ids = torch.randint(-1, 6, (30000,)).cuda()
+    dout = torch.randn(30000, 48).to(dtype).cuda()
+    eager = ops.embedding_wgrad(dout, ids, 6)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.embedding_wgrad(dout, ids, 6)
+    for k in range(4):
+        if k == 2:
+            dout.mul_(2)
+            ids.copy_(ids.flip(0))
+            eager = ops.embedding_wgrad(dout, ids, 6)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager), k
