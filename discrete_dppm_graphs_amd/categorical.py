@@ -37,8 +37,12 @@ class _ClassLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         dx, dweight = ctx.saved_tensors
-        return (dx * g.to(dx.dtype) if ctx.needs_input_grad[0] else None, dweight * g.to(dweight.dtype) if ctx.needs_input_grad[1] else None,
-                None, None, None)
+        return (_times(dx, g) if ctx.needs_input_grad[0] else None, _times(dweight, g) if ctx.needs_input_grad[1] else None, None, None, None)
+
+
+def _times(t, g):
+    """t * g with the float32 scalar g as it is: a product in bfloat16 would round g, too"""
+    return t * g if t.dtype is torch.float32 else (t.float() * g).to(t.dtype)
 
 
 def loss_func_ce(x, weight, target, row_weight=None, denom=None):

@@ -55,6 +55,17 @@ def test_lookup_layer_loss_and_step_together():
             assert np.abs(w.detach().cpu().double().numpy().ravel() - p).max() <= 64 * U * 1e-2 * 10 + 4 * U * np.abs(p).max()
 
 
+def test_bfloat16_gradients_take_the_incoming_one_unrounded():
+    from discrete_dppm_graphs_amd import ops
+    from discrete_dppm_graphs_amd.categorical import loss_func_ce
+    x, w, y = torch.randn(70, 40).bfloat16().cuda(), torch.randn(90, 40).bfloat16().cuda(), torch.randint(0, 90, (70,)).cuda()
+    _, _, dx, dw = ops.loss_ce(x, w, y)
+    x.requires_grad_(True), w.requires_grad_(True)
+    (loss_func_ce(x, w, y) * 0.3).backward()
+    assert torch.equal(x.grad, (dx.double() * float(np.float32(0.3))).float().bfloat16())      # 8 + 24 bits are exact in float64; float32, then bfloat16
+    assert torch.equal(w.grad, (dw.double() * float(np.float32(0.3))).float().bfloat16())
+
+
 def test_gradients_scale_with_the_incoming_one_and_stop_where_not_wanted():
     from discrete_dppm_graphs_amd.categorical import embedding, loss_func_ce
     torch.manual_seed(1)
