@@ -4,8 +4,8 @@
 // Both are HBM-bound.  The lookup reads and writes each row once, 16 bytes a lane.  The gradient sorts the positions by class (a stable
 // radix sort of (class, position) pairs), so that the rows of one class lie together and are summed in the order of their positions in
 // float32 registers: no atomics, the same bits from call to call, and one write per row of dW.  A class with many positions is split over
-// fixed chunks of the sorted order, whose partial rows a second launch joins, again in order.  Small tables need no sorting: their sums lie in
-// LDS (embed_small_kernel).
+// fixed chunks of the sorted order, whose partial rows a second launch joins, again in order.  Small tables and few positions need no sorting
+// (embed_small_kernel, embed_range_kernel).
 #include "dppm_common.h"
 
 namespace dppm {
@@ -439,6 +439,21 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, long chunks)
 // A table of few classes needs no sorting: every thread holds the sums of all classes over its VEC columns in LDS, [class][thread] -- free of bank
 // conflicts whatever the classes are -- and walks its rows in order.  Class V is the bin of rows without one.  Sums begin with -0, which no
 // addition tells from nothing: a sum that still is -0 at the end had no position (or only zeros of that sign).
+// dW's value k from its sum
+struct Target { void* dw; int bf16, accumulate; float scale; };
+__device__ __forceinline__ void finish_value(const Target& t, long k, float sum) {
+  const bool none = __float_as_uint(sum) == 0x80000000u;
+  if (none && t.accumulate) return;
+  const float s = none ? 0.f : sum * t.scale;
+  if (t.bf16) {
+    const glb<uint16_t> to = (glb<uint16_t>)t.dw + k;
+    *to = to_bf16(t.accumulate ? bf16_lo(*to) + s : s);
+  } else {
+    const glb<float> to = (glb<float>)t.dw + k;
+    *to = t.accumulate ? *to + s : s;
+  }
+}
+
 struct SmallArgs {
   const void* dout; const int64_t* ids; float* part;       // part: [workgroups][V][D]
   long T, per;                                             // per: rows of a workgroup
@@ -511,31 +526,103 @@ __global__ __launch_bounds__(256) void embed_small_kernel(SmallArgs a) {
   }
 }
 
-// 64 values a workgroup, 16 threads each over the parts
-template <bool OBF>
-__global__ __launch_bounds__(1024) void embed_small_join_kernel(const float* __restrict__ part, int parts, long n, float scale, int accumulate, void* __restrict__ dw) {
-  __shared__ float w[16][64];
-  const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
-  const long k = (long)blockIdx.x * 64 + c;
+// Few positions of a table that is not small: a workgroup takes 16 classes, up to `per` positions and 16 threads' columns.  It first lists those of its
+// positions that have one of its classes -- in order, a wave's quarter after the other's --, then sums their rows as above, 16 streams of
+// them.  No sorting, and no more than per / 16 rows in a thread's way whatever the classes are.
+constexpr int RANGE = 16, RANGE_MOST = 1280, RANGE_LANES = 16;      // a list entry: 12 bits of the position, 4 of the class
+template <bool IBF, int VEC>
+__global__ __launch_bounds__(256) void embed_range_kernel(SmallArgs a, int groups, Target t) {
+  extern __shared__ __attribute__((aligned(16))) float sums[];       // [RANGE + 1][256][VEC]
+  __shared__ uint16_t list[RANGE_MOST];
+  __shared__ int found[4];
+  typedef float vec __attribute__((ext_vector_type(VEC)));
+  typedef typename Raw<IBF, VEC>::type raw;
+  vec* const mine = reinterpret_cast<vec*>(sums) + threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int slice = blockIdx.x % a.slices, rest = blockIdx.x / a.slices, group = rest % groups;
+  const long block = rest / groups, r0 = block * a.per;
+  const int n = (int)(r0 + a.per < a.T ? a.per : a.T - r0), quarter = (n + 3) / 4, v0 = group * RANGE, most = a.V - v0 < RANGE ? a.V - v0 : RANGE;
+  const int c = (slice * RANGE_LANES + (threadIdx.x & (RANGE_LANES - 1))) * VEC;
+  {
+    uint16_t* const own = list + wave * quarter;
+    const int end = (wave + 1) * quarter < n ? (wave + 1) * quarter : n;
+    int count = 0;
+    constexpr int AHEAD = 4;
+    for (int t0 = wave * quarter + lane; t0 - lane < end; t0 += 64 * AHEAD) {
+      long id[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) id[u] = t0 + 64 * u < end ? ((glb<const int64_t>)a.ids)[r0 + t0 + 64 * u] : -1;
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const bool in = id[u] >= v0 && id[u] < v0 + most;
+        const uint64_t all = __ballot(in);
+        if (in) own[count + __popcll(all & ((1ull << lane) - 1ull))] = (uint16_t)((t0 + 64 * u) << 4 | (int)(id[u] - v0));
+        count += __popcll(all);
+      }
+    }
+    if (lane == 0) found[wave] = count;
+  }
+  __syncthreads();
+  const int f0 = found[0], f1 = f0 + found[1], f2 = f1 + found[2], total = f2 + found[3];
+  constexpr int AHEAD = 8, STREAMS = 256 / RANGE_LANES;
+  if (total) {
+#pragma unroll
+    for (int v = 0; v <= RANGE; ++v) mine[v * 256] = vec(-0.f);
+  }
+  for (int k0 = threadIdx.x / RANGE_LANES; c < a.D && k0 < total; k0 += AHEAD * STREAMS) {
+    int at[AHEAD];
+    raw x[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = k0 + u * STREAMS < total ? k0 + u * STREAMS : k0;
+      const int w = (k >= f0) + (k >= f1) + (k >= f2), begin = w == 0 ? 0 : w == 1 ? f0 : w == 2 ? f1 : f2;
+      const uint32_t entry = list[w * quarter + k - begin];
+      at[u] = (k0 + u * STREAMS < total ? (int)(entry & 15u) : RANGE) * 256;
+      x[u] = *(glb<const raw>)((glb<const char>)a.dout + ((r0 + (entry >> 4)) * a.D + c) * (IBF ? 2 : 4));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; u += 2) {
+      const vec first = mine[at[u]] + values_of<IBF, VEC>(x[u]), second = mine[at[u + 1]];
+      mine[at[u]] = first;
+      mine[at[u + 1]] = (at[u] == at[u + 1] ? first : second) + values_of<IBF, VEC>(x[u + 1]);
+    }
+  }
+  __syncthreads();
+  const int v = threadIdx.x / RANGE_LANES;
+  if (v >= most || c >= a.D) return;
+  const vec* const all = reinterpret_cast<const vec*>(sums) + v * 256 + (threadIdx.x & (RANGE_LANES - 1));
+  vec sum = vec(-0.f);
+  if (total) {
+#pragma unroll
+    for (int q = 0; q < STREAMS; ++q) sum += all[q * RANGE_LANES];
+  }
+  if (t.dw) {                // the only part
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) finish_value(t, (long)(v0 + v) * a.D + c + k, sum[k]);
+  } else
+    *(glb<vec>)((glb<float>)a.part + (block * a.V + v0 + v) * a.D + c) = sum;
+}
+
+// Q threads a value over the parts: 16, or 1 for few parts
+template <int Q>
+__global__ __launch_bounds__(1024) void embed_small_join_kernel(const float* __restrict__ part, int parts, long n, Target t) {
+  constexpr int C = 1024 / Q;
+  __shared__ float w[Q][C];
+  const int c = threadIdx.x % C, q = threadIdx.x / C;
+  const long k = (long)blockIdx.x * C + c;
   float s = -0.f;
   if (k < n) {
 #pragma unroll 8
-    for (int p = q; p < parts; p += 16) s += part[p * n + k];
+    for (int p = q; p < parts; p += Q) s += part[p * n + k];
   }
-  w[q][c] = s;
-  __syncthreads();
+  if constexpr (Q > 1) {
+    w[q][c] = s;
+    __syncthreads();
+  }
   if (q || k >= n) return;
-  for (int p = 1; p < 16; ++p) s += w[p][c];
-  const bool none = __float_as_uint(s) == 0x80000000u;
-  if (none && accumulate) return;
-  s = none ? 0.f : s * scale;
-  if constexpr (OBF) {
-    const glb<uint16_t> to = (glb<uint16_t>)dw + k;
-    *to = to_bf16(accumulate ? bf16_lo(*to) + s : s);
-  } else {
-    const glb<float> to = (glb<float>)dw + k;
-    *to = accumulate ? *to + s : s;
-  }
+  for (int p = 1; p < Q; ++p) s += w[p][c];
+  finish_value(t, k, s);
 }
 
 __global__ __launch_bounds__(256) void embed_zero_kernel(uint16_t* __restrict__ p, long halves) {   // a gradient without positions
@@ -595,6 +682,35 @@ SmallPlan small_plan(long T, long V, long D, bool fours) {
   p.total = (size_t)p.blocks * V * D * 4;
   return p;
 }
+// embed_range_kernel: with no more positions than leave a workgroup 1280 when there are two workgroups a CU (72 KB of LDS), and no more than 2500
+// workgroups.  Classes as a language has them / all positions in one class, float32, sorted and so, in us: 300 x 128, 1000 classes 18 / 17 and 6 / 8; 5003
+// x 128, 1000 classes 24 / 26 and 14 / 21; 1000 x 256, 8000 classes 27 / 27 and 16 / 16.  With 2000 positions a workgroup: 4000 x 250, 1000
+// classes 24 / 29 and 29 / 53; with 4000 workgroups: 1280 x 1000, 4000 classes 28 / 30 and 34 / 20.
+struct RangePlan { bool fits; int vec, slices, groups, blocks; long per; size_t total; };
+RangePlan range_plan(long T, long V, long D, bool fours) {
+  RangePlan p{};
+  if (T < 1) return p;
+  p.vec = fours ? 4 : 1;
+  p.slices = cdiv(D, RANGE_LANES * p.vec);
+  p.groups = cdiv(V, RANGE);
+  const long each = (long)p.slices * p.groups, room = 512 / each, most = room < 1 ? 1 : room;
+  p.fits = T <= RANGE_MOST * most && each <= 2500;
+  if (!p.fits) return p;
+  long blocks = T / 256 < most ? T / 256 : most;            // 256 positions are not worth a part of their own
+  if (blocks < 1) blocks = 1;
+  p.per = (T + blocks - 1) / blocks;
+  p.blocks = (int)((T + p.per - 1) / p.per);
+  p.total = (size_t)p.blocks * V * D * 4;
+  return p;
+}
+template <bool IBF, int VEC>
+int launch_range(const SmallArgs& a, const RangePlan& p, const Target& t, hipStream_t st) {
+  constexpr size_t LDS = (RANGE + 1) * 1024 * VEC;
+  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(embed_range_kernel<IBF, VEC>), LDS, "dppm_embedding_wgrad"));
+  hipLaunchKernelGGL((embed_range_kernel<IBF, VEC>), dim3((unsigned)(p.blocks * p.groups * p.slices)), dim3(256), LDS, st, a, p.groups, p.blocks == 1 ? t : Target{});
+  return DPPM_OK;
+}
+
 template <bool IBF, int VEC>
 int launch_small(const SmallArgs& a, const SmallPlan& p, hipStream_t st) {
   DPPM_TRY(lds_limit(reinterpret_cast<const void*>(embed_small_kernel<IBF, VEC>), (int)p.lds, "dppm_embedding_wgrad"));
@@ -646,8 +762,10 @@ extern "C" int dppm_embedding_fwd(const void* weight, int bf16, const int64_t* i
 extern "C" size_t dppm_embedding_wgrad_workspace_bytes(int64_t T, int64_t V, int64_t D) {
   if (T < 1 || V < 1 || D < 1 || T >= (1L << 31) || V >= (1L << 31) || D > (1L << 21)) return 0;
   const size_t sorted = layout_of(T, V, D).total, ones = small_plan(T, V, D, false).total, fours = D % 4 == 0 ? small_plan(T, V, D, true).total : 0;
-  const size_t small = ones > fours ? ones : fours;
-  return sorted > small ? sorted : small;      // the largest, so that the size does not depend on types and addresses
+  const size_t ones_r = range_plan(T, V, D, false).total, fours_r = D % 4 == 0 ? range_plan(T, V, D, true).total : 0;
+  size_t most = sorted;
+  for (const size_t n : {ones, fours, ones_r, fours_r}) most = n > most ? n : most;
+  return most;      // the largest, so that the size does not depend on types and addresses
 }
 
 extern "C" int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64_t* ids, float scale, void* dweight, int dweight_bf16, int accumulate,
@@ -665,18 +783,31 @@ extern "C" int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64
   }
   DPPM_REQUIRE(dout && ids && workspace, "dppm_embedding_wgrad: null pointer");
   const Layout L = layout_of(T, V, D);
-  DPPM_REQUIRE(workspace_bytes >= L.total, "dppm_embedding_wgrad: workspace of %zu bytes, %zu needed", workspace_bytes, L.total);
+  const size_t need = dppm_embedding_wgrad_workspace_bytes(T, V, D);
+  DPPM_REQUIRE(workspace_bytes >= need, "dppm_embedding_wgrad: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   DPPM_REQUIRE((uintptr_t)workspace % 16 == 0, "dppm_embedding_wgrad: the workspace must be 16-byte aligned");
   char* ws = reinterpret_cast<char*>(workspace);
-  const SmallPlan few = small_plan(T, V, D, D % 4 == 0 && (uintptr_t)dout % (dout_bf16 ? 8 : 16) == 0);
-  if (few.fits && workspace_bytes >= few.total) {
-    const SmallArgs a{dout, ids, reinterpret_cast<float*>(ws), (long)T, few.per, (int)V, (int)D, few.lanes_log2, few.slices};
-    if (dout_bf16) DPPM_TRY(few.vec == 4 ? (launch_small<true, 4>(a, few, st)) : few.vec == 2 ? (launch_small<true, 2>(a, few, st)) : (launch_small<true, 1>(a, few, st)));
-    else DPPM_TRY(few.vec == 4 ? (launch_small<false, 4>(a, few, st)) : few.vec == 2 ? (launch_small<false, 2>(a, few, st)) : (launch_small<false, 1>(a, few, st)));
+  const bool fours = D % 4 == 0 && (uintptr_t)dout % (dout_bf16 ? 8 : 16) == 0;
+  const SmallPlan small = small_plan(T, V, D, fours);
+  const RangePlan range = range_plan(T, V, D, fours);
+  if (small.fits || range.fits) {
+    SmallArgs a{dout, ids, reinterpret_cast<float*>(ws), (long)T, small.per, (int)V, (int)D, small.lanes_log2, small.slices};
+    const Target t{dweight, dweight_bf16, accumulate, scale};
+    int parts = small.blocks;
+    if (small.fits) {
+      if (dout_bf16) DPPM_TRY(small.vec == 4 ? (launch_small<true, 4>(a, small, st)) : small.vec == 2 ? (launch_small<true, 2>(a, small, st)) : (launch_small<true, 1>(a, small, st)));
+      else DPPM_TRY(small.vec == 4 ? (launch_small<false, 4>(a, small, st)) : small.vec == 2 ? (launch_small<false, 2>(a, small, st)) : (launch_small<false, 1>(a, small, st)));
+    } else {
+      a.per = range.per; a.slices = range.slices;
+      parts = range.blocks;
+      if (dout_bf16) DPPM_TRY(range.vec == 4 ? (launch_range<true, 4>(a, range, t, st)) : (launch_range<true, 1>(a, range, t, st)));
+      else DPPM_TRY(range.vec == 4 ? (launch_range<false, 4>(a, range, t, st)) : (launch_range<false, 1>(a, range, t, st)));
+    }
     const long n = V * D;
-    const dim3 grid((unsigned)((n + 63) / 64)), block(1024);
-    if (dweight_bf16) hipLaunchKernelGGL((embed_small_join_kernel<true>), grid, block, 0, st, a.part, few.blocks, n, scale, accumulate, dweight);
-    else hipLaunchKernelGGL((embed_small_join_kernel<false>), grid, block, 0, st, a.part, few.blocks, n, scale, accumulate, dweight);
+    if (small.fits || parts > 1) {
+      if (parts <= 8) hipLaunchKernelGGL((embed_small_join_kernel<1>), dim3((unsigned)((n + 1023) / 1024)), dim3(1024), 0, st, a.part, parts, n, t);
+      else hipLaunchKernelGGL((embed_small_join_kernel<16>), dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st, a.part, parts, n, t);
+    }
     return check_launch("dppm_embedding_wgrad");
   }
   SortBufs b;

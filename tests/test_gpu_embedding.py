@@ -205,6 +205,46 @@ def test_small_tables(ops, T, V, D):
                 assert ((more.double() - total).abs() <= tol)[present].all()
 
 
+@pytest.mark.parametrize("kind", ["uniform", "skewed", "one", "padded", "none"])
+@pytest.mark.parametrize("T,V,D", [(1, 200, 8), (255, 200, 4), (257, 300, 20), (3000, 156, 64), (4096, 1000, 65), (5003, 1000, 128), (1280, 4096, 64), (1281, 4096, 64), (1280, 4097, 64),
+                                   (8191, 300, 33), (8192, 160, 60), (100000, 157, 5), (655360, 159, 1), (8193, 160, 60), (700, 40000, 1), (700, 40001, 1), (20, 60000, 16), (900, 161, 130)])
+def test_few_positions(ops, T, V, D, kind):
+    """rows that are listed and not sorted, by one workgroup for a class or several; and the first sizes beyond"""
+    rng = np.random.default_rng(T + 5 * V + D + len(kind))
+    ids = classes_of(rng, T, V, kind)
+    d32 = torch.as_tensor(rng.normal(size=(T, D)).astype(np.float32))
+    for din, dw in ((F32, F32), (BF16, BF16), (F32, BF16)):
+        d = d32.to(din)
+        want, mag, n = sums(d, ids, V)
+        out = torch.full((V, D), 7.0, dtype=dw, device="cuda")
+        got = ops.embedding_wgrad(d.cuda(), ids.cuda(), V, scale=0.37, out=out).cpu().double()
+        sc = float(np.float32(0.37))
+        tol = (n + 1) * U32 * mag * sc
+        tol = tol + (U16 * (want * sc).abs() + U16 * tol if dw == BF16 else 0)
+        assert ((got - want * sc).abs() <= tol).all(), (din, dw)
+        assert torch.equal(ops.embedding_wgrad(d.cuda(), ids.cuda(), V, scale=0.37, out=torch.empty_like(out)), out)
+        start = torch.as_tensor(rng.normal(size=(V, D)).astype(np.float32)).to(dw)
+        start[::3] = -0.0
+        more = ops.embedding_wgrad(d.cuda(), ids.cuda(), V, out=start.clone().cuda(), accumulate=True).cpu()
+        absent = (n == 0).squeeze(1)
+        bits = torch.int32 if dw == F32 else torch.int16
+        assert torch.equal(more[absent].view(bits), start[absent].view(bits))
+        total = start.double() + want
+        tol = (n + 2) * U32 * (mag + start.double().abs())
+        tol = tol + (U16 * (total.abs() + tol) if dw == BF16 else 0)
+        assert ((more.double() - total).abs() <= tol).all()
+
+
+def test_few_positions_nan_stays_in_its_class(ops):
+    d = torch.ones(3000, 40).cuda()
+    ids = (torch.arange(3000) % 400).cuda()
+    d[5], d[406] = float("nan"), float("inf")
+    got = ops.embedding_wgrad(d, ids, 410)
+    bad = torch.zeros(410, dtype=torch.bool)
+    bad[5] = bad[6] = True
+    assert torch.equal(torch.isfinite(got.cpu()).all(1), ~bad) and (got[400:] == 0).all()
+
+
 def test_small_tables_of_zeros(ops):
     """sums that are -0, and an infinite scale, for rows that do not occur"""
     dout = torch.full((40, 8), -0.0).cuda()
