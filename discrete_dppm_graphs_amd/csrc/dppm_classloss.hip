@@ -593,7 +593,7 @@ __global__ __launch_bounds__(256) void parts_kernel(PartsJob x, PartsJob w, int 
 }
 
 // ------------------------------------------------------------------------------------------------ few classes
-// Up to 32 classes of up to 512 values: all of W lies in LDS and a row's scores in the registers of four lanes, so that one pass over x gives the
+// Up to 16 classes of 512 values, 32 of 256, 64 of 128, 128 of 64: all of W lies in LDS and a row's scores in the registers of four lanes, so that one pass over x gives the
 // losses, dx and each workgroup's part of dW, and neither scores nor d reach memory.  x is read twice (the second time from the caches), dx
 // written once.  A wave takes 16 rows at a time, in three products on the matrix cores:
 //   s = W x^T    k = dims: lane i + 16 g holds row i, dims 32 step + 8 g .. + 7 (16 or 32 bytes of x); out come classes 4 g .. 4 g + 3 of row i,
@@ -610,7 +610,7 @@ struct FewArgs {
   float* part; RowsPart* parts;                    // [workgroups][V][D], [workgroups]
 };
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-constexpr int FEW_CLASSES = 32, FEW_VALUES = 512;  // (padded classes / 16) * padded D at most FEW_VALUES: dW fits in 128 registers
+constexpr int FEW_CLASSES = 128, FEW_VALUES = 512;  // (padded classes / 16) * padded D at most FEW_VALUES: dW fits in 128 registers
 
 template <bool F32>
 __device__ __forceinline__ void load8(const void* x, long at, float (&v)[8]) {
@@ -634,7 +634,7 @@ __device__ __forceinline__ f32x4 load4(const void* x, long at) {
 
 // CT: sixteens of classes, NC: sixty-fours of dims
 template <bool F32, int CT, int NC>
-__global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : 2) void few_kernel(FewArgs a) {
+__global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ __attribute__((aligned(16))) float turned[4][CT][16][20];
   __shared__ RowsPart sums[4];
@@ -766,13 +766,14 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : 2) void few_kernel(FewArgs 
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<f32x4*>(&turned[wave][ct][i][4 * g]) = p[ct];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    u32x4 plane[2];      // bfloat16: d in two planes, class 4 g + j of the first sixteen, then of the second
+    constexpr int PAIRS = (CT + 1) / 2;
+    u32x4 plane[2][PAIRS];      // bfloat16: d in two planes, class 4 g + j of each sixteen, by pairs of sixteens
     if (!F32) {
       f32x4 rest[CT];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
+        for (int ct = 0; ct < 2 * PAIRS; ++ct)
 #pragma unroll
           for (int j = 0; j < 4; j += 2) {
             uint32_t w = 0;
@@ -781,7 +782,7 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : 2) void few_kernel(FewArgs 
               w = pack_bf16(lo, hi);
               if (k == 0) { rest[ct][j] = lo - __uint_as_float(w << 16); rest[ct][j + 1] = hi - __uint_as_float(w & 0xffff0000u); }
             }
-            plane[k][2 * ct + j / 2] = w;
+            plane[k][ct / 2][2 * (ct & 1) + j / 2] = w;
           }
     }
 #pragma unroll 1
@@ -794,10 +795,12 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : 2) void few_kernel(FewArgs 
           const uint16_t* w = hc + (((2 * st + u) * 16 + i) * 4 + g) * CT * 4;
 #pragma unroll
           for (int k = 1; k >= 0; --k) {
-            if constexpr (CT == 2)
-              o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const tn_frag*>(w), __builtin_bit_cast(tn_frag, plane[k]), o[u], 0, 0, 0);
+            if constexpr (CT == 1)
+              o[u] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(*reinterpret_cast<const s16x4*>(w), __builtin_bit_cast(s16x4, u32x2{plane[k][0].x, plane[k][0].y}), o[u], 0, 0, 0);
             else
-              o[u] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(*reinterpret_cast<const s16x4*>(w), __builtin_bit_cast(s16x4, u32x2{plane[k].x, plane[k].y}), o[u], 0, 0, 0);
+#pragma unroll
+              for (int h = 0; h < PAIRS; ++h)
+                o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const tn_frag*>(w + 8 * h), __builtin_bit_cast(tn_frag, plane[k][h]), o[u], 0, 0, 0);
           }
         } else
 #pragma unroll
@@ -819,7 +822,8 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : 2) void few_kernel(FewArgs 
       }
     }
     const uint32_t have = (uint32_t)__ballot(counts);    // bit i: row i; what a row without a class holds is not looked at
-#pragma unroll
+    constexpr int TOGETHER = F32 && CT == 6 ? 2 : 4;     // (fours spill there)
+#pragma unroll TOGETHER
     for (int k = 0; k < 4; ++k) {
       const int row = 4 * k + g;
       const bool has = have >> row & 1;
@@ -1072,11 +1076,12 @@ int gradients(GradJob x, GradJob w, float* part, size_t part_bytes, hipStream_t 
 
 // few_kernel: the rule on sizes, and its workspace.  Losses and gradients in one pass and by the products in tiles, which pad the classes to 128 and
 // hold x^T, scores and d in memory, bfloat16 / float32: 2^20 rows x 64, 5 classes 87 / 137 us and 443 / 1289 (60 / 118 at a copy's rate); at its largest
-// sizes, 2^16 x 512, 16 classes 57 / 90 and 98 / 350, 300 x 256, 32 classes 20 / 24 and 35 / 68.
+// sizes, 2^16 x 512, 16 classes 57 / 90 and 98 / 350, x 128, 64 classes 42 / 67 and 58 / 113, x 64, 128 classes 61 / 71 and 65 / 117 (losses alone 20 / 29
+// and 17 / 40); 1000 x 64, 100 classes 20 / 24 and 33 / 47.
 struct FewPlan { bool fits; int ct, nc, grid, counters; size_t counts, parts, part, total; };
 FewPlan few_plan(long T, long V, long D, bool grad) {
   FewPlan f{};
-  f.ct = V <= 16 ? 1 : 2;
+  f.ct = V <= 16 ? 1 : V <= 32 ? 2 : V <= 64 ? 4 : V <= 96 ? 6 : 8;
   f.nc = D <= 64 ? 1 : D <= 128 ? 2 : D <= 256 ? 4 : 8;
   f.fits = V <= FEW_CLASSES && D % 8 == 0 && D <= FEW_VALUES && f.ct * f.nc * 64 <= FEW_VALUES;
   if (!f.fits) return f;
@@ -1107,11 +1112,17 @@ int few_classes(const FewPlan& f, FewArgs a, bool denominator, float* loss, void
     else if (f.nc == 2) DPPM_TRY((launch_few<F32, 1, 2>(a, f.grid, st)));
     else if (f.nc == 4) DPPM_TRY((launch_few<F32, 1, 4>(a, f.grid, st)));
     else DPPM_TRY((launch_few<F32, 1, 8>(a, f.grid, st)));
-  } else {
+  } else if (f.ct == 2) {
     if (f.nc == 1) DPPM_TRY((launch_few<F32, 2, 1>(a, f.grid, st)));
     else if (f.nc == 2) DPPM_TRY((launch_few<F32, 2, 2>(a, f.grid, st)));
     else DPPM_TRY((launch_few<F32, 2, 4>(a, f.grid, st)));
-  }
+  } else if (f.ct == 4) {
+    if (f.nc == 1) DPPM_TRY((launch_few<F32, 4, 1>(a, f.grid, st)));
+    else DPPM_TRY((launch_few<F32, 4, 2>(a, f.grid, st)));
+  } else if (f.ct == 6)
+    DPPM_TRY((launch_few<F32, 6, 1>(a, f.grid, st)));
+  else
+    DPPM_TRY((launch_few<F32, 8, 1>(a, f.grid, st)));
   const int n = a.dx ? a.V * a.D : 0;
   hipLaunchKernelGGL(few_join_kernel, dim3(1 + cdiv(n, 64)), dim3(1024), 0, st, a.part, f.grid, n, dweight, (int)!F32, LossArgs{a.parts, f.grid, a.denom, loss});
   return DPPM_OK;

@@ -98,9 +98,10 @@ def test_very_many_rows_of_few_classes(ops, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("T,V,D", [(1, 1, 8), (15, 16, 64), (16, 17, 64), (17, 32, 40), (300, 5, 128), (129, 20, 72), (1000, 16, 256), (4097, 31, 248), (65, 17, 256), (513, 7, 512),
-                                   (90, 1, 264), (9001, 2, 8), (70000, 5, 64), (50, 33, 64), (50, 5, 520), (50, 17, 264)])
+                                   (90, 1, 264), (9001, 2, 8), (70000, 5, 64), (50, 33, 64), (50, 5, 520), (50, 17, 264),
+                                   (700, 64, 128), (3001, 50, 96), (300, 64, 136), (700, 128, 64), (5003, 100, 48), (300, 129, 64), (300, 65, 72)])
 def test_few_classes(ops, T, V, D, dtype):
-    """up to 32 classes of up to 512 values go in one pass, every size of it; and the first sizes that do not"""
+    """few classes go in one pass, every size of it (16 classes of 512 values to 128 of 64); and the first sizes that do not"""
     x, w, y, rw = make(T, V, D, dtype, T + V + D)
     got = check(ops, x, w, y, rw)
     check(ops, x, w, y, None, 2.5)
