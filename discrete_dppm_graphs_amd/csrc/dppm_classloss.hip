@@ -900,7 +900,7 @@ __global__ __launch_bounds__(1024) void few_join_kernel(const float* __restrict_
 // ------------------------------------------------------------------------------------------------ host
 using Wide = TnTile<256, 256, 2, 4, 2>;
 using Mid = TnTile<128, 128, 2, 2, 2>;
-using Narrow = TnTile<64, 32, 2, 1, 4>;     // few rows: many small workgroups that stream W
+using Narrow = TnTile<64, 32, 2, 1, 4>;     // scores of few rows or few tiles: many small workgroups
 
 constexpr long CUS = 256;
 // Elements between rows of a buffer of this file's own: whole lines of 64, an odd number of them, so that the rows of a tile do not all start in
@@ -916,11 +916,18 @@ struct Plan {
   size_t inv, counts, rparts, residual, stats, lse, tscore, xp, wp, xt, e, d, dw, part, total, part_bytes;
 };
 
-// Which tile: the one with the shorter time by what one step of 64 in k takes a full chip of workgroups -- 1.15 us for 256 x 256 tiles (one
-// a CU), 0.95 us for 128 x 128 ones (two a CU) -- times rounds of workgroups.
-bool wide_scores(long M, long N, long steps) {
-  const auto us = [&](long t, long slots, double step) { return (double)((cdiv(M, t) * (long)cdiv(N, t) + slots - 1) / slots) * (double)steps * step; };
-  return us(256, CUS, 1.15) < us(128, 2 * CUS, 0.95);
+// Which tile for the scores (0: 256 x 256, 1: 128 x 128, 2: 64 x 32): the one with the shortest time by what one step of 64 in k takes a full chip of
+// workgroups -- 1.15 us for one a CU, 0.95 for two, 0.48 for three --, what a round of tiles takes besides, and rounds of workgroups.  The smallest are
+// for what would leave CUs without a tile (the whole loss in float32, with 128 x 128 and so: 256 x 2000, 1000 classes 220 and 125 us; 4000 x 512, 500
+// classes 121 and 113; 1000 x 256, 5000 classes 113 and 129).
+int tile_for_scores(long rows, long V, long steps) {
+  if (rows <= 32) return 2;      // W streams through once either way: 64 x 32 tiles have it on every CU
+  const auto us = [&](long m, long n, long each, double step, double round) {
+    return (double)((cdiv(V, m) * (long)cdiv(rows, n) + each * CUS - 1) / (each * CUS)) * ((double)steps * step + round);
+  };
+  const double t[3] = {us(256, 256, 1, 1.15, 8.0), us(128, 128, 2, 0.95, 6.0), us(64, 32, 3, 0.48, 1.2) + 3.0};
+  const int least = t[1] < t[0] ? 1 : 0;
+  return t[2] < t[least] ? 2 : least;
 }
 
 // Tiles of both gradients, and how many parts of k each is cut to: by the time of one launch that deals out the longer tiles first, a step of 64
@@ -957,11 +964,6 @@ Shape shape_of(const Gradients& g) {
   return best;
 }
 size_t part_bytes_of(const Shape& s, const Gradients& g) { return ((s.x > 1 ? (size_t)s.x * g.rows : 0) + (s.w > 1 ? (size_t)s.w * g.V : 0)) * g.D * 4; }
-int tile_for_scores(long rows, long V, long steps) {
-  if (rows <= 32) return 2;      // W streams through once either way: 64 x 32 tiles have it on every CU
-  return wide_scores(V, rows, steps) ? 0 : 1;
-}
-
 Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
   Plan p{};
   p.f32 = f32; p.grad = grad; p.T = T; p.V = V; p.D = D;
