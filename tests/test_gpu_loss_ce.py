@@ -90,6 +90,21 @@ def test_tiles_of_256(ops, T, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,V,D", [(1001, 5003, 200), (4099, 1201, 100), (901, 4600, 264)])
+def test_tiles_of_128(ops, T, V, D, dtype):
+    """sizes whose scores are cut into 128 x 128 tiles, with ragged edges"""
+    x, w, y, rw = make(T, V, D, dtype, 16)
+    check(ops, x, w, y, rw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,V,D", [(2060, 2300, 2056), (600, 2300, 2050)])
+def test_gradients_by_whole_and_cut_tiles_of_256(ops, T, V, D, dtype):
+    x, w, y, rw = make(T, V, D, dtype, 17)
+    check(ops, x, w, y, rw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_very_many_rows_of_few_classes(ops, dtype):
     """more than 65535 workgroups of 16 rows"""
     x, w, y, rw = make(1_100_003, 3, 8, dtype, 9)
