@@ -593,9 +593,9 @@ __global__ __launch_bounds__(256) void parts_kernel(PartsJob x, PartsJob w, int 
 }
 
 // ------------------------------------------------------------------------------------------------ few classes
-// Up to 16 classes of 512 values, 32 of 256, 64 of 128, 128 of 64: all of W lies in LDS and a row's scores in the registers of four lanes, so that one pass over x gives the
-// losses, dx and each workgroup's part of dW, and neither scores nor d reach memory.  x is read twice (the second time from the caches), dx
-// written once.  A wave takes 16 rows at a time, in three products on the matrix cores:
+// Up to 16 classes of 512 values, 32 of 256, 64 of 128, 128 of 64: all of W lies in LDS and a row's scores in the registers of four lanes, so that
+// one pass over x gives the losses, dx and each workgroup's part of dW, and neither scores nor d reach memory.  x is read twice (the second
+// time from the caches), dx written once.  A wave takes 16 rows at a time, in three products on the matrix cores:
 //   s = W x^T    k = dims: lane i + 16 g holds row i, dims 32 step + 8 g .. + 7 (16 or 32 bytes of x); out come classes 4 g .. 4 g + 3 of row i,
 //   dx^T = W^T d k = classes: those four are the operand as they stand; out come the same dims of row i as were read,
 //   dW += d x    k = rows: d turned in LDS, x read again with a lane's four dims of row 4 t + g.
@@ -612,28 +612,53 @@ struct FewArgs {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr int FEW_CLASSES = 128, FEW_VALUES = 512;  // (padded classes / 16) * padded D at most FEW_VALUES: dW fits in 128 registers
 
-template <bool F32>
-__device__ __forceinline__ void load8(const void* x, long at, float (&v)[8]) {
-  if (F32) {
-    const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x) + at);
-    const f32x4 a = p[0], b = p[1];
+// N (4 or 8) values of a row of D from dim d on, zeros behind the last (with N = 4 and WIDE, the caller sees to that): float32 as they are, bfloat16 by
+// twos.  WIDE: D is a multiple of 8 and rows are aligned to 16 bytes.
+template <bool F32, int N> struct Few;
+template <int N> struct Few<true, N> { float v[N]; };
+template <int N> struct Few<false, N> { uint32_t v[N / 2]; };
+template <bool F32, bool WIDE, int N>
+__device__ __forceinline__ Few<F32, N> load_few(const void* x, long row, int d, int D) {
+  Few<F32, N> r;
+  if constexpr (WIDE) {
+    const long at = row * D + (d < D ? d : 0);
+    if constexpr (F32) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x) + at);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+      for (int h = 0; h < N / 4; ++h) {
+        const f32x4 w = p[h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.v[4 * h + e] = w[e];
+      }
+    } else if constexpr (N == 8) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(x) + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.v[e] = w[e];
+    } else {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint16_t*>(x) + at);
+      r.v[0] = w.x;
+      r.v[1] = w.y;
+    }
+    if (N == 8 && d >= D) r = Few<F32, N>{};
   } else {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(x) + at);
+    const long at = row * D;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+    for (int e = 0; e < N; ++e) {
+      const int k = d + e < D ? d + e : 0;
+      if constexpr (F32) {
+        const float w = reinterpret_cast<const float*>(x)[at + k];
+        r.v[e] = d + e < D ? w : 0.f;
+      } else {
+        const uint32_t w = d + e < D ? reinterpret_cast<const uint16_t*>(x)[at + k] : 0u;
+        r.v[e / 2] = e & 1 ? r.v[e / 2] | w << 16 : w;
+      }
+    }
   }
-}
-template <bool F32>
-__device__ __forceinline__ f32x4 load4(const void* x, long at) {
-  if (F32) return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(x) + at);
-  const u32x2 w = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint16_t*>(x) + at);
-  return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
+  return r;
 }
 
 // CT: sixteens of classes, NC: sixty-fours of dims
-template <bool F32, int CT, int NC>
+template <bool F32, bool WIDE, int CT, int NC>
 __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ __attribute__((aligned(16))) float turned[4][CT][16][20];
@@ -645,26 +670,19 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   for (int k = threadIdx.x; k < 16 * CT * 8 * NC; k += 256) {
     const int v = k / (8 * NC), d = k % (8 * NC) * 8, st = d / 32, o = d % 32 / 8, ct = v / 16, c = v % 16;
-    const bool in = v < a.V && d < a.D;
-    const long from = in ? (long)v * a.D + d : 0;
+    const Few<F32, 8> w = load_few<F32, WIDE, 8>(a.weight, v < a.V ? v : 0, v < a.V ? d : a.D, a.D);
     if constexpr (F32) {
-      float w[8];
-      load8<F32>(a.weight, from, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = in ? w[e] : 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int at = (2 * st + u) * CT + ct;
-        *reinterpret_cast<f32x4*>(wk + (at * 16 + c) * 16 + 4 * o) = f32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
+        *reinterpret_cast<f32x4*>(wk + (at * 16 + c) * 16 + 4 * o) = f32x4{w.v[4 * u], w.v[4 * u + 1], w.v[4 * u + 2], w.v[4 * u + 3]};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) wc[(at * 16 + 4 * o + e) * 16 + c] = w[4 * u + e];
+        for (int e = 0; e < 4; ++e) wc[(at * 16 + 4 * o + e) * 16 + c] = w.v[4 * u + e];
       }
     } else {
-      u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.weight) + from);
-      if (!in) w = u32x4{0u, 0u, 0u, 0u};
-      *reinterpret_cast<u32x4*>(hk + ((st * CT + ct) * 16 + c) * 32 + 8 * o) = w;
+      *reinterpret_cast<u32x4*>(hk + ((st * CT + ct) * 16 + c) * 32 + 8 * o) = u32x4{w.v[0], w.v[1], w.v[2], w.v[3]};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) hc[((((2 * st + e / 4) * 16 + 4 * o + e % 4) * 4 + c / 4) * CT + ct) * 4 + c % 4] = (uint16_t)(w[e / 2] >> e % 2 * 16);
+      for (int e = 0; e < 8; ++e) hc[((((2 * st + e / 4) * 16 + 4 * o + e % 4) * 4 + c / 4) * CT + ct) * 4 + c % 4] = (uint16_t)(w.v[e / 2] >> e % 2 * 16);
     }
   }
   float inv = 0.f;
@@ -680,7 +698,7 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
 #pragma unroll
       for (int e = 0; e < 4; ++e) dw[ct][c][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   RowsPart mine{0.0, 0u, 0u};
-  constexpr int AHEAD = NC == 1 ? 2 : 4;                 // steps of 32 dims that are read together
+  constexpr int AHEAD = NC == 1 || !WIDE ? 2 : 4;                 // steps of 32 dims that are read together
   const int steps = (a.D + 31) / 32;
   for (long t0 = ((long)blockIdx.x * 4 + wave) * 16; t0 < a.T; t0 += (long)gridDim.x * 64) {
     const long t = t0 + i < a.T ? t0 + i : a.T - 1;      // rows behind the last repeat it and count for nothing
@@ -690,41 +708,26 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) s[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; 32 * s0 < a.D; s0 += AHEAD) {
-      if constexpr (F32) {
-        float v[AHEAD][8];
+      Few<F32, 8> v[AHEAD];
 #pragma unroll
-        for (int h = 0; h < AHEAD; ++h) {
-          const int d = 32 * (s0 + h) + 8 * g;
-          load8<F32>(a.x, t * a.D + (d < a.D ? d : 0), v[h]);
-          if (d >= a.D) {
+      for (int h = 0; h < AHEAD; ++h) v[h] = load_few<F32, WIDE, 8>(a.x, t, 32 * (s0 + h) + 8 * g, a.D);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[h][e] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < AHEAD; ++h)
+      for (int h = 0; h < AHEAD; ++h) {
+        if constexpr (F32) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
               const f32x4 w = *reinterpret_cast<const f32x4*>(wk + (((2 * (s0 + h) + u) * CT + ct) * 16 + i) * 16 + 4 * g);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], v[h][4 * u + e], s[ct], 0, 0, 0);
+              for (int e = 0; e < 4; ++e) s[ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], v[h].v[4 * u + e], s[ct], 0, 0, 0);
             }
-      } else {
-        u32x4 v[AHEAD];
-#pragma unroll
-        for (int h = 0; h < AHEAD; ++h) {
-          const int d = 32 * (s0 + h) + 8 * g;
-          v[h] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.x) + t * a.D + (d < a.D ? d : 0));
-          if (d >= a.D) v[h] = u32x4{0u, 0u, 0u, 0u};
-        }
-#pragma unroll
-        for (int h = 0; h < AHEAD; ++h)
+        } else {
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct)
             s[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const tn_frag*>(hk + (((s0 + h) * CT + ct) * 16 + i) * 32 + 8 * g),
                                                             __builtin_bit_cast(tn_frag, v[h]), s[ct], 0, 0, 0);
+        }
       }
     }
     float top = -INFINITY;
@@ -812,7 +815,14 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
       }
       const int d = 32 * st + 8 * g;
       if (in && d < a.D) {
-        if (F32) {
+        if constexpr (!WIDE) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (d + e < a.D) {
+              if (F32) reinterpret_cast<float*>(a.dx)[t * a.D + d + e] = o[e / 4][e % 4];
+              else reinterpret_cast<uint16_t*>(a.dx)[t * a.D + d + e] = to_bf16(o[e / 4][e % 4]);
+            }
+        } else if (F32) {
           f32x4* to = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.dx) + t * a.D + d);
           to[0] = o[0];
           to[1] = o[1];
@@ -822,20 +832,22 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
       }
     }
     const uint32_t have = (uint32_t)__ballot(counts);    // bit i: row i; what a row without a class holds is not looked at
-    constexpr int TOGETHER = F32 && CT == 6 ? 2 : 4;     // (fours spill there)
+    constexpr int TOGETHER = (F32 && CT == 6) || (!WIDE && CT * NC == 8) ? 2 : 4;     // (fours spill there)
 #pragma unroll TOGETHER
     for (int k = 0; k < 4; ++k) {
       const int row = 4 * k + g;
       const bool has = have >> row & 1;
-      const long from = (t0 + row < a.T ? t0 + row : a.T - 1) * a.D;
+      const long from = t0 + row < a.T ? t0 + row : a.T - 1;
       float d[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) d[ct] = turned[wave][ct][row][i];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int at = 64 * c + 4 * i;
-        f32x4 v = load4<F32>(a.x, from + (at < a.D ? at : 0));
-        if (!has || at >= a.D) v = f32x4{0.f, 0.f, 0.f, 0.f};
+        const Few<F32, 4> w = load_few<F32, WIDE, 4>(a.x, from, 64 * c + 4 * i, a.D);
+        f32x4 v;
+        if constexpr (F32) v = f32x4{w.v[0], w.v[1], w.v[2], w.v[3]};
+        else v = f32x4{__uint_as_float(w.v[0] << 16), __uint_as_float(w.v[0] & 0xffff0000u), __uint_as_float(w.v[1] << 16), __uint_as_float(w.v[1] & 0xffff0000u)};
+        if (!has || 64 * c + 4 * i >= a.D) v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -1079,13 +1091,13 @@ int gradients(GradJob x, GradJob w, float* part, size_t part_bytes, hipStream_t 
 // few_kernel: the rule on sizes, and its workspace.  Losses and gradients in one pass and by the products in tiles, which pad the classes to 128 and
 // hold x^T, scores and d in memory, bfloat16 / float32: 2^20 rows x 64, 5 classes 87 / 137 us and 443 / 1289 (60 / 118 at a copy's rate); at its largest
 // sizes, 2^16 x 512, 16 classes 57 / 90 and 98 / 350, x 128, 64 classes 42 / 67 and 58 / 113, x 64, 128 classes 61 / 71 and 65 / 117 (losses alone 20 / 29
-// and 17 / 40); 1000 x 64, 100 classes 20 / 24 and 33 / 47.
+// and 17 / 40); 1000 x 64, 100 classes 20 / 24 and 33 / 47.  Rows that are not aligned are read value by value: 2^20 x 63, 5 classes 217 / 313 and 714 / 1463.
 struct FewPlan { bool fits; int ct, nc, grid, counters; size_t counts, parts, part, total; };
 FewPlan few_plan(long T, long V, long D, bool grad) {
   FewPlan f{};
   f.ct = V <= 16 ? 1 : V <= 32 ? 2 : V <= 64 ? 4 : V <= 96 ? 6 : 8;
   f.nc = D <= 64 ? 1 : D <= 128 ? 2 : D <= 256 ? 4 : 8;
-  f.fits = V <= FEW_CLASSES && D % 8 == 0 && D <= FEW_VALUES && f.ct * f.nc * 64 <= FEW_VALUES;
+  f.fits = V <= FEW_CLASSES && D <= FEW_VALUES && f.ct * f.nc * 64 <= FEW_VALUES;
   if (!f.fits) return f;
   const long groups = (T + 63) / 64, most = CUS * (f.ct * f.nc <= 2 ? 4 : 2);
   f.grid = (int)(groups < most ? groups : most);
@@ -1095,14 +1107,14 @@ FewPlan few_plan(long T, long V, long D, bool grad) {
   f.total = f.part + (grad ? (size_t)f.grid * V * D * 4 : 0);
   return f;
 }
-template <bool F32, int CT, int NC>
+template <bool F32, bool WIDE, int CT, int NC>
 int launch_few(const FewArgs& a, int grid, hipStream_t st) {
   constexpr int LDS = NC * CT * (F32 ? 8192 : 4096);
-  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(few_kernel<F32, CT, NC>), LDS, "dppm_loss_ce"));
-  hipLaunchKernelGGL((few_kernel<F32, CT, NC>), dim3(grid), dim3(256), LDS, st, a);
+  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(few_kernel<F32, WIDE, CT, NC>), LDS, "dppm_loss_ce"));
+  hipLaunchKernelGGL((few_kernel<F32, WIDE, CT, NC>), dim3(grid), dim3(256), LDS, st, a);
   return DPPM_OK;
 }
-template <bool F32>
+template <bool F32, bool WIDE>
 int few_classes(const FewPlan& f, FewArgs a, bool denominator, float* loss, void* dweight, char* ws, hipStream_t st) {
   a.counts = reinterpret_cast<uint32_t*>(ws + f.counts);
   a.parts = reinterpret_cast<RowsPart*>(ws + f.parts);
@@ -1110,21 +1122,21 @@ int few_classes(const FewPlan& f, FewArgs a, bool denominator, float* loss, void
   a.counters = denominator ? 0 : f.counters;
   if (a.counters) hipLaunchKernelGGL(count_kernel, dim3(a.counters), dim3(256), 0, st, a.target, a.T, (long)a.V, reinterpret_cast<uint32_t*>(ws + f.counts));
   if (f.ct == 1) {
-    if (f.nc == 1) DPPM_TRY((launch_few<F32, 1, 1>(a, f.grid, st)));
-    else if (f.nc == 2) DPPM_TRY((launch_few<F32, 1, 2>(a, f.grid, st)));
-    else if (f.nc == 4) DPPM_TRY((launch_few<F32, 1, 4>(a, f.grid, st)));
-    else DPPM_TRY((launch_few<F32, 1, 8>(a, f.grid, st)));
+    if (f.nc == 1) DPPM_TRY((launch_few<F32, WIDE, 1, 1>(a, f.grid, st)));
+    else if (f.nc == 2) DPPM_TRY((launch_few<F32, WIDE, 1, 2>(a, f.grid, st)));
+    else if (f.nc == 4) DPPM_TRY((launch_few<F32, WIDE, 1, 4>(a, f.grid, st)));
+    else DPPM_TRY((launch_few<F32, WIDE, 1, 8>(a, f.grid, st)));
   } else if (f.ct == 2) {
-    if (f.nc == 1) DPPM_TRY((launch_few<F32, 2, 1>(a, f.grid, st)));
-    else if (f.nc == 2) DPPM_TRY((launch_few<F32, 2, 2>(a, f.grid, st)));
-    else DPPM_TRY((launch_few<F32, 2, 4>(a, f.grid, st)));
+    if (f.nc == 1) DPPM_TRY((launch_few<F32, WIDE, 2, 1>(a, f.grid, st)));
+    else if (f.nc == 2) DPPM_TRY((launch_few<F32, WIDE, 2, 2>(a, f.grid, st)));
+    else DPPM_TRY((launch_few<F32, WIDE, 2, 4>(a, f.grid, st)));
   } else if (f.ct == 4) {
-    if (f.nc == 1) DPPM_TRY((launch_few<F32, 4, 1>(a, f.grid, st)));
-    else DPPM_TRY((launch_few<F32, 4, 2>(a, f.grid, st)));
+    if (f.nc == 1) DPPM_TRY((launch_few<F32, WIDE, 4, 1>(a, f.grid, st)));
+    else DPPM_TRY((launch_few<F32, WIDE, 4, 2>(a, f.grid, st)));
   } else if (f.ct == 6)
-    DPPM_TRY((launch_few<F32, 6, 1>(a, f.grid, st)));
+    DPPM_TRY((launch_few<F32, WIDE, 6, 1>(a, f.grid, st)));
   else
-    DPPM_TRY((launch_few<F32, 8, 1>(a, f.grid, st)));
+    DPPM_TRY((launch_few<F32, WIDE, 8, 1>(a, f.grid, st)));
   const int n = a.dx ? a.V * a.D : 0;
   hipLaunchKernelGGL(few_join_kernel, dim3(1 + cdiv(n, 64)), dim3(1024), 0, st, a.part, f.grid, n, dweight, (int)!F32, LossArgs{a.parts, f.grid, a.denom, loss});
   return DPPM_OK;
@@ -1162,10 +1174,12 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
   DPPM_REQUIRE((uintptr_t)workspace % 16 == 0, "dppm_loss_ce_fwd_bwd: the workspace must be 16-byte aligned");
   const bool grad = dx != nullptr, aligned = ((uintptr_t)x | (uintptr_t)weight) % 16 == 0;
   const FewPlan few = few_plan(T, V, D, grad);
-  if (few.fits && aligned && (uintptr_t)dx % 16 == 0) {
+  if (few.fits) {
     DPPM_REQUIRE(workspace_bytes >= few.total, "dppm_loss_ce_fwd_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, few.total);
     const FewArgs a{x, weight, target, row_weight, nullptr, 0, (long)T, (int)V, (int)D, (float)denom, row_loss, dx, nullptr, nullptr};
-    DPPM_TRY((bf16 ? few_classes<false> : few_classes<true>)(few, a, denom > 0, loss_out, dweight, reinterpret_cast<char*>(workspace), as_stream(stream)));
+    const bool wide = D % 8 == 0 && aligned && (uintptr_t)dx % 16 == 0;
+    const auto run = bf16 ? (wide ? few_classes<false, true> : few_classes<false, false>) : (wide ? few_classes<true, true> : few_classes<true, false>);
+    DPPM_TRY(run(few, a, denom > 0, loss_out, dweight, reinterpret_cast<char*>(workspace), as_stream(stream)));
     return check_launch("dppm_loss_ce_fwd_bwd");
   }
   const Plan p = plan_of(T, V, D, !bf16, grad, aligned);
