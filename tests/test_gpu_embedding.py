@@ -235,14 +235,37 @@ def test_few_positions(ops, T, V, D, kind):
         assert ((more.double() - total).abs() <= tol).all()
 
 
-def test_few_positions_nan_stays_in_its_class(ops):
-    d = torch.ones(3000, 40).cuda()
-    ids = (torch.arange(3000) % 400).cuda()
-    d[5], d[406] = float("nan"), float("inf")
-    got = ops.embedding_wgrad(d, ids, 410)
-    bad = torch.zeros(410, dtype=torch.bool)
-    bad[5] = bad[6] = True
-    assert torch.equal(torch.isfinite(got.cpu()).all(1), ~bad) and (got[400:] == 0).all()
+@pytest.mark.parametrize("kind", ["uniform", "skewed", "one", "padded", "none"])
+@pytest.mark.parametrize("T,V,D", [(8192, 1000, 512), (5003, 5000, 128), (8192, 60000, 33), (1025, 70001, 40), (8193, 5000, 100), (20001, 9000, 64), (70000, 300000, 4)])
+def test_sorted_positions(ops, T, V, D, kind):
+    """sorted by one workgroup and by tiles, in one pass to three; same checks"""
+    test_few_positions(ops, T, V, D, kind)
+
+
+@pytest.mark.parametrize("T,V,D", [(8000, 9000, 64), (20000, 9000, 64), (900, 9000, 64), (900, 600, 64)])
+def test_gradient_in_a_graph(ops, T, V, D):
+    rng = np.random.default_rng(T)
+    ids, d = classes_of(rng, T, V, "skewed").cuda(), torch.randn(T, D, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dw = ops.embedding_wgrad(d, ids, V, 2.0)
+    for k in range(4):
+        ids.copy_(classes_of(np.random.default_rng(90 + k), T, V, "padded"))
+        d.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dw, ops.embedding_wgrad(d, ids, V, 2.0)), k
+
+
+@pytest.mark.parametrize("T,V", [(3000, 400), (8000, 9000), (20000, 9000)])
+def test_nan_stays_in_its_class(ops, T, V):
+    d = torch.ones(T, 40).cuda()
+    ids = (torch.arange(T) % V).cuda()
+    d[5], d[T - 1] = float("nan"), float("inf")
+    got = ops.embedding_wgrad(d, ids, V + 10)
+    bad = torch.zeros(V + 10, dtype=torch.bool)
+    bad[5] = bad[(T - 1) % V] = True
+    assert torch.equal(torch.isfinite(got.cpu()).all(1), ~bad) and (got[V:] == 0).all()
 
 
 def test_small_tables_of_zeros(ops):
