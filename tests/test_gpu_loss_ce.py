@@ -130,8 +130,9 @@ def test_few_classes(ops, T, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_few_classes_non_finite(ops, dtype):
-    x, w, y, rw = make(200, 5, 64, dtype, 12, missing=0.0)
+@pytest.mark.parametrize("V,D", [(5, 64), (90, 63), (300, 72), (300, 128), (2000, 40)])
+def test_non_finite_rows_with_and_without_a_class(ops, V, D, dtype):
+    x, w, y, rw = make(200, V, D, dtype, 12, missing=0.0)
     clean = ops.loss_ce(x.cuda(), w.cuda(), y.cuda(), rw.cuda(), 200.0)
     bad = torch.zeros(200, dtype=torch.bool)
     bad[3] = bad[40] = bad[199] = True
@@ -139,7 +140,7 @@ def test_few_classes_non_finite(ops, dtype):
     _, row_loss, dx, _ = ops.loss_ce(x.cuda(), w.cuda(), y.cuda(), rw.cuda(), 200.0)
     assert torch.equal(torch.isfinite(row_loss.cpu()), ~bad) and torch.equal(torch.isfinite(dx.cpu().float()).all(1), ~bad)
     assert torch.equal(dx.cpu()[~bad], clean[2].cpu()[~bad])
-    y[bad] = torch.tensor([-1, 5, 2 ** 40])              # nothing that such rows hold counts once they have no class
+    y[bad] = torch.tensor([-1, V, 2 ** 40])              # nothing that such rows hold counts once they have no class
     rw[bad] = torch.tensor([float("inf"), float("nan"), 1.0])
     loss, row_loss, dx, dw = ops.loss_ce(x.cuda(), w.cuda(), y.cuda(), rw.cuda(), 200.0)
     z = x.clone()
