@@ -593,7 +593,7 @@ __global__ __launch_bounds__(256) void parts_kernel(PartsJob x, PartsJob w, int 
 }
 
 // ------------------------------------------------------------------------------------------------ few classes
-// Up to 16 classes of 512 values, 32 of 256, 64 of 128, 128 of 64: all of W lies in LDS and a row's scores in the registers of four lanes, so that
+// Up to 16 classes of 512 values, 32 of 256, 64 of 128, 128 of 64 (of wider rows in two passes, below): all of W lies in LDS and a row's scores in the registers of four lanes, so that
 // one pass over x gives the losses, dx and each workgroup's part of dW, and neither scores nor d reach memory.  x is read twice (the second
 // time from the caches), dx written once.  A wave takes 16 rows at a time, in three products on the matrix cores:
 //   s = W x^T    k = dims: lane i + 16 g holds row i, dims 32 step + 8 g .. + 7 (16 or 32 bytes of x); out come classes 4 g .. 4 g + 3 of row i,
@@ -608,6 +608,7 @@ struct FewArgs {
   long T; int V, D; float denom;
   float* row_loss; void* dx;                       // dx null: losses only
   float* part; RowsPart* parts;                    // [workgroups][V][D], [workgroups]
+  float* d; int slices;                            // in two passes: [T][padded classes]; slices of the dims
 };
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr int FEW_CLASSES = 128, FEW_VALUES = 512;  // (padded classes / 16) * padded D at most FEW_VALUES: dW fits in 128 registers
@@ -657,36 +658,42 @@ __device__ __forceinline__ Few<F32, N> load_few(const void* x, long row, int d, 
   return r;
 }
 
-// CT: sixteens of classes, NC: sixty-fours of dims
-template <bool F32, bool WIDE, int CT, int NC>
-__global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_kernel(FewArgs a) {
+// CT: sixteens of classes, NC: sixty-fours of dims.  Wider rows go in two passes of this kernel: SCORES, whose W has all dims (and one order), leaves d in
+// memory, 64 bytes a row and sixteen classes; GRADIENTS takes a slice of 64 NC dims of x and W a workgroup.
+enum FewPass { ALL, SCORES, GRADIENTS };
+template <bool F32, bool WIDE, int CT, int NC, FewPass PASS>
+__global__ __launch_bounds__(256, PASS == SCORES ? 2 : CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ __attribute__((aligned(16))) float turned[4][CT][16][20];
   __shared__ RowsPart sums[4];
   float* const wk = reinterpret_cast<float*>(lds);       // float32: [slot][ct][class][q]
-  float* const wc = wk + NC * CT * 1024;                 //          [slot][ct][q][class]
+  float* const wc = wk + (PASS == ALL ? NC * CT * 1024 : 0);     //  [slot][ct][q][class]
   uint16_t* const hk = reinterpret_cast<uint16_t*>(lds); // bfloat16: [step][ct][class][dim]
-  uint16_t* const hc = hk + NC * CT * 1024;              //           [slot][q][class / 4][ct][class % 4]
+  uint16_t* const hc = hk + (PASS == ALL ? NC * CT * 1024 : 0);  //   [slot][q][class / 4][ct][class % 4]
+  const int sixty_fours = PASS == SCORES ? (a.D + 127) / 128 * 2 : NC;
+  const int slices = PASS == GRADIENTS ? a.slices : 1, block = blockIdx.x / slices, blocks = gridDim.x / slices, d0 = (blockIdx.x - block * slices) * 64 * NC;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-  for (int k = threadIdx.x; k < 16 * CT * 8 * NC; k += 256) {
-    const int v = k / (8 * NC), d = k % (8 * NC) * 8, st = d / 32, o = d % 32 / 8, ct = v / 16, c = v % 16;
-    const Few<F32, 8> w = load_few<F32, WIDE, 8>(a.weight, v < a.V ? v : 0, v < a.V ? d : a.D, a.D);
+  for (int k = threadIdx.x; k < 16 * CT * 8 * sixty_fours; k += 256) {
+    const int v = k / (8 * sixty_fours), d = k % (8 * sixty_fours) * 8, st = d / 32, o = d % 32 / 8, ct = v / 16, c = v % 16;
+    const Few<F32, 8> w = load_few<F32, WIDE, 8>(a.weight, v < a.V ? v : 0, v < a.V ? d0 + d : a.D, a.D);
     if constexpr (F32) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int at = (2 * st + u) * CT + ct;
-        *reinterpret_cast<f32x4*>(wk + (at * 16 + c) * 16 + 4 * o) = f32x4{w.v[4 * u], w.v[4 * u + 1], w.v[4 * u + 2], w.v[4 * u + 3]};
+        if (PASS != GRADIENTS) *reinterpret_cast<f32x4*>(wk + (at * 16 + c) * 16 + 4 * o) = f32x4{w.v[4 * u], w.v[4 * u + 1], w.v[4 * u + 2], w.v[4 * u + 3]};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) wc[(at * 16 + 4 * o + e) * 16 + c] = w.v[4 * u + e];
+        for (int e = 0; e < 4; ++e)
+          if (PASS != SCORES) wc[(at * 16 + 4 * o + e) * 16 + c] = w.v[4 * u + e];
       }
     } else {
-      *reinterpret_cast<u32x4*>(hk + ((st * CT + ct) * 16 + c) * 32 + 8 * o) = u32x4{w.v[0], w.v[1], w.v[2], w.v[3]};
+      if (PASS != GRADIENTS) *reinterpret_cast<u32x4*>(hk + ((st * CT + ct) * 16 + c) * 32 + 8 * o) = u32x4{w.v[0], w.v[1], w.v[2], w.v[3]};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) hc[((((2 * st + e / 4) * 16 + 4 * o + e % 4) * 4 + c / 4) * CT + ct) * 4 + c % 4] = (uint16_t)(w.v[e / 2] >> e % 2 * 16);
+      for (int e = 0; e < 8; ++e)
+        if (PASS != SCORES) hc[((((2 * st + e / 4) * 16 + 4 * o + e % 4) * 4 + c / 4) * CT + ct) * 4 + c % 4] = (uint16_t)(w.v[e / 2] >> e % 2 * 16);
     }
   }
   float inv = 0.f;
-  if (a.dx)
+  if (PASS != GRADIENTS && a.dx)
     inv = inverse_of<256>(a.denom > 0.f ? 0u : a.counters ? rows_counted<256>(a.counts, a.counters) : rows_with_class<256>(a.target, a.T, a.V), a.denom);
   __syncthreads();
 
@@ -698,74 +705,85 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
 #pragma unroll
       for (int e = 0; e < 4; ++e) dw[ct][c][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   RowsPart mine{0.0, 0u, 0u};
-  constexpr int AHEAD = NC == 1 || !WIDE ? 2 : 4;                 // steps of 32 dims that are read together
-  const int steps = (a.D + 31) / 32;
-  for (long t0 = ((long)blockIdx.x * 4 + wave) * 16; t0 < a.T; t0 += (long)gridDim.x * 64) {
+  constexpr int AHEAD = (NC == 1 && PASS == ALL) || !WIDE ? 2 : 4;                 // steps of 32 dims that are read together
+  const int steps = (a.D - d0 < 64 * NC ? a.D - d0 + 31 : 64 * NC) / 32;
+  for (long t0 = ((long)block * 4 + wave) * 16; t0 < a.T; t0 += (long)blocks * 64) {
     const long t = t0 + i < a.T ? t0 + i : a.T - 1;      // rows behind the last repeat it and count for nothing
     const int64_t y = a.target[t];
     const bool in = t0 + i < a.T, counts = in && y >= 0 && y < a.V;
-    f32x4 s[CT];
+    f32x4 p[CT];                                         // exponentials, then d
+    if constexpr (PASS != GRADIENTS) {
+      f32x4 s[CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) s[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; 32 * s0 < a.D; s0 += AHEAD) {
-      Few<F32, 8> v[AHEAD];
+      for (int ct = 0; ct < CT; ++ct) s[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int s0 = 0; 32 * s0 < a.D; s0 += AHEAD) {
+        Few<F32, 8> v[AHEAD];
 #pragma unroll
-      for (int h = 0; h < AHEAD; ++h) v[h] = load_few<F32, WIDE, 8>(a.x, t, 32 * (s0 + h) + 8 * g, a.D);
+        for (int h = 0; h < AHEAD; ++h) v[h] = load_few<F32, WIDE, 8>(a.x, t, 32 * (s0 + h) + 8 * g, a.D);
 #pragma unroll
-      for (int h = 0; h < AHEAD; ++h) {
-        if constexpr (F32) {
+        for (int h = 0; h < AHEAD; ++h) {
+          if constexpr (F32) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              const f32x4 w = *reinterpret_cast<const f32x4*>(wk + (((2 * (s0 + h) + u) * CT + ct) * 16 + i) * 16 + 4 * g);
+              for (int ct = 0; ct < CT; ++ct) {
+                const f32x4 w = *reinterpret_cast<const f32x4*>(wk + (((2 * (s0 + h) + u) * CT + ct) * 16 + i) * 16 + 4 * g);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], v[h].v[4 * u + e], s[ct], 0, 0, 0);
-            }
-        } else {
+                for (int e = 0; e < 4; ++e) s[ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], v[h].v[4 * u + e], s[ct], 0, 0, 0);
+              }
+          } else {
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            s[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const tn_frag*>(hk + (((s0 + h) * CT + ct) * 16 + i) * 32 + 8 * g),
-                                                            __builtin_bit_cast(tn_frag, v[h]), s[ct], 0, 0, 0);
+            for (int ct = 0; ct < CT; ++ct)
+              s[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const tn_frag*>(hk + (((s0 + h) * CT + ct) * 16 + i) * 32 + 8 * g),
+                                                              __builtin_bit_cast(tn_frag, v[h]), s[ct], 0, 0, 0);
+          }
         }
       }
-    }
-    float top = -INFINITY;
+      float top = -INFINITY;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+      for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (16 * ct + 4 * g + j < a.V) top = fmaxf(top, s[ct][j]);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    float sum = 0.f, own = 0.f;
-    f32x4 p[CT];
+        for (int j = 0; j < 4; ++j)
+          if (16 * ct + 4 * g + j < a.V) top = fmaxf(top, s[ct][j]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      float sum = 0.f, own = 0.f;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+      for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int v = 16 * ct + 4 * g + j;
-        p[ct][j] = v < a.V ? exp_of<F32>(s[ct][j] - top) : 0.f;
-        sum += p[ct][j];
-        if (v == y) own = s[ct][j];
+        for (int j = 0; j < 4; ++j) {
+          const int v = 16 * ct + 4 * g + j;
+          p[ct][j] = v < a.V ? exp_of<F32>(s[ct][j] - top) : 0.f;
+          sum += p[ct][j];
+          if (v == y) own = s[ct][j];
+        }
+      sum += __shfl_xor(sum, 16, 64);
+      own += __shfl_xor(own, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      own += __shfl_xor(own, 32, 64);
+      const float loss = counts ? top + logf(sum) - own : 0.f;
+      const float weight = counts && a.row_weight ? a.row_weight[t] : 1.f;
+      if (g == 0) {
+        if (in) a.row_loss[t] = loss;
+        if (counts) { mine.rows += 1; mine.loss += loss != 0.f ? (double)loss * weight : 0.0; }
       }
-    sum += __shfl_xor(sum, 16, 64);
-    own += __shfl_xor(own, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
-    own += __shfl_xor(own, 32, 64);
-    const float loss = counts ? top + logf(sum) - own : 0.f;
-    const float weight = counts && a.row_weight ? a.row_weight[t] : 1.f;
-    if (g == 0) {
-      if (in) a.row_loss[t] = loss;
-      if (counts) { mine.rows += 1; mine.loss += loss != 0.f ? (double)loss * weight : 0.0; }
-    }
-    if (!a.dx) continue;
+      if (!a.dx) continue;
 
-    const float share = weight * inv, r = 1.f / sum;
+      const float share = weight * inv, r = 1.f / sum;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+      for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[ct][j] = counts ? (p[ct][j] * r - (16 * ct + 4 * g + j == y ? 1.f : 0.f)) * share : 0.f;      // d
+        for (int j = 0; j < 4; ++j) p[ct][j] = counts ? (p[ct][j] * r - (16 * ct + 4 * g + j == y ? 1.f : 0.f)) * share : 0.f;      // d
+    } else {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) p[ct] = in ? *reinterpret_cast<const f32x4*>(a.d + (t * CT + ct) * 16 + 4 * g) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if constexpr (PASS == SCORES) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        if (in) *reinterpret_cast<f32x4*>(a.d + (t * CT + ct) * 16 + 4 * g) = p[ct];
+      continue;
+    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<f32x4*>(&turned[wave][ct][i][4 * g]) = p[ct];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -813,7 +831,7 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
           for (int j = 0; j < 4; ++j) o[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], p[ct][j], o[u], 0, 0, 0);
         }
       }
-      const int d = 32 * st + 8 * g;
+      const int d = d0 + 32 * st + 8 * g;
       if (in && d < a.D) {
         if constexpr (!WIDE) {
 #pragma unroll
@@ -843,11 +861,11 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
       for (int ct = 0; ct < CT; ++ct) d[ct] = turned[wave][ct][row][i];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const Few<F32, 4> w = load_few<F32, WIDE, 4>(a.x, from, 64 * c + 4 * i, a.D);
+        const Few<F32, 4> w = load_few<F32, WIDE, 4>(a.x, from, d0 + 64 * c + 4 * i, a.D);
         f32x4 v;
         if constexpr (F32) v = f32x4{w.v[0], w.v[1], w.v[2], w.v[3]};
         else v = f32x4{__uint_as_float(w.v[0] << 16), __uint_as_float(w.v[0] & 0xffff0000u), __uint_as_float(w.v[1] << 16), __uint_as_float(w.v[1] & 0xffff0000u)};
-        if (!has || 64 * c + 4 * i >= a.D) v = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (!has || d0 + 64 * c + 4 * i >= a.D) v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -861,12 +879,12 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
   for (int o = 8; o; o >>= 1) { mine.loss += __shfl_xor(mine.loss, o, 64); mine.rows += __shfl_xor(mine.rows, o, 64); }
   if (lane == 0) sums[wave] = mine;
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (PASS != GRADIENTS && threadIdx.x == 0) {
     RowsPart all = sums[0];
     for (int w = 1; w < 4; ++w) { all.loss += sums[w].loss; all.rows += sums[w].rows; }
     a.parts[blockIdx.x] = all;
   }
-  if (!a.dx) return;
+  if (PASS == SCORES || !a.dx) return;
   for (int w = 0; w < 4; ++w) {                          // the waves' parts of dW in turn, in the place of W
     if (wave == w) {
 #pragma unroll
@@ -882,8 +900,8 @@ __global__ __launch_bounds__(256, CT * NC <= 2 ? 4 : CT == 8 ? 1 : 2) void few_k
     }
     __syncthreads();
   }
-  const int n = a.V * a.D;
-  for (int k = threadIdx.x; k < n; k += 256) a.part[(long)blockIdx.x * n + k] = wk[k / a.D * 64 * NC + k % a.D];
+  const int width = a.D - d0 < 64 * NC ? a.D - d0 : 64 * NC;
+  for (int k = threadIdx.x; k < a.V * width; k += 256) a.part[((long)block * a.V + k / width) * a.D + d0 + k % width] = wk[k / width * 64 * NC + k % width];
 }
 
 __global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ target, long T, long V, uint32_t* __restrict__ counts) { count_rows(target, T, V, blockIdx.x, counts); }
@@ -1092,53 +1110,88 @@ int gradients(GradJob x, GradJob w, float* part, size_t part_bytes, hipStream_t 
 // hold x^T, scores and d in memory, bfloat16 / float32: 2^20 rows x 64, 5 classes 87 / 137 us and 443 / 1289 (60 / 118 at a copy's rate); at its largest
 // sizes, 2^16 x 512, 16 classes 57 / 90 and 98 / 350, x 128, 64 classes 42 / 67 and 58 / 113, x 64, 128 classes 61 / 71 and 65 / 117 (losses alone 20 / 29
 // and 17 / 40); 1000 x 64, 100 classes 20 / 24 and 33 / 47.  Rows that are not aligned are read value by value: 2^20 x 63, 5 classes 217 / 313 and 714 / 1463.
-struct FewPlan { bool fits; int ct, nc, grid, counters; size_t counts, parts, part, total; };
-FewPlan few_plan(long T, long V, long D, bool grad) {
+struct FewPlan { bool fits, two; int ct, nc, grid, slices, blocks, counters, lds; size_t counts, parts, d, part, total; };
+FewPlan few_plan(long T, long V, long D, bool f32, bool grad, bool wide) {
   FewPlan f{};
   f.ct = V <= 16 ? 1 : V <= 32 ? 2 : V <= 64 ? 4 : V <= 96 ? 6 : 8;
   f.nc = D <= 64 ? 1 : D <= 128 ? 2 : D <= 256 ? 4 : 8;
-  f.fits = V <= FEW_CLASSES && D <= FEW_VALUES && f.ct * f.nc * 64 <= FEW_VALUES;
-  if (!f.fits) return f;
-  const long groups = (T + 63) / 64, most = CUS * (f.ct * f.nc <= 2 ? 4 : 2);
-  f.grid = (int)(groups < most ? groups : most);
+  if (V > FEW_CLASSES) return f;
+  const long groups = (T + 63) / 64;
+  if (f.ct * f.nc * 64 <= FEW_VALUES && D <= FEW_VALUES) {
+    const long most = CUS * (f.ct * f.nc <= 2 ? 4 : 2);
+    f.grid = f.blocks = (int)(groups < most ? groups : most);
+    f.slices = 1;
+  } else {
+    // In two passes, with all of W in LDS in one order and d of T rows in memory; in tiles and so, bfloat16 / float32: 2^16 x 1024, 5 classes 193 / 663 and
+    // 99 / 209 us; 8192 x 256, 40 classes 34 / 59 and 29 / 35; 1000 x 1024, 5 classes 34 / 73 and 27 / 34.  bfloat16 with more than 64 classes (8192 x
+    // 256, 100 classes 38 and 44) or unaligned rows (1000 x 777, 20 classes 39 and 54), and its losses alone, stay in tiles.
+    f.lds = f.ct * cdiv(D, 128) * (f32 ? 8192 : 4096);
+    if (f.lds > (128 << 10) || T * f.ct > (1L << 24) || !(f32 || (grad && wide && f.ct <= 4))) return f;
+    f.two = true;
+    f.nc = f.ct == 6 ? 1 : 8 / f.ct;
+    f.slices = cdiv(D, 64 * f.nc);
+    const long one = CUS * (f.lds > (72 << 10) ? 1 : 2), two = 2 * CUS / f.slices;
+    f.grid = (int)(groups < one ? groups : one);
+    f.blocks = (int)(groups < two ? groups : two < 1 ? 1 : two);
+  }
+  f.fits = true;
   f.counters = grad && T > COUNTED ? cdiv(T, COUNTED) : 0;
   f.parts = ((size_t)f.counters * 4 + 255) / 256 * 256;
-  f.part = f.parts + ((size_t)f.grid * sizeof(RowsPart) + 255) / 256 * 256;
-  f.total = f.part + (grad ? (size_t)f.grid * V * D * 4 : 0);
+  f.d = f.parts + ((size_t)f.grid * sizeof(RowsPart) + 255) / 256 * 256;
+  f.part = f.d + (grad && f.two ? (size_t)T * f.ct * 64 : 0);
+  f.total = f.part + (grad ? (size_t)f.blocks * V * D * 4 : 0);
   return f;
 }
-template <bool F32, bool WIDE, int CT, int NC>
-int launch_few(const FewArgs& a, int grid, hipStream_t st) {
-  constexpr int LDS = NC * CT * (F32 ? 8192 : 4096);
-  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(few_kernel<F32, WIDE, CT, NC>), LDS, "dppm_loss_ce"));
-  hipLaunchKernelGGL((few_kernel<F32, WIDE, CT, NC>), dim3(grid), dim3(256), LDS, st, a);
+template <bool F32, bool WIDE, int CT, int NC, FewPass PASS>
+int launch_few(const FewArgs& a, int grid, int lds, hipStream_t st) {
+  DPPM_TRY(lds_limit(reinterpret_cast<const void*>(few_kernel<F32, WIDE, CT, NC, PASS>), lds, "dppm_loss_ce"));
+  hipLaunchKernelGGL((few_kernel<F32, WIDE, CT, NC, PASS>), dim3(grid), dim3(256), lds, st, a);
   return DPPM_OK;
+}
+template <bool F32, bool WIDE, int CT, int NC>
+int one_pass(const FewPlan& f, const FewArgs& a, hipStream_t st) { return launch_few<F32, WIDE, CT, NC, ALL>(a, f.grid, NC * CT * (F32 ? 8192 : 4096), st); }
+template <bool F32, bool WIDE, int CT, int NC>
+int two_passes(const FewPlan& f, const FewArgs& a, hipStream_t st) {
+  DPPM_TRY((launch_few<F32, WIDE, CT, NC, SCORES>(a, f.grid, f.lds, st)));
+  return a.dx ? launch_few<F32, WIDE, CT, NC, GRADIENTS>(a, f.blocks * f.slices, NC * CT * 4096, st) : DPPM_OK;
 }
 template <bool F32, bool WIDE>
 int few_classes(const FewPlan& f, FewArgs a, bool denominator, float* loss, void* dweight, char* ws, hipStream_t st) {
   a.counts = reinterpret_cast<uint32_t*>(ws + f.counts);
   a.parts = reinterpret_cast<RowsPart*>(ws + f.parts);
   a.part = reinterpret_cast<float*>(ws + f.part);
+  a.d = reinterpret_cast<float*>(ws + f.d);
+  a.slices = f.slices;
   a.counters = denominator ? 0 : f.counters;
   if (a.counters) hipLaunchKernelGGL(count_kernel, dim3(a.counters), dim3(256), 0, st, a.target, a.T, (long)a.V, reinterpret_cast<uint32_t*>(ws + f.counts));
-  if (f.ct == 1) {
-    if (f.nc == 1) DPPM_TRY((launch_few<F32, WIDE, 1, 1>(a, f.grid, st)));
-    else if (f.nc == 2) DPPM_TRY((launch_few<F32, WIDE, 1, 2>(a, f.grid, st)));
-    else if (f.nc == 4) DPPM_TRY((launch_few<F32, WIDE, 1, 4>(a, f.grid, st)));
-    else DPPM_TRY((launch_few<F32, WIDE, 1, 8>(a, f.grid, st)));
+  if (f.two) {
+    if constexpr (F32 || WIDE) {
+      if (f.ct == 1) DPPM_TRY((two_passes<F32, WIDE, 1, 8>(f, a, st)));
+      else if (f.ct == 2) DPPM_TRY((two_passes<F32, WIDE, 2, 4>(f, a, st)));
+      else if (f.ct == 4) DPPM_TRY((two_passes<F32, WIDE, 4, 2>(f, a, st)));
+      if constexpr (F32) {
+        if (f.ct == 6) DPPM_TRY((two_passes<F32, WIDE, 6, 1>(f, a, st)));
+        else if (f.ct == 8) DPPM_TRY((two_passes<F32, WIDE, 8, 1>(f, a, st)));
+      }
+    }
+  } else if (f.ct == 1) {
+    if (f.nc == 1) DPPM_TRY((one_pass<F32, WIDE, 1, 1>(f, a, st)));
+    else if (f.nc == 2) DPPM_TRY((one_pass<F32, WIDE, 1, 2>(f, a, st)));
+    else if (f.nc == 4) DPPM_TRY((one_pass<F32, WIDE, 1, 4>(f, a, st)));
+    else DPPM_TRY((one_pass<F32, WIDE, 1, 8>(f, a, st)));
   } else if (f.ct == 2) {
-    if (f.nc == 1) DPPM_TRY((launch_few<F32, WIDE, 2, 1>(a, f.grid, st)));
-    else if (f.nc == 2) DPPM_TRY((launch_few<F32, WIDE, 2, 2>(a, f.grid, st)));
-    else DPPM_TRY((launch_few<F32, WIDE, 2, 4>(a, f.grid, st)));
+    if (f.nc == 1) DPPM_TRY((one_pass<F32, WIDE, 2, 1>(f, a, st)));
+    else if (f.nc == 2) DPPM_TRY((one_pass<F32, WIDE, 2, 2>(f, a, st)));
+    else DPPM_TRY((one_pass<F32, WIDE, 2, 4>(f, a, st)));
   } else if (f.ct == 4) {
-    if (f.nc == 1) DPPM_TRY((launch_few<F32, WIDE, 4, 1>(a, f.grid, st)));
-    else DPPM_TRY((launch_few<F32, WIDE, 4, 2>(a, f.grid, st)));
+    if (f.nc == 1) DPPM_TRY((one_pass<F32, WIDE, 4, 1>(f, a, st)));
+    else DPPM_TRY((one_pass<F32, WIDE, 4, 2>(f, a, st)));
   } else if (f.ct == 6)
-    DPPM_TRY((launch_few<F32, WIDE, 6, 1>(a, f.grid, st)));
+    DPPM_TRY((one_pass<F32, WIDE, 6, 1>(f, a, st)));
   else
-    DPPM_TRY((launch_few<F32, WIDE, 8, 1>(a, f.grid, st)));
+    DPPM_TRY((one_pass<F32, WIDE, 8, 1>(f, a, st)));
   const int n = a.dx ? a.V * a.D : 0;
-  hipLaunchKernelGGL(few_join_kernel, dim3(1 + cdiv(n, 64)), dim3(1024), 0, st, a.part, f.grid, n, dweight, (int)!F32, LossArgs{a.parts, f.grid, a.denom, loss});
+  hipLaunchKernelGGL(few_join_kernel, dim3(1 + cdiv(n, 64)), dim3(1024), 0, st, a.part, f.blocks, n, dweight, (int)!F32, LossArgs{a.parts, f.grid, a.denom, loss});
   return DPPM_OK;
 }
 
@@ -1159,7 +1212,7 @@ using namespace dppm;
 
 extern "C" size_t dppm_loss_ce_workspace_bytes(int64_t T, int64_t V, int64_t D, int bf16, int want_grad) {
   if (!sizes_ok(T, V, D) || T == 0) return 0;
-  const size_t tiles = plan_of(T, V, D, !bf16, want_grad, false).total, few = few_plan(T, V, D, want_grad).total;
+  const size_t tiles = plan_of(T, V, D, !bf16, want_grad, false).total, few = few_plan(T, V, D, !bf16, want_grad, true).total;
   return tiles > few ? tiles : few;      // the largest of the layouts, so that the size does not depend on addresses
 }
 
@@ -1173,11 +1226,11 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
   DPPM_REQUIRE((dx == nullptr) == (dweight == nullptr), "dppm_loss_ce_fwd_bwd: dx and dweight come together");
   DPPM_REQUIRE((uintptr_t)workspace % 16 == 0, "dppm_loss_ce_fwd_bwd: the workspace must be 16-byte aligned");
   const bool grad = dx != nullptr, aligned = ((uintptr_t)x | (uintptr_t)weight) % 16 == 0;
-  const FewPlan few = few_plan(T, V, D, grad);
+  const bool wide = D % 8 == 0 && aligned && (uintptr_t)dx % 16 == 0;
+  const FewPlan few = few_plan(T, V, D, !bf16, grad, wide);
   if (few.fits) {
     DPPM_REQUIRE(workspace_bytes >= few.total, "dppm_loss_ce_fwd_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, few.total);
-    const FewArgs a{x, weight, target, row_weight, nullptr, 0, (long)T, (int)V, (int)D, (float)denom, row_loss, dx, nullptr, nullptr};
-    const bool wide = D % 8 == 0 && aligned && (uintptr_t)dx % 16 == 0;
+    const FewArgs a{x, weight, target, row_weight, nullptr, 0, (long)T, (int)V, (int)D, (float)denom, row_loss, dx, nullptr, nullptr, nullptr, 1};
     const auto run = bf16 ? (wide ? few_classes<false, true> : few_classes<false, false>) : (wide ? few_classes<true, true> : few_classes<true, false>);
     DPPM_TRY(run(few, a, denom > 0, loss_out, dweight, reinterpret_cast<char*>(workspace), as_stream(stream)));
     return check_launch("dppm_loss_ce_fwd_bwd");

@@ -130,7 +130,15 @@ def test_few_classes(ops, T, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("V,D", [(5, 64), (90, 63), (300, 72), (300, 128), (2000, 40)])
+@pytest.mark.parametrize("T,V,D", [(700, 5, 1000), (300, 16, 2048), (300, 16, 2056), (100, 2, 4096), (1000, 30, 600), (2000, 60, 200), (500, 90, 130), (700, 120, 256), (700, 128, 300), (129, 3, 1027),
+                                   (5000, 20, 777), (1, 1, 513), (15, 33, 129), (9001, 7, 520), (40000, 40, 192)])
+def test_few_classes_of_wide_rows(ops, T, V, D, dtype):
+    """few classes in two passes: every number of classes, slices of dims that are whole and not, the first sizes beyond"""
+    test_few_classes(ops, T, V, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,D", [(5, 64), (5, 600), (90, 63), (300, 72), (300, 128), (2000, 40)])
 def test_non_finite_rows_with_and_without_a_class(ops, V, D, dtype):
     x, w, y, rw = make(200, V, D, dtype, 12, missing=0.0)
     clean = ops.loss_ce(x.cuda(), w.cuda(), y.cuda(), rw.cuda(), 200.0)
