@@ -12,7 +12,7 @@
 //    its 11 bits keep 2^-11 of each down to 2^-14 of the maximum and 2^-25 of the maximum below, so that the only rounding of d that counts
 //    is its own -- and in float32 for float32;
 //  * rows: lse, the rows' losses;
-//  * turn: exponentials to n d, rounded once to the operands' type (bfloat16: the own class's entry without loss in dx);
+//  * turn: exponentials to n d, rounded once to the operands' type (bfloat16: the own class's entry without loss in dx, plan_of says why not in dW);
 //  * dx = d W and dW = d^T x: W and d are read transposed from LDS where the contracted dimension is not the contiguous one; x, the smallest,
 //    is transposed in memory, with zeros for rows that have no class.
 // The exponentials held at a time are those of one block of rows, at most 2^30 (bfloat16) or 2^27 (float32) of them: memory does not grow
@@ -1001,8 +1001,11 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
   p.pairs = f32 ? 6 : 1;
   // d of bfloat16 inputs: one bfloat16 plane.  A row's own entry is most of its d, and what it loses would add as much to dx as dx's own rounding
   // does (0.0024 of the gradient in place of 0.0017), so it is held back in float32 and added in dx's epilogue (4099 x 1000, 50001 classes: 1.484 ms
-  // without, 1.498 with it).  In dW it averages out over a class's rows, except where rows are few: there d has two planes (8 rows, 25840
-  // classes: off by 0.0029 with one plane, 0.0016 with two; 47 and 58 us; 100 rows x 512: 78 and 88 us).
+  // without, 1.498 with it).  In dW it stays, as half a step of bfloat16 at most of each entry, the step to which the result itself is rounded: the row
+  // of a class that one row of x has is off by it as a whole, and dW by 0.0020-0.0022 of itself in place of 0.0016-0.0017.  To add it there, the rows of x
+  // have to be found by class in every tile, whose first loads then wait for four dependent ones (the same sizes: 1.38 -> 1.47 ms, 1.62 with half of the
+  // rows in one class; 4000 x 512, 500 classes 50 -> 61 and 81 us).  For few rows d has two planes and both gradients are exact to their own rounding (8
+  // rows, 25840 classes: off by 0.0029 with one plane, 0.0016 with two; 47 and 58 us; 100 rows x 512: 78 and 88 us).
   const bool exact_d = !f32 && T <= 128;
   p.d_planes = f32 ? 3 : exact_d ? 2 : 1;
   p.d_pairs = f32 ? 6 : p.d_planes;
