@@ -28,8 +28,9 @@ def embedding(weight, ids, scale=1.0):
 
 class _ClassLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, target, row_weight, denom):
-        loss, _, dx, dweight = ops.loss_ce(x, weight, target, row_weight, denom, want_grad=any(ctx.needs_input_grad[:2]))
+    def forward(ctx, x, weight, target, row_weight, denom, grad):
+        # needs_input_grad says which inputs require one, also where none are recorded
+        loss, _, dx, dweight = ops.loss_ce(x, weight, target, row_weight, denom, want_grad=grad and any(ctx.needs_input_grad[:2]))
         ctx.save_for_backward(dx, dweight)
         return loss
 
@@ -37,7 +38,7 @@ class _ClassLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         dx, dweight = ctx.saved_tensors
-        return (_times(dx, g) if ctx.needs_input_grad[0] else None, _times(dweight, g) if ctx.needs_input_grad[1] else None, None, None, None)
+        return (_times(dx, g) if ctx.needs_input_grad[0] else None, _times(dweight, g) if ctx.needs_input_grad[1] else None, None, None, None, None)
 
 
 def _times(t, g):
@@ -47,7 +48,8 @@ def _times(t, g):
 
 def loss_func_ce(x, weight, target, row_weight=None, denom=None):
     """Softmax cross entropy of the classes' rows weight [V, D] against the last hidden layer x [..., D] (float32 scalar, differentiable
-    with respect to x and weight): ops.loss_ce over the flattened positions; target [...] int64, outside [0, V): no class."""
+    with respect to x and weight): ops.loss_ce over the flattened positions; target [...] int64, outside [0, V): no class.  The gradients are
+    computed with the loss, and not at all under torch.no_grad() or inference_mode."""
     d = x.shape[-1]
     return _ClassLoss.apply(x.reshape(-1, d).contiguous(), weight.contiguous(), target.reshape(-1).contiguous(),
-                            None if row_weight is None else row_weight.reshape(-1).contiguous(), denom)
+                            None if row_weight is None else row_weight.reshape(-1).contiguous(), denom, torch.is_grad_enabled())
