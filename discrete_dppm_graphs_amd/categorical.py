@@ -49,7 +49,10 @@ def _times(t, g):
 def loss_func_ce(x, weight, target, row_weight=None, denom=None):
     """Softmax cross entropy of the classes' rows weight [V, D] against the last hidden layer x [..., D] (float32 scalar, differentiable
     with respect to x and weight): ops.loss_ce over the flattened positions; target [...] int64, outside [0, V): no class.  The gradients are
-    computed with the loss, and not at all under torch.no_grad() or inference_mode."""
+    computed with the loss, and not at all under torch.no_grad() or inference_mode.  row_weight [...] and denom are constants: a row_weight that
+    requires a gradient is refused where gradients are recorded."""
+    if row_weight is not None and row_weight.requires_grad and torch.is_grad_enabled():
+        raise ValueError("row_weight: requires a gradient, which the class loss does not give; detach it")
     d = x.shape[-1]
     return _ClassLoss.apply(x.reshape(-1, d).contiguous(), weight.contiguous(), target.reshape(-1).contiguous(),
                             None if row_weight is None else row_weight.reshape(-1).contiguous(), denom, torch.is_grad_enabled())

@@ -39,6 +39,18 @@ def test_one_input_that_requires_a_gradient(calls, which):
     assert calls == [True] and [t.grad is not None for t in (x, w)] == [which == 0, which == 1]
 
 
+def test_a_row_weight_that_requires_a_gradient_is_refused(calls):
+    x, w, y = torch.zeros(4, 3, requires_grad=True), torch.zeros(5, 3), torch.zeros(4, dtype=torch.int64)
+    rw = torch.ones(4, requires_grad=True)
+    with pytest.raises(ValueError, match="row_weight"):
+        categorical.loss_func_ce(x, w, y, rw)
+    assert calls == []
+    with torch.no_grad():
+        categorical.loss_func_ce(x, w, y, rw)
+    categorical.loss_func_ce(x, w, y, rw.detach()).backward()
+    assert calls == [False, True]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,V,D", [(600, 2000, 96), (3000, 5, 64)])
 def test_an_evaluated_loss_allocates_no_gradients(T, V, D):
