@@ -15,8 +15,8 @@
 //  * turn: exponentials to n d, rounded once to the operands' type (bfloat16: the own class's entry without loss in dx, plan_of says why not in dW);
 //  * dx = d W and dW = d^T x: W and d are read transposed from LDS where the contracted dimension is not the contiguous one; x, the smallest,
 //    is transposed in memory, with zeros for rows that have no class.
-// The exponentials held at a time are those of one block of rows, at most 2^30 (bfloat16) or 2^27 (float32) of them: memory does not grow
-// with T.  Several blocks add up dW in float32.  Few classes go another way, in one pass (few_kernel).
+// The exponentials held at a time are those of one block of rows, at most 2^30 (bfloat16) or 2^27 (float32) of them -- or 64 rows', where that is
+// more (more than 2^21 float32 classes) --: memory does not grow with T.  Several blocks add up dW in float32.  Few classes go another way, in one pass (few_kernel).
 #include "dppm_common.h"
 #include "dppm_tngemm.h"
 
@@ -1014,10 +1014,10 @@ Plan plan_of(long T, long V, long D, bool f32, bool grad, bool direct) {
   p.Vp = pitch_of(V);
   const long most = grad ? (1L << (f32 ? 27 : 30)) : (1L << 31);     // (row, class) pairs of a block; without gradients only statistics are held
   p.R = T;
-  const long by_pairs = (T * V + most - 1) / most, by_rows = (T + (1L << 22) - 1) >> 22;     // 255 rows of x^T stay within 2^32 bytes
-  const long n = by_pairs > by_rows ? by_pairs : by_rows;
-  if (n > 1) {              // blocks of one size, whole tiles
-    p.R = ((T + n - 1) / n + 255) / 256 * 256;
+  const long fit = most / V < 1L << 22 ? most / V : 1L << 22;        // 255 rows of x^T stay within 2^32 bytes
+  if (T > fit) {            // blocks of one size: whole tiles of rows, or where 256 do not fit, whole steps of 64 of the products over rows
+    const long unit = fit >= 256 ? 256 : 64, largest = fit >= unit ? fit / unit * unit : unit, n = (T + largest - 1) / largest;
+    p.R = ((T + n - 1) / n + unit - 1) / unit * unit;
     if (p.R > T) p.R = T;
   }
   p.blocks = cdiv(T, p.R);
@@ -1284,7 +1284,7 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
       break;
     }
     // a thread's share of the strips is what takes the time: with few rows, more threads a row
-    const int by = rows <= 64 ? 2 : 32, n = cdiv(rows, by);
+    const int by = T <= 64 ? 2 : 32, n = cdiv(rows, by);
     const bool join = grad && b == 0;
     if (by == 2) hipLaunchKernelGGL((rows_kernel<2>), dim3(n + join), dim3(256), 0, st, r, join ? counts : nullptr, p.counters, (float)denom, f(p.inv));
     else hipLaunchKernelGGL((rows_kernel<32>), dim3(n + join), dim3(256), 0, st, r, join ? counts : nullptr, p.counters, (float)denom, f(p.inv));

@@ -294,7 +294,8 @@ int dppm_embedding_wgrad(const void* dout, int dout_bf16, const int64_t* ids, fl
  * (d is rounded to bfloat16 once, from exponentials held in half precision; what a row's own entry loses there is added to dx), sums in
  * float32.  float32: operands split into three bfloat16 pieces, float32-grade products (DPPM_PREC_F32X6), or for few classes (up to 16 of
  * 2048 values ... 128 of 256) products in float32.  The same bits from call to call.  T < 2^30, V <= 2^23, D <= 2^16.
- * workspace: dppm_loss_ce_workspace_bytes(), 16-byte aligned; it holds up to 2^30 exponentials (2^27 for float32) at a time whatever T. */
+ * workspace: dppm_loss_ce_workspace_bytes(), 16-byte aligned; it holds up to 2^30 exponentials (2^27 for float32, or those of 64 rows where
+ * that is more) at a time whatever T. */
 size_t dppm_loss_ce_workspace_bytes(int64_t T, int64_t V, int64_t D, int bf16, int want_grad);
 int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16, const int64_t* target, const float* row_weight, double denom,
                          int64_t T, int64_t V, int64_t D, float* loss_out, float* row_loss, void* dx, void* dweight, void* workspace,
