@@ -312,22 +312,24 @@ template <bool IBF, bool OBF, int VEC>
 __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a, int sum_blocks) {
   if ((int)blockIdx.x >= sum_blocks) {
     __shared__ int absent[FILL_ROWS];
-    const long r0 = (long)((int)blockIdx.x - sum_blocks) * FILL_ROWS;
-    if (threadIdx.x < FILL_ROWS) {
-      const long row = r0 + threadIdx.x;
-      long lo = 0, hi = a.T;
-      while (lo < hi) {
-        const long mid = (lo + hi) >> 1;
-        if ((long)a.key[mid] < row) lo = mid + 1;
-        else hi = mid;
+    for (long r0 = (long)((int)blockIdx.x - sum_blocks) * FILL_ROWS; r0 < a.V; r0 += (long)((int)gridDim.x - sum_blocks) * FILL_ROWS) {
+      if (threadIdx.x < FILL_ROWS) {
+        const long row = r0 + threadIdx.x;
+        long lo = 0, hi = a.T;
+        while (lo < hi) {
+          const long mid = (lo + hi) >> 1;
+          if ((long)a.key[mid] < row) lo = mid + 1;
+          else hi = mid;
+        }
+        absent[threadIdx.x] = row < a.V && !(lo < a.T && (long)a.key[lo] == row);
       }
-      absent[threadIdx.x] = row < a.V && !(lo < a.T && (long)a.key[lo] == row);
+      __syncthreads();
+      constexpr int ES = OBF ? 2 : 4;
+      const int zl = a.D * ES <= 256 ? 8 : 64;      // short rows: eight lanes each
+      for (int r = threadIdx.x / zl; r < FILL_ROWS; r += 256 / zl)
+        if (absent[r]) zero_bytes(reinterpret_cast<char*>(a.dw) + (r0 + r) * a.D * ES, (long)a.D * ES, threadIdx.x & (zl - 1), zl);
+      __syncthreads();
     }
-    __syncthreads();
-    constexpr int ES = OBF ? 2 : 4;
-    const int zl = a.D * ES <= 256 ? 8 : 64;      // short rows: eight lanes each
-    for (int r = threadIdx.x / zl; r < FILL_ROWS; r += 256 / zl)
-      if (absent[r]) zero_bytes(reinterpret_cast<char*>(a.dw) + (r0 + r) * a.D * ES, (long)a.D * ES, threadIdx.x & (zl - 1), zl);
     return;
   }
   const int lanes = 1 << a.lanes_log2;
@@ -384,9 +386,9 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a, int sum_block
 // A run that goes on behind the chunk it began in: its first partial row plus those of the chunks that follow, shared over the groups of
 // a workgroup and added up in a fixed order.
 template <bool OBF, int VEC>
-__global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, long chunks) {
+__global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, long chunks, long first) {      // chunks from `first` on
   const int lanes = 1 << a.lanes_log2, groups = 256 >> a.lanes_log2;
-  const long chunk = blockIdx.x;
+  const long chunk = first + blockIdx.x;
   const uint32_t none = (uint32_t)a.V;
   const long p0 = chunk * a.cp, p1 = p0 + a.cp;
   if (p1 >= a.T) return;
@@ -629,6 +631,8 @@ __global__ __launch_bounds__(256) void embed_zero_kernel(uint16_t* __restrict__ 
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < halves; i += (long)gridDim.x * 256) p[i] = 0;
 }
 
+constexpr long MOST_BLOCKS = 1L << 23;      // of 256 threads: a launch has fewer than 2^32 in a dimension
+
 int log2_ceil(long x) { int l = 0; while ((1L << l) < x) ++l; return l; }
 
 struct Layout { long tile, tiles, chunks; int cp, pitch, passes, bits; size_t key[2], pos[2], hist, part, total; };
@@ -722,9 +726,12 @@ template <bool IBF, bool OBF, int VEC>
 void launch_sums(const SumArgs& s, long chunks, hipStream_t st) {
   const int per_block = 256 >> s.lanes_log2;
   const long sum_blocks = (chunks * s.slices + per_block - 1) / per_block;
-  const long fill = s.accumulate ? 0 : (s.V + FILL_ROWS - 1) / FILL_ROWS;
+  const long groups = (s.V + FILL_ROWS - 1) / FILL_ROWS, fill = s.accumulate ? 0 : groups < MOST_BLOCKS / 4 ? groups : MOST_BLOCKS / 4;
   hipLaunchKernelGGL((embed_sum_kernel<IBF, OBF, VEC>), dim3((unsigned)(sum_blocks + fill)), dim3(256), 0, st, s, (int)sum_blocks);
-  if (chunks > 1) hipLaunchKernelGGL((embed_join_kernel<OBF, VEC>), dim3((unsigned)(chunks - 1), (unsigned)s.slices), dim3(256), 0, st, s, chunks);
+  for (long first = 0; first < chunks - 1; first += MOST_BLOCKS) {
+    const long n = chunks - 1 - first < MOST_BLOCKS ? chunks - 1 - first : MOST_BLOCKS;
+    hipLaunchKernelGGL((embed_join_kernel<OBF, VEC>), dim3((unsigned)n, (unsigned)s.slices), dim3(256), 0, st, s, chunks, first);
+  }
 }
 
 }  // namespace
@@ -746,15 +753,20 @@ extern "C" int dppm_embedding_fwd(const void* weight, int bf16, const int64_t* i
   const bool wide = D % vec == 0 && ((uintptr_t)weight | (uintptr_t)out) % 16 == 0;
   const long per_row = wide ? D / vec : D;
   const int tl = log2_ceil(per_row) < 8 ? log2_ceil(per_row) : 8;
-  const long rows = (256 >> tl) * FWD_ROWS;
-  const dim3 grid((unsigned)((T + rows - 1) / rows)), block(256);
+  const long rows = (256 >> tl) * FWD_ROWS, es = bf16 ? 2 : 4;
   const hipStream_t st = as_stream(stream);
-  if (bf16) {
-    if (wide) hipLaunchKernelGGL((embed_fwd_kernel<true, 8>), grid, block, 0, st, weight, ids, scale, out, (long)T, (long)V, (int)D, tl);
-    else hipLaunchKernelGGL((embed_fwd_kernel<true, 1>), grid, block, 0, st, weight, ids, scale, out, (long)T, (long)V, (int)D, tl);
-  } else {
-    if (wide) hipLaunchKernelGGL((embed_fwd_kernel<false, 4>), grid, block, 0, st, weight, ids, scale, out, (long)T, (long)V, (int)D, tl);
-    else hipLaunchKernelGGL((embed_fwd_kernel<false, 1>), grid, block, 0, st, weight, ids, scale, out, (long)T, (long)V, (int)D, tl);
+  for (long t0 = 0; t0 < T; t0 += rows * MOST_BLOCKS) {
+    const long n = T - t0 < rows * MOST_BLOCKS ? T - t0 : rows * MOST_BLOCKS;
+    const dim3 grid((unsigned)((n + rows - 1) / rows)), block(256);
+    const int64_t* const at = ids + t0;
+    void* const to = reinterpret_cast<char*>(out) + t0 * D * es;
+    if (bf16) {
+      if (wide) hipLaunchKernelGGL((embed_fwd_kernel<true, 8>), grid, block, 0, st, weight, at, scale, to, n, (long)V, (int)D, tl);
+      else hipLaunchKernelGGL((embed_fwd_kernel<true, 1>), grid, block, 0, st, weight, at, scale, to, n, (long)V, (int)D, tl);
+    } else {
+      if (wide) hipLaunchKernelGGL((embed_fwd_kernel<false, 4>), grid, block, 0, st, weight, at, scale, to, n, (long)V, (int)D, tl);
+      else hipLaunchKernelGGL((embed_fwd_kernel<false, 1>), grid, block, 0, st, weight, at, scale, to, n, (long)V, (int)D, tl);
+    }
   }
   return check_launch("dppm_embedding_fwd");
 }
