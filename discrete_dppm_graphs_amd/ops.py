@@ -507,7 +507,8 @@ class TensorSet:
     params: contiguous float32 tensors on one GPU, 16-byte aligned, none overlapping another; grads: one for each, all float32 or all
     bfloat16, same number of values; copies: None, or for each parameter a bfloat16 tensor (or None) that every step writes the new
     parameter to.  weight_decay: one number, or one for each tensor.  state_bits: 32 (float32 moments) or 8 (e4m3 of m and of sqrt(v)
-    with a float32 scale per 256 values).  state: buffers as in self.state to go on from; zeros if None.
+    with a float32 scale per 256 values).  state: buffers as in self.state to go on from (16-byte aligned, 8-bit ones and their scales 4); zeros
+    if None.
     The set keeps its tensors alive; set_grads() points it at other gradients.  Moments of tensor i lie at self.offsets[i] of the flat
     buffers (offsets are multiples of 256 values)."""
 
@@ -571,6 +572,8 @@ class TensorSet:
         for k, (s, t) in want.items():
             if _chk(given[k], f"state[{k!r}]", (s,), t).device != self.device:
                 raise ValueError(f"state[{k!r}]: on {given[k].device}, the parameters on {self.device}")
+            if given[k].data_ptr() % (16 if self.state_bits == 32 else 4):      # four moments at a time; four codes, one scale
+                raise ValueError(f"state[{k!r}]: not aligned to {16 if self.state_bits == 32 else 4} bytes")
         return dict(given)
 
     def _refuse_shared(self, grads):
