@@ -98,6 +98,12 @@ __device__ __forceinline__ uint32_t magnitude_max(uint32_t v, float x) {
   return v > b ? v : b;
 }
 
+// v_sqrt_f32 takes denormal operands as zero, which with eps = 0 would divide by it
+__device__ __forceinline__ float fast_root(float v) {
+  const bool tiny = v < 0x1p-126f;
+  return __builtin_amdgcn_sqrtf(tiny ? v * 0x1p64f : v) * (tiny ? 0x1p-32f : 1.f);
+}
+
 // four values from `at` on; FULL: all of them lie before the tensor's end, n values long
 template <bool BF, bool FULL>
 __device__ __forceinline__ void load4(const void* src, long at, long n, float (&out)[4]) {
@@ -232,8 +238,8 @@ __device__ __forceinline__ void adamw_chunk(const dppm_tensor_entry& e, long bas
       m[i][k] = m[i][k] + (gg - m[i][k]) * a.one_minus_b1;
       v[i][k] = v[i][k] * a.b2 + a.one_minus_b2 * gg * gg;
       // the hardware's root and reciprocal are off by one unit in the last place: enough for the update, which is small against p.  A root
-      // that is stored is rounded correctly.  (eps = 0: v' is 0 or over 2^-149, so that the denominator is 0 or far from the denormals.)
-      root[k] = BITS == 8 ? sqrtf(v[i][k]) : __builtin_amdgcn_sqrtf(v[i][k]);
+      // that is stored is rounded correctly.  (eps = 0: v' is 0 or at least 2^-149, so that the denominator is 0 or far from the denormals.)
+      root[k] = BITS == 8 ? sqrtf(v[i][k]) : fast_root(v[i][k]);
       p[i][k] = p[i][k] * decay - a.step_size * (m[i][k] * __builtin_amdgcn_rcpf(root[k] * a.bc2_rsqrt + a.eps));
     }
     if (BITS == 8) {

@@ -1,4 +1,4 @@
-"""ops.TensorSet and ops.adamw_step at the edges of what they take: state buffers that are not aligned."""
+"""ops.TensorSet and ops.adamw_step at the edges of what they take: state buffers that are not aligned, gradients whose squares are denormal."""
 import numpy as np
 import pytest
 import torch
@@ -34,3 +34,17 @@ def test_state_buffers_that_are_not_aligned_are_refused(ops, bits):
     for params, held in ((p, state), (q, four)):        # one of 4 codes, 4 floats, one scale is aligned enough
         ops.adamw_step(ops.TensorSet([params], [g], state_bits=bits, state=held), 1e-2, 0.9, 0.999, 1e-8, 1)
     assert torch.equal(p, q) and all(torch.equal(state[k].view(torch.uint8), four[k].view(torch.uint8)) for k in state)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+def test_gradients_whose_squares_are_denormal(ops, bits, eps):
+    """v' = (1 - beta2) g^2 from 1e-43 on, against float64.  (1 - beta2) g is rounded, then its product with g, off by half of 2^-149 there:
+    |dv| <= 4 u v + 2^-150, so the root by half of that relative to v; the rest of the update by 32 u, and 8 u where 1 - beta is rounded."""
+    g = np.geomspace(1e-20, 1e-14, 256).astype(np.float32)
+    p = torch.zeros(256, device="cuda")
+    ops.adamw_step(ops.TensorSet([p], [torch.as_tensor(g).cuda()], state_bits=bits), 1e-3, 0.9, 0.999, eps, 1)
+    g = g.astype(np.float64)
+    want = -1e-3 * g / (g + eps)
+    v = 0.001 * g * g
+    assert (np.abs(p.double().cpu().numpy() - want) <= np.abs(want) * ((4 * U * v + 2.0 ** -150) / v + 40 * U)).all()
