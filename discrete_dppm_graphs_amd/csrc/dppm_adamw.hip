@@ -189,7 +189,8 @@ __device__ __forceinline__ NormOut clip_of(const double* part, int n, double gsc
   const double norm = sqrt((w[0] + w[1]) + (w[2] + w[3])) * fabs(gscale);
   const double coef = max_norm / (norm + 1e-6);
   if (norm_out && threadIdx.x == 0) *norm_out = (float)norm;
-  return NormOut{(float)(gscale * (coef < 1.0 ? coef : 1.0)), norm <= 1.7e308};     // not ok for infinity and NaN: the step leaves everything as it was
+  // not ok where the caller reads infinity (a float32) or NaN: the step leaves everything as it was
+  return NormOut{(float)(gscale * (coef < 1.0 ? coef : 1.0)), (float)norm <= 3.402823466e38f};
 }
 
 __global__ __launch_bounds__(256) void grad_norm_kernel(const double* __restrict__ part, int n, double gscale, double max_norm, float* __restrict__ norm_out,

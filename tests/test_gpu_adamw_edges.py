@@ -1,4 +1,5 @@
-"""ops.TensorSet and ops.adamw_step at the edges of what they take: state buffers that are not aligned, gradients whose squares are denormal."""
+"""ops.TensorSet and ops.adamw_step at the edges of what they take: state buffers that are not aligned, gradients whose squares are
+denormal, norms that float32 cannot hold."""
 import numpy as np
 import pytest
 import torch
@@ -48,3 +49,15 @@ def test_gradients_whose_squares_are_denormal(ops, bits, eps):
     want = -1e-3 * g / (g + eps)
     v = 0.001 * g * g
     assert (np.abs(p.double().cpu().numpy() - want) <= np.abs(want) * ((4 * U * v + 2.0 ** -150) / v + 40 * U)).all()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("n,most,fits", [(2, 2.0 ** 127, True), (8, 2.0 ** 127, False), (3_000_000, 2.0 ** 125, False)])
+def test_a_norm_that_float32_cannot_hold_is_infinite(ops, bits, n, most, fits):
+    """finite gradients: their norm sqrt(n) most is returned, and the step made, while it is under 2^128; else it is infinite and nothing changes"""
+    p, g = torch.ones(n, device="cuda"), torch.full((n,), most, device="cuda")
+    tset = ops.TensorSet([p], [g], state_bits=bits)
+    norm = ops.adamw_step(tset, 1e-2, 0.9, 0.999, 1e-8, 1, max_norm=1.0)
+    assert (p != 1).all() if fits else (p == 1).all()
+    assert all((v.view(torch.uint8) != 0).any().item() == fits for v in tset.state.values())
+    assert abs(norm.item() / (n ** 0.5 * most) - 1) <= U if fits else norm.item() == float("inf")
