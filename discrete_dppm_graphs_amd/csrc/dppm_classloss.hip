@@ -476,7 +476,8 @@ struct GradOut {
   const float* add;           // float32 [N][ldc] that is added first, or null
   float* part; long part_stride;   // with splits: float32 [splits][N][ldc] instead
   const float* scale;         // what the products are multiplied with
-  const float* residual; const int64_t* target;    // dx, one plane of d: += residual[n] * A's row of target[n]; or null
+  const int64_t* target;                 // dx: the rows' classes
+  const float* residual;                 // dx, one plane of d: += residual[n] * A's row of target[n]; or null
   int c_bf16, past, wide;     // past: c is larger than the caches; wide: rows of c start on 16 bytes and M is a multiple of 8
 };
 
@@ -530,9 +531,16 @@ __device__ __forceinline__ void grad_tile(const TnArgs& g, const GradOut& o, cha
   }
   const float scale = *o.scale;
 #pragma unroll
-  for (int i = 0; i < T::MI; ++i)
+  for (int j = 0; j < T::NI; ++j) {
+    bool has = true;
+    if (TRA) {      // a row without a class has zeros in d, and in dx also where the table holds infinity or NaN
+      const int n = n0 + (wave / T::WGM) * T::WN + 16 * j + (lane & 15);
+      const int64_t y = o.target[n < g.N ? n : g.N - 1];
+      has = y >= 0 && y < g.K;
+    }
 #pragma unroll
-    for (int j = 0; j < T::NI; ++j) acc[i][j] *= scale;
+    for (int i = 0; i < T::MI; ++i) acc[i][j] = has ? acc[i][j] * scale : tn_acc{0.f, 0.f, 0.f, 0.f};
+  }
   const int ms = m0 + (wave % T::WGM) * T::WM, ns = n0 + (wave / T::WGM) * T::WN;
   if (o.c_bf16 && o.wide && !o.part && !o.add) {
 #pragma unroll
@@ -832,6 +840,7 @@ __global__ __launch_bounds__(256, PASS == SCORES ? 2 : CT * NC <= 2 ? 4 : CT == 
         }
       }
       const int d = d0 + 32 * st + 8 * g;
+      if (!counts) o[0] = o[1] = f32x4{0.f, 0.f, 0.f, 0.f};      // also where the table holds infinity or NaN
       if (in && d < a.D) {
         if constexpr (!WIDE) {
 #pragma unroll
@@ -1322,7 +1331,8 @@ extern "C" int dppm_loss_ce_fwd_bwd(const void* x, const void* weight, int bf16,
     gw.K = whole; gw.ksteps = cdiv(rows, 64); gw.pairs = p.d_pairs;      // d has zeros to whole steps
     float* total = p.blocks == 1 ? nullptr : (p.f32 ? reinterpret_cast<float*>(dweight) : f(p.dw));
     GradJob jx = grad_job(gx, reinterpret_cast<char*>(dx) + t0 * D * es, bf16, f(p.inv));
-    if (p.d_planes == 1) { jx.o.residual = f(p.residual); jx.o.target = target + t0; }
+    jx.o.target = target + t0;
+    if (p.d_planes == 1) jx.o.residual = f(p.residual);
     GradJob jw = grad_job(gw, last || p.f32 ? dweight : (void*)total, bf16 && last, f(p.inv));
     jw.o.add = b == 0 ? nullptr : total;
     DPPM_TRY(gradients(jx, jw, f(p.part), p.part_bytes, st));
