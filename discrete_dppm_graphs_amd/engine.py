@@ -131,7 +131,8 @@ class FlatState:
         if 'names' in sd and list(sd['names']) != list(self.names):
             raise ValueError("FlatState.load_state_dict: parameter names differ from this model's")
         for k, m in moments.items():
-            if sd[k].numel() != m.numel() or sd[k].dtype != m.dtype:
+            codes = torch.float8_e4m3fn in (m.dtype, sd[k].dtype)      # 8-bit codes mean something with their scales alone; other types are converted
+            if sd[k].numel() != m.numel() or (codes and sd[k].dtype != m.dtype):
                 raise ValueError("FlatState.load_state_dict: moment size %d (%s) != %d (%s)" % (sd[k].numel(), sd[k].dtype, m.numel(), m.dtype))
         for k, m in moments.items():
             m.copy_(sd[k].to(m.device))
