@@ -286,9 +286,10 @@ __device__ __forceinline__ void adamw_chunk(const dppm_tensor_entry& e, long bas
   }
 }
 
-// clip: what grad_norm_kernel left; or null, and with parts > 0 every workgroup sums the few partial sums itself, which spares the launch
+// clip: what grad_norm_kernel left; or null, and with parts > 0 every workgroup sums the few partial sums itself, which spares the launch.  Clipped
+// float32 steps with the launch and without it, in us: 512 chunks 14.0 / 11.4, 600 17.8 / 16.0, 1024 25.4 / 23.1, 2048 47.0 / 43.7, 4096 84.8 / 86.2.
 struct Clip { const NormOut* clip; const double* part; int parts; double gscale, max_norm; float* norm_out; };
-constexpr int FEW_PARTS = 256;
+constexpr int FEW_PARTS = 1024;
 
 template <bool GBF, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(const dppm_tensor_entry* __restrict__ tab, const int2* __restrict__ chunks, Clip clip, StepArgs a) {

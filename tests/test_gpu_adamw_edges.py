@@ -61,3 +61,19 @@ def test_a_norm_that_float32_cannot_hold_is_infinite(ops, bits, n, most, fits):
     assert (p != 1).all() if fits else (p == 1).all()
     assert all((v.view(torch.uint8) != 0).any().item() == fits for v in tset.state.values())
     assert abs(norm.item() / (n ** 0.5 * most) - 1) <= U if fits else norm.item() == float("inf")
+
+
+@pytest.mark.parametrize("chunks", [1, 512, 513, 2047, 2048, 2049, 5000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norms_by_either_number_of_launches(ops, chunks, dtype):
+    """summed in float64 and rounded once to float32; the clipped step is the unclipped one of the scaled gradients, whose factor is rounded (4 u
+    of m' and root each side, 40 u of an update of at most lr)"""
+    n = chunks * 4096 - 3
+    g = torch.Generator(device="cuda").manual_seed(chunks)
+    grad = torch.randn(n, generator=g, device="cuda").to(dtype)
+    norm = grad.double().square().sum().sqrt().item()
+    p, q = torch.ones(n, device="cuda"), torch.ones(n, device="cuda")
+    got = ops.adamw_step(ops.TensorSet([p], [grad]), 1e-2, 0.9, 0.999, 1e-3, 1, max_norm=0.5 * norm)
+    ops.adamw_step(ops.TensorSet([q], [grad]), 1e-2, 0.9, 0.999, 1e-3, 1, grad_scale=0.5 * norm / (norm + 1e-6))
+    assert abs(got.item() - norm) <= 2 * U * norm
+    assert (p - q).abs().max().item() <= 40 * U * 1e-2 + 2 * U
