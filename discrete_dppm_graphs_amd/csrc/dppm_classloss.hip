@@ -454,8 +454,8 @@ __device__ __forceinline__ void lay_out_tile(const LayOut& a, int id) {
     }
 }
 
-// Everything that can be laid out before the products, in one launch: `first` workgroups for a, `second` for b, and one more that leaves
-// 1 / n in inv (null: not wanted).
+// Everything that can be laid out before the products, in one launch: `first` workgroups for a, `second` for b, and the rest count the rows that have a
+// class, COUNTED rows each (rows_kernel puts the counts together).
 template <bool F32>
 __global__ __launch_bounds__(256) void prepare_kernel(LayOut a, int first, LayOut b, int second, const int64_t* __restrict__ target, long T, long V,
                                                       uint32_t* __restrict__ counts) {
@@ -572,7 +572,6 @@ __device__ __forceinline__ void grad_tile(const TnArgs& g, const GradOut& o, cha
     });
 }
 
-// the parts of a split product, in order, and what was there before
 // Both gradients in one launch: few tiles of one leave room for the other's, and the last round of tiles is one and not two (the whole loss, bfloat16:
 // 300 x 64, 100 classes 35.8 -> 28.8 us, 1000 x 256, 5000 classes 70 -> 57, 4099 x 1000, 50001 classes 1510 -> 1419).  The product with the
 // longer tiles comes first.
@@ -586,6 +585,7 @@ __global__ __launch_bounds__(T::NT) void grad_kernel(GradJob x, GradJob w, int f
   else grad_tile<T, true, false>(x.g, x.o, lds, id);
 }
 
+// The parts of a split product, in order, behind what was there before.
 struct PartsJob { const float* part; long n; int splits; const float* add; void* c; int c_bf16; };
 __global__ __launch_bounds__(256) void parts_kernel(PartsJob x, PartsJob w, int first) {
   const bool early = (int)blockIdx.x < first;

@@ -9,7 +9,8 @@
 // lane, no registers) into a ring of stages, all but one of them ahead of the one that is multiplied.  A row of a stage is 128 bytes = one line
 // = 8 chunks of 16; chunk c of row r lies in slot c ^ g, g = q ^ ((q >> 1 ^ q >> 2) & 1), q = (r >> 1) & 7: a 16-byte LDS read is served 16 lanes at
 // a time, lanes 0-3, 12-15 and 20-27 together (then the others), that is rows 0-3 and 12-15 of one chunk with rows 4-11 of the next, and this
-// way they fall on all banks (SQ_LDS_BANK_CONFLICT 0; with g = r & 7 half of the LDS time was conflicts).  The DMA writes lanes side by side, so
+// way they fall on all banks (SQ_LDS_BANK_CONFLICT 0 in both kernels for float32, 2047 x 512 against 20011 classes; for bfloat16 1-9 % of the LDS cycles,
+// all of it of tn_rows16; with g = r & 7 half of the LDS time was conflicts).  The DMA writes lanes side by side, so
 // the swizzle is made on the global side: a lane fetches the chunk whose slot it fills.
 //
 // An operand that is contiguous in m lies in a stage as it comes, 64 rows of k with BM values, and its fragments are read by
