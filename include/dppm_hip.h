@@ -314,8 +314,9 @@ typedef struct dppm_tensor_entry {
 } dppm_tensor_entry;
 
 /* One AdamW step (decoupled weight decay, bias correction with `step` starting at 1) over all tensors of `table`, in one launch, or with
- * max_norm > 0 in two (three with more than 2048 chunks): then the gradients' norm over all tensors (of grad * grad_scale) goes to *norm_out, the gradients are scaled
- * by min(1, max_norm / (norm + 1e-6)), and a step whose norm is infinite (as a float32) or NaN changes nothing.
+ * max_norm > 0 in two (three with more than 2048 chunks): then the gradients' norm over all tensors (of grad * grad_scale) goes to
+ * *norm_out, the gradients are scaled by min(1, max_norm / (norm + 1e-6)), and a step whose norm is infinite (as a float32) or NaN changes
+ * nothing.
  * chunks: DEVICE array [n_chunks][2] of (index in table, chunk in that tensor), one pair for each dppm_adamw_chunk() values begun of
  * every tensor.  state_bits 8 or 32; 8-bit moments are rounded stochastically from Philox4x32-10 with key = seed and counter =
  * (g, tensor, g >> 32, step), g = index / 4: the same call gives the same bits, and a captured call replays the step number and the
